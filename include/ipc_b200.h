@@ -309,6 +309,69 @@ typedef struct ipc_optim {
 int ipc_weight_update_opt(void* w, const void* e, const void* x_up, int M, int K, int B, int groups,
                           const ipc_optim_t* opt, int recompute, int act, int dtype, int algo, void* workspace,
                           size_t workspace_bytes, void* stream);
+/* ---------------------------------------------------------------------------
+ * Microscaled operands: blocks of 32 numbers that share one power of two.
+ *
+ * A block whose largest magnitude is m is kept as a scale byte s + 127 and 32
+ * codes c; each number reads back as c * 2^s.
+ *   8 bits: s is the smallest integer >= -127 with m <= 127 * 2^s; c is the
+ *           integer nearest to v * 2^-s (ties to even).
+ *   4 bits: s is the smallest integer >= -127 with m <= 6 * 2^s; c is the
+ *           nearest of +-{0, 0.5, 1, 1.5, 2, 3, 4, 6} (ties to the even code; bit 3
+ *           of a code is the sign, bits 0-2 the place in this list).
+ * A block that holds an infinity or a NaN is kept as codes 0 with the scale
+ * byte 255 and reads back as NaN.
+ *
+ * 8-bit checkpoint of states x [D, B], blocks along the batch:
+ *   codes  [D, 32 ceil(B/32)] int8 (16-byte aligned; padding is 0)
+ *   scales [ceil(B/32), D] bytes
+ * 4-bit operand of R rows and K columns, blocks along the columns, which a
+ * product sums over; Kp = 128 ceil(K/128):
+ *   codes  [R, Kp/2] bytes (16-byte aligned), the lower column in the lower
+ *          four bits; padding is 0
+ *   scales [ceil(R/128), Kp/128, 32, 4, 4] bytes (16-byte aligned): row r, block j at
+ *          [r/128, j/4, r%32, r%128/32, j%4]; padding is 0
+ * No reference counterpart: the reference keeps and multiplies fp16 only.
+ * --------------------------------------------------------------------------- */
+/* codes, scales = the 8-bit checkpoint of x [D, B]. */
+int ipc_mx8_store(const void* x, signed char* codes, unsigned char* scales, int D, int B, int dtype, void* stream);
+/* out [D, B] = cast(f(x^)), x^ the states a checkpoint stands for. */
+int ipc_mx8_restore(const signed char* codes, const unsigned char* scales, void* out, int D, int B, int act, int dtype,
+                    void* stream);
+/*
+ * Weight update from a checkpoint of x_up [K, B], A = cast(f(x^)), e [M, B]:
+ *   IPC_MODE_WEIGHT  W = cast(W + scale * E @ A^T)          (out = W [M, K], in/out)
+ *   IPC_MODE_WDELTA  dw = scale * E @ A^T in fp32; IPC_FLAG_ACCUMULATE adds into dw
+ *   IPC_MODE_WGRAD   out = cast(scale * E @ A^T) in `dtype`
+ * The workspace (16-byte aligned; ipc_mx8_weight_ws_bytes gives its size) follows
+ * the rules of ipc_fused_gemm_ws.  IPC_ALGO_OUTER is IPC_ERR_ARG.
+ */
+#define IPC_MODE_WGRAD 6
+int ipc_mx8_weight(int mode, void* out, const void* e, const signed char* codes, const unsigned char* scales, int M,
+                   int K, int B, float scale, int flags, int act, int dtype, int algo, void* workspace,
+                   size_t workspace_bytes, void* stream);
+int ipc_mx8_weight_ws_bytes(int mode, int M, int K, int B, int dtype, int algo, size_t* bytes);
+/*
+ * Error of the layer above from its checkpoint (backpropagation through
+ * mu = W f(x_up)):  e_up [K, B] = cast(f'(x^) * (W^T @ E)), w [M, K], e [M, B].
+ */
+int ipc_mx8_backward(void* e_up, const void* w, const void* e, const signed char* codes, const unsigned char* scales,
+                     int M, int K, int B, int act, int dtype, int algo, void* stream);
+/*
+ * codes, scales = the 4-bit operand of f(x) (f in fp32, not rounded before it
+ * is stored): turned == 0 takes x [R, K] (weights), turned != 0 x [K, R]
+ * (feature-major states of R samples).
+ */
+int ipc_mxfp4_quantize(const void* x, unsigned char* codes, unsigned char* scales, int R, int K, int turned, int act,
+                       int dtype, void* stream);
+/* out [R, K] = cast of the values a 4-bit operand stands for (exact in bf16 and fp32). */
+int ipc_mxfp4_restore(const unsigned char* codes, const unsigned char* scales, void* out, int R, int K, int dtype,
+                      void* stream);
+/* out [M, B] = cast(W4 @ A4^T): W4 a 4-bit operand of M rows, A4 one of B rows (samples), both of K columns;
+ * products are exact, sums in fp32. */
+int ipc_mxfp4_forward(const unsigned char* w, const unsigned char* w_scales, const unsigned char* a,
+                      const unsigned char* a_scales, void* out, int M, int K, int B, int dtype, void* stream);
+
 /* First error a device-side bounded wait recorded since the last clear
  * (IPC_OK if none; IPC_ERR_TIMEOUT when a pipeline wait gave up).  Synchronises
  * with the device; clear != 0 resets the word.  No reference counterpart. */

@@ -29,6 +29,7 @@ DTYPE_NAMES = {"float32": torch.float32, "float16": torch.float16, "bfloat16": t
 ALGO_CODES = {"auto": 0, "simt": 1, "generic": 1, "tcgen05": 2, "outer": 3}
 
 MODE_PRED, MODE_INFER, MODE_WEIGHT, MODE_WDELTA, MODE_FORWARD = 0, 1, 2, 3, 4
+MODE_WGRAD = 6
 FLAG_ACTIVATE_B, FLAG_AOUT_STORED, FLAG_ACCUMULATE, FLAG_MULTIMEM_RED = 1, 2, 4, 8
 
 # Split-K scratch that covers every shape the weight update splits: a split happens only with fewer
@@ -47,6 +48,8 @@ EXPORTED = (
     "ipc_activate", "ipc_net_train", "ipc_net_plan", "ipc_fused_gemm", "ipc_device_status",
     "ipc_fused_gemm_ws", "ipc_weight_update_noalloc", "ipc_selftest_barrier_timeout", "ipc_set_max_ctas",
     "ipc_fused_gemm_ws_bytes", "ipc_fused_gemm_tuned", "ipc_weight_update_opt", "ipc_count_correct",
+    "ipc_mx8_store", "ipc_mx8_restore", "ipc_mx8_weight", "ipc_mx8_weight_ws_bytes", "ipc_mx8_backward",
+    "ipc_mxfp4_quantize", "ipc_mxfp4_restore", "ipc_mxfp4_forward",
 )
 
 
@@ -144,6 +147,14 @@ def load() -> ctypes.CDLL:
                                      POINTER(IpcGemmTune), vp]),
         "ipc_weight_update_opt": (i, [vp, vp, vp, i, i, i, i, POINTER(IpcOptim), i, i, i, i, vp, c_size_t, vp]),
         "ipc_count_correct": (i, [vp, i, i, vp, vp, i, vp]),
+        "ipc_mx8_store": (i, [vp, vp, vp, i, i, i, vp]),
+        "ipc_mx8_restore": (i, [vp, vp, vp, i, i, i, i, vp]),
+        "ipc_mx8_weight": (i, [i, vp, vp, vp, vp, i, i, i, f, i, i, i, i, vp, c_size_t, vp]),
+        "ipc_mx8_weight_ws_bytes": (i, [i, i, i, i, i, i, POINTER(c_size_t)]),
+        "ipc_mx8_backward": (i, [vp, vp, vp, vp, vp, i, i, i, i, i, i, vp]),
+        "ipc_mxfp4_quantize": (i, [vp, vp, vp, i, i, i, i, i, vp]),
+        "ipc_mxfp4_restore": (i, [vp, vp, vp, i, i, i, vp]),
+        "ipc_mxfp4_forward": (i, [vp, vp, vp, vp, vp, i, i, i, i, vp]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)

@@ -9,6 +9,7 @@
 #include "ipc_common.cuh"
 #include "ipc_elementwise.cuh"
 #include "ipc_generic.cuh"
+#include "ipc_mx.cuh"
 #include "ipc_tc.cuh"
 
 namespace ipc {
@@ -420,6 +421,132 @@ int ipc_fused_gemm_ws(int mode, const void* a, const void* b, void* out, const v
   IPC_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "workspace must be 16-byte aligned");
   return fused_gemm_impl(mode, a, b, out, aux, aux2, M, K, B, groups, scale, flags, act, dtype, algo,
                          static_cast<float*>(workspace), workspace_bytes, stream);
+}
+
+// ------------------------------------------------------------- microscaled operands (ipc_mx.cuh)
+static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+int ipc_mx8_store(const void* x, signed char* codes, unsigned char* scales, int D, int B, int dtype, void* stream) {
+  int rc = common_checks(D, 1, B, 1, IPC_ACT_IDENTITY, dtype, IPC_ALGO_AUTO);
+  if (rc) return rc;
+  if (D == 0 || B == 0) return IPC_OK;
+  IPC_REQUIRE(x && codes && scales, "null operand pointer");
+  IPC_REQUIRE(aligned16(codes), "checkpoint codes must be 16-byte aligned");
+  return launch_mx8_store(x, codes, scales, D, B, dtype, reinterpret_cast<cudaStream_t>(stream));
+}
+
+int ipc_mx8_restore(const signed char* codes, const unsigned char* scales, void* out, int D, int B, int act, int dtype,
+                    void* stream) {
+  int rc = common_checks(D, 1, B, 1, act, dtype, IPC_ALGO_AUTO);
+  if (rc) return rc;
+  if (D == 0 || B == 0) return IPC_OK;
+  IPC_REQUIRE(codes && scales && out, "null operand pointer");
+  IPC_REQUIRE(aligned16(codes), "checkpoint codes must be 16-byte aligned");
+  return launch_mx8_restore(codes, scales, out, D, B, B, B, act, dtype, reinterpret_cast<cudaStream_t>(stream));
+}
+
+// f(x) of a checkpoint read back into the head of the workspace (a multiple of 256 bytes)
+static size_t mx8_values_bytes(int K, int B, int dtype) {
+  return ((size_t)K * B * dt_size(dtype) + 255) / 256 * 256;
+}
+
+int ipc_mx8_weight_ws_bytes(int mode, int M, int K, int B, int dtype, int algo, size_t* bytes) {
+  int rc = common_checks(M, K, B, 1, IPC_ACT_IDENTITY, dtype, algo);
+  if (rc) return rc;
+  IPC_REQUIRE(mode == IPC_MODE_WEIGHT || mode == IPC_MODE_WDELTA || mode == IPC_MODE_WGRAD, "not a weight mode: %d", mode);
+  IPC_REQUIRE(bytes != nullptr, "null result pointer");
+  *bytes = mx8_values_bytes(K, B, dtype);
+  if (B > 16 && tc_eligible(mode, M, K, B, dtype, algo, false, true)) *bytes += IPC_SPLITK_WS_BYTES;
+  return IPC_OK;
+}
+
+int ipc_mx8_weight(int mode, void* out, const void* e, const signed char* codes, const unsigned char* scales, int M,
+                   int K, int B, float scale, int flags, int act, int dtype, int algo, void* workspace,
+                   size_t workspace_bytes, void* stream) {
+  int rc = common_checks(M, K, B, 1, act, dtype, algo);
+  if (rc) return rc;
+  IPC_REQUIRE(mode == IPC_MODE_WEIGHT || mode == IPC_MODE_WDELTA || mode == IPC_MODE_WGRAD, "not a weight mode: %d", mode);
+  IPC_REQUIRE((flags & ~IPC_FLAG_ACCUMULATE) == 0, "only IPC_FLAG_ACCUMULATE applies (flags = %d)", flags);
+  IPC_REQUIRE(mode == IPC_MODE_WDELTA || !(flags & IPC_FLAG_ACCUMULATE), "IPC_FLAG_ACCUMULATE applies to IPC_MODE_WDELTA only");
+  IPC_REQUIRE(algo != IPC_ALGO_OUTER, "IPC_ALGO_OUTER does not read checkpoints");
+  if (M == 0 || K == 0) return IPC_OK;
+  IPC_REQUIRE(out && (B == 0 || (e && codes && scales)), "null operand pointer");
+  IPC_REQUIRE(aligned16(codes), "checkpoint codes must be 16-byte aligned");
+  const size_t need = mx8_values_bytes(K, B, dtype);
+  IPC_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), "workspace of %lld bytes, %lld needed (ipc_mx8_weight_ws_bytes)",
+              (long long)workspace_bytes, (long long)need);
+  IPC_REQUIRE(aligned16(workspace), "workspace must be 16-byte aligned");
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (B > 0) {
+    rc = launch_mx8_restore(codes, scales, workspace, K, B, B, B, act, dtype, s);
+    if (rc) return rc;
+  }
+  GemmArgs p{};
+  p.A = e; p.lda = B; p.gsA = (long long)M * B;
+  p.Bm = workspace; p.ldb = B; p.gsB = (long long)K * B;
+  p.Mg = M; p.Ng = K; p.Kg = B; p.groups = 1;
+  p.out = out; p.gsOut = (long long)M * K;
+  p.scale = scale;
+  p.accumulate = (flags & IPC_FLAG_ACCUMULATE) != 0;
+  const size_t rest = workspace_bytes - need;
+  if (B > 16 && tc_eligible(mode, M, K, B, dtype, algo, false, rest > 0))
+    return launch_tc(p, mode, act, dtype, s, rest ? reinterpret_cast<float*>(static_cast<char*>(workspace) + need) : nullptr, rest);
+  if (algo == IPC_ALGO_TCGEN05)
+    return set_error(IPC_ERR_UNSUPPORTED, "tcgen05 path: not eligible (M=%d K=%d B=%d dtype=%d)", M, K, B, dtype);
+  return launch_generic(p, mode, false, act, dtype, s);
+}
+
+int ipc_mx8_backward(void* e_up, const void* w, const void* e, const signed char* codes, const unsigned char* scales,
+                     int M, int K, int B, int act, int dtype, int algo, void* stream) {
+  int rc = common_checks(M, K, B, 1, act, dtype, algo);
+  if (rc) return rc;
+  IPC_REQUIRE(algo != IPC_ALGO_OUTER, "IPC_ALGO_OUTER applies to the weight update only");
+  if (K == 0 || B == 0) return IPC_OK;
+  IPC_REQUIRE(e_up && codes && scales && (M == 0 || (w && e)), "null operand pointer");
+  IPC_REQUIRE(aligned16(codes), "checkpoint codes must be 16-byte aligned");
+  GemmArgs p{};
+  p.A = w; p.lda = K; p.gsA = (long long)M * K;
+  p.Bm = e; p.ldb = B; p.gsB = (long long)M * B;
+  p.Mg = K; p.Ng = B; p.Kg = M; p.groups = 1;
+  p.out = e_up; p.gsOut = (long long)K * B;
+  p.ck = codes; p.cks = scales; p.ld_ck = mx8_ld(B);
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (tc_eligible(MODE_BK, K, M, B, dtype, algo, false)) return launch_tc(p, MODE_BK, act, dtype, s);
+  if (algo == IPC_ALGO_TCGEN05)
+    return set_error(IPC_ERR_UNSUPPORTED, "tcgen05 path: not eligible (M=%d K=%d B=%d dtype=%d)", M, K, B, dtype);
+  if (skinny_eligible(MODE_BK, K, M, B, dtype, algo)) return launch_skinny(p, MODE_BK, false, act, dtype, s);
+  return launch_generic(p, MODE_BK, false, act, dtype, s);
+}
+
+int ipc_mxfp4_quantize(const void* x, unsigned char* codes, unsigned char* scales, int R, int K, int turned, int act,
+                       int dtype, void* stream) {
+  int rc = common_checks(R, K, 1, 1, act, dtype, IPC_ALGO_AUTO);
+  if (rc) return rc;
+  if (R == 0 || K == 0) return IPC_OK;
+  IPC_REQUIRE(x && codes && scales, "null operand pointer");
+  IPC_REQUIRE(aligned16(codes) && aligned16(scales), "4-bit codes and scales must be 16-byte aligned");
+  return launch_mx4_quantize(x, codes, scales, R, K, turned != 0, act, dtype, reinterpret_cast<cudaStream_t>(stream));
+}
+
+int ipc_mxfp4_restore(const unsigned char* codes, const unsigned char* scales, void* out, int R, int K, int dtype,
+                      void* stream) {
+  int rc = common_checks(R, K, 1, 1, IPC_ACT_IDENTITY, dtype, IPC_ALGO_AUTO);
+  if (rc) return rc;
+  if (R == 0 || K == 0) return IPC_OK;
+  IPC_REQUIRE(codes && scales && out, "null operand pointer");
+  IPC_REQUIRE(aligned16(codes) && aligned16(scales), "4-bit codes and scales must be 16-byte aligned");
+  return launch_mx4_restore(codes, scales, out, R, K, dtype, reinterpret_cast<cudaStream_t>(stream));
+}
+
+int ipc_mxfp4_forward(const unsigned char* w, const unsigned char* w_scales, const unsigned char* a,
+                      const unsigned char* a_scales, void* out, int M, int K, int B, int dtype, void* stream) {
+  int rc = common_checks(M, K, B, 1, IPC_ACT_IDENTITY, dtype, IPC_ALGO_AUTO);
+  if (rc) return rc;
+  if (M == 0 || B == 0) return IPC_OK;
+  IPC_REQUIRE(out && (K == 0 || (w && w_scales && a && a_scales)), "null operand pointer");
+  IPC_REQUIRE(aligned16(w) && aligned16(w_scales) && aligned16(a) && aligned16(a_scales),
+              "4-bit codes and scales must be 16-byte aligned");
+  return launch_mx4_gemm(w, w_scales, a, a_scales, out, M, K, B, dtype, reinterpret_cast<cudaStream_t>(stream));
 }
 
 int ipc_set_max_ctas(int max_ctas) { return set_max_ctas(max_ctas); }

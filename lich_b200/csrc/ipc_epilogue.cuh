@@ -2,6 +2,7 @@
 #pragma once
 #include "ipc_common.cuh"
 #include "ipc_generic.cuh"
+#include "ipc_mx.cuh"
 
 namespace ipc {
 
@@ -26,6 +27,11 @@ __device__ __forceinline__ void epilogue(const GemmArgs& p, int g, int m, int n,
   } else if constexpr (MODE == MODE_W) {
     T* w = reinterpret_cast<T*>(p.out) + g * p.gsOut;
     w[idx] = St<T>::st(St<T>::ld(w[idx]) + p.scale * acc);
+  } else if constexpr (MODE == MODE_G) {
+    (reinterpret_cast<T*>(p.out) + g * p.gsOut)[idx] = St<T>::st(p.scale * acc);
+  } else if constexpr (MODE == MODE_BK) {
+    const float x = (float)p.ck[(long long)m * p.ld_ck + n] * mx_scale(p.cks[(long long)(n / MX_BLOCK) * p.Mg + m]);
+    (reinterpret_cast<T*>(p.out) + g * p.gsOut)[idx] = St<T>::st(act_df<ACT>(x) * acc);
   } else if constexpr (MODE == MODE_F) {
     T* o = reinterpret_cast<T*>(p.out) + g * p.gsOut;
     o[idx] = St<T>::st(acc);

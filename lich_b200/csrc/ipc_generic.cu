@@ -10,6 +10,8 @@
 //   W  (tilelang_kernels.py:268-349)  A = E[M,B]        B = f(X_up)^T          W = cast(W + a C)
 //   WD (no reference counterpart)     as W, but dw (+)= a C in fp32
 //   F  (trainer.py:512-515, 828-833)  as P                                   OUT = cast(C) [, A_out = f(OUT)]
+//   G  (no reference counterpart)     as W                                   OUT = cast(a C)
+//   BK (no reference counterpart)     as I                                   OUT = cast(f'(x) C), x in 8 bits
 // Padding of the activated operand stays zero (tilelang_kernels.py:165-167).
 #include <cstdio>
 
@@ -26,8 +28,8 @@ constexpr int BM = 64, BN = 64, BK = 32, NTHREADS = 128;
 // Operand orientation per mode.
 template <int MODE>
 struct Orient {
-  static constexpr bool a_kcontig = (MODE != MODE_I);  // I reads W_low [K,M]: m contiguous
-  static constexpr bool b_ncontig = (MODE == MODE_P || MODE == MODE_I || MODE == MODE_F);
+  static constexpr bool a_kcontig = (MODE != MODE_I && MODE != MODE_BK);  // I, BK read W_low [K,M]: m contiguous
+  static constexpr bool b_ncontig = (MODE == MODE_P || MODE == MODE_I || MODE == MODE_F || MODE == MODE_BK);
 };
 
 // Load element A(m,k) / B(k,n) of the current group (zero outside the matrix).
@@ -210,13 +212,14 @@ int launch_one(const GemmArgs& p, cudaStream_t s) {
 int launch_generic(const GemmArgs& p, int mode, bool bact, int act, int dtype, cudaStream_t s) {
   if (p.Mg <= 0 || p.Ng <= 0 || p.groups <= 0) return IPC_OK;  // empty output: nothing to do
   IPC_DISPATCH_DT(dtype, TT, {
-    if (!bact && mode != MODE_I && !(mode == MODE_F && p.aux2 != nullptr)) {
+    if (!bact && mode != MODE_I && mode != MODE_BK && !(mode == MODE_F && p.aux2 != nullptr)) {
       // the activation only enters through the B operand -> one instantiation
       switch (mode) {
         case MODE_P: return launch_one<TT, IPC_ACT_IDENTITY, MODE_P, false>(p, s);
         case MODE_W: return launch_one<TT, IPC_ACT_IDENTITY, MODE_W, false>(p, s);
         case MODE_WD: return launch_one<TT, IPC_ACT_IDENTITY, MODE_WD, false>(p, s);
         case MODE_F: return launch_one<TT, IPC_ACT_IDENTITY, MODE_F, false>(p, s);
+        case MODE_G: return launch_one<TT, IPC_ACT_IDENTITY, MODE_G, false>(p, s);
         default: break;
       }
     }
@@ -224,6 +227,7 @@ int launch_generic(const GemmArgs& p, int mode, bool bact, int act, int dtype, c
       switch (mode) {
         case MODE_P: return launch_one<TT, AC, MODE_P, true>(p, s);
         case MODE_I: return launch_one<TT, AC, MODE_I, false>(p, s);
+        case MODE_BK: return launch_one<TT, AC, MODE_BK, false>(p, s);
         case MODE_W: return launch_one<TT, AC, MODE_W, true>(p, s);
         case MODE_WD: return launch_one<TT, AC, MODE_WD, true>(p, s);
         case MODE_F:

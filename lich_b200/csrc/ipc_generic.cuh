@@ -6,7 +6,9 @@
 
 namespace ipc {
 
-enum GemmMode { MODE_P = 0, MODE_I = 1, MODE_W = 2, MODE_WD = 3, MODE_F = 4, MODE_WO = 5 };
+// G: a weight gradient in the storage type, cast(scale acc) (operands as W).  BK: the error of the layer above,
+// cast(f'(x) acc) with x from an 8-bit checkpoint (operands as I).
+enum GemmMode { MODE_P = 0, MODE_I = 1, MODE_W = 2, MODE_WD = 3, MODE_F = 4, MODE_WO = 5, MODE_G = 6, MODE_BK = 7 };
 
 // Optimizer step applied where a weight update meets W (MODE_WO and the small-batch / split-K paths), so no
 // gradient tensor is written to memory.  The gradient of the energy sum_l |e_l|^2 / 2 with respect to W[l]
@@ -44,8 +46,8 @@ __device__ __forceinline__ float opt_step(const OptParams& o, float w, float g, 
 // C[m,n] = sum_k A(m,k) B(k,n) per group, then a MODE epilogue on the
 // row-major [Mg, Ng] output.  Orientation (fixed by MODE):
 //   P, F : A(m,k) = A[m*lda + k]   B(k,n) = B[k*ldb + n]   (Mg,Ng,Kg) = (M,B,K)
-//   I : A(m,k) = A[k*lda + m]   B(k,n) = B[k*ldb + n]   (Mg,Ng,Kg) = (M,B,K)
-//   W : A(m,k) = A[m*lda + k]   B(k,n) = B[n*ldb + k]   (Mg,Ng,Kg) = (M,K,B)
+//   I, BK : A(m,k) = A[k*lda + m]   B(k,n) = B[k*ldb + n]   (Mg,Ng,Kg) = (M,B,K)
+//   W, WD, WO, G : A(m,k) = A[m*lda + k]   B(k,n) = B[n*ldb + k]   (Mg,Ng,Kg) = (M,K,B)
 struct GemmArgs {
   const void* A;
   long long lda, gsA;
@@ -63,6 +65,9 @@ struct GemmArgs {
   int a_out_from_stored;  // I: A_out = f(cast(x_new)) (what recompute mode reads back) instead of f(x_new)
   OptParams opt;    // WO: the optimizer step applied to W
   int mcast;        // WD: out is a multicast (NVLS) address, the epilogue adds with multimem.red
+  const signed char* ck;     // BK: 8-bit checkpoint of the [Mg, Ng] states, codes ld_ck apart, 16-byte aligned ...
+  const unsigned char* cks;  // ... and its scale bytes [ceil(Ng / 32)][Mg]  (ipc_mx.cuh)
+  long long ld_ck;
 };
 
 int launch_generic(const GemmArgs& p, int mode, bool bact, int act, int dtype, cudaStream_t s);

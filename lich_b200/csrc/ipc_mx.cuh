@@ -1,0 +1,86 @@
+// Microscaled storage: blocks of 32 numbers that share one power of two.
+//
+// A block whose largest magnitude is m is stored as a scale byte s + 127 and 32 codes c, each number
+// standing for c * 2^s:
+//   8 bits  s = the smallest integer with m <= 127 * 2^s; c = v * 2^-s rounded to the nearest integer
+//   4 bits  s = the smallest integer with m <= 6 * 2^s;   c = v * 2^-s rounded to sign + {0, .5, 1, 1.5, 2, 3, 4, 6}
+// (ties to even), s >= -127.  The scale is the smallest that clips nothing: the alternative for 4 bits that
+// takes the exponent of m alone clips every m above 6 * 2^s by up to a quarter.  Scaling by a power of two is exact, so
+// a code depends on the stored value alone, and c * 2^s is exact in bf16.  A block that holds an infinity or a
+// NaN is stored as codes 0 with the scale byte 255 and reads back as 32 NaNs.
+#pragma once
+#include "ipc_common.cuh"
+
+namespace ipc {
+
+constexpr int MX_BLOCK = 32;
+constexpr uint32_t MX_NAN_BYTE = 255;
+
+// Scale byte of a block from the bits of its largest magnitude (a non-negative float, or NaN).
+// TOP_EXP / TOP_MANT: the exponent and mantissa field of the largest code (127 = 2^6 * 1.984375, 6 = 2^2 * 1.5).
+template <int TOP_EXP, uint32_t TOP_MANT>
+__device__ __forceinline__ uint32_t mx_scale_byte(uint32_t max_bits) {
+  if (max_bits >= 0x7f800000u) return MX_NAN_BYTE;
+  const int e = (int)(max_bits >> 23) - TOP_EXP + ((max_bits & 0x7fffffu) > TOP_MANT ? 1 : 0);
+  return (uint32_t)max(e, 0);
+}
+__device__ __forceinline__ uint32_t mx8_scale_byte(uint32_t max_bits) { return mx_scale_byte<6, 0x7e0000u>(max_bits); }
+__device__ __forceinline__ uint32_t mx4_scale_byte(uint32_t max_bits) { return mx_scale_byte<2, 0x400000u>(max_bits); }
+
+// 2^s and 2^-s of a scale byte (2^-127 is a subnormal float; 255 stands for NaN and its codes for 0)
+__device__ __forceinline__ float mx_scale(uint32_t byte) {
+  return __uint_as_float(byte == 0 ? 0x00400000u : byte == MX_NAN_BYTE ? 0x7fc00000u : byte << 23);
+}
+__device__ __forceinline__ float mx_inv_scale(uint32_t byte) {
+  return byte == MX_NAN_BYTE ? 0.f : __uint_as_float((254u - byte) << 23);
+}
+// One 8-bit code.  A block marked NaN multiplies by 0: v * 0 is 0 or NaN, and NaN converts to 0.
+__device__ __forceinline__ int mx8_code(float v, float inv) { return __float2int_rn(v * inv); }
+
+// Eight numbers (already scaled, |v| <= 6) as 4-bit codes, the first in the lowest bits.
+__device__ __forceinline__ uint32_t mx4_pack8(const float (&v)[8]) {
+  uint32_t r;
+  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b2, %6, %5;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n\t"
+      "mov.b32 %0, {b0, b1, b2, b3};\n\t}"
+      : "=r"(r)
+      : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
+  return r;
+}
+// The inverse: eight 4-bit codes as four half2.
+__device__ __forceinline__ void mx4_unpack8(uint32_t codes, uint32_t (&h)[4]) {
+  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+      "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, b0;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %2, b2;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %3, b3;\n\t}"
+      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+      : "r"(codes));
+}
+
+// Layouts.  8 bits: codes [D][32 * ceil(B/32)], scale bytes [ceil(B/32)][D], blocks along the batch.
+// 4 bits, R rows of K columns: codes [R][Kp/2], Kp = 128 * ceil(K/128), lower column in the lower nibble; scale
+// bytes in atoms of 128 rows x 4 blocks, [ceil(R/128)][Kp/128][32][4][4] with row r, block j at
+// [r/128][j/4][r%32][r%128/32][j%4] (what the tensor core's scale operand takes).
+__host__ __device__ inline long long mx8_ld(int B) { return ((long long)B + 31) / 32 * 32; }
+__host__ __device__ inline long long mx4_kp(int K) { return ((long long)K + 127) / 128 * 128; }
+__device__ __forceinline__ long long mx4_scale_at(int r, int j, int atoms_k) {
+  return ((long long)(r >> 7) * atoms_k + (j >> 2)) * 512 + (r & 31) * 16 + ((r >> 5) & 3) * 4 + (j & 3);
+}
+
+int launch_mx8_store(const void* x, signed char* codes, unsigned char* scales, int D, int B, int dtype, cudaStream_t s);
+// out[d][b] = cast(f(codes * 2^s)), rows ld_out apart; columns B .. pad_cols - 1 of out are zeroed (pad_cols >= B)
+int launch_mx8_restore(const signed char* codes, const unsigned char* scales, void* out, int D, int B, long long ld_out,
+                       int pad_cols, int act, int dtype, cudaStream_t s);
+int launch_mx4_quantize(const void* x, unsigned char* codes, unsigned char* scales, int R, int K, int turned, int act,
+                        int dtype, cudaStream_t s);
+int launch_mx4_restore(const unsigned char* codes, const unsigned char* scales, void* out, int R, int K, int dtype,
+                       cudaStream_t s);
+int launch_mx4_gemm(const unsigned char* w, const unsigned char* ws, const unsigned char* a, const unsigned char* as,
+                    void* out, int M, int K, int B, int dtype, cudaStream_t s);
+
+}  // namespace ipc

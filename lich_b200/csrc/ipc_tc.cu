@@ -26,7 +26,8 @@
 // Operand orientation per mode (UMMA "K-major" = reduction dim contiguous):
 //   P, F : A = W [M, K]          K-major    B = A_up [K, N]        MN-major
 //   I    : A = W_low [K, M]      MN-major   B = E_low [K, N]       MN-major
-//   W, WD: A = E [M, Bt]         K-major    B = A_up [Kw, Bt]      K-major
+//   W, WD, G: A = E [M, Bt]      K-major    B = A_up [Kw, Bt]      K-major
+//   BK (the error of the layer above, f'(x) (W^T E), x in 8 bits): as I
 // The B operand is taken as stored (a saved activation): applying f inside
 // the GEMM would repeat it M/128 times per element; callers materialise
 // f(X) once (ipc_activate, or the A_out of the state update / forward sweep).
@@ -48,6 +49,7 @@
 
 #include "ipc_common.cuh"
 #include "ipc_generic.cuh"
+#include "ipc_mx.cuh"
 #include "ipc_tc.cuh"
 
 namespace ipc {
@@ -111,6 +113,9 @@ struct TcParams {
   int mcast;  // WD: out is a multicast (NVLS) address; the epilogue adds into every GPU's copy
   int raster;  // M-tiles per raster band of the tile walk
   OptParams opt;  // WO: optimizer step applied to W in the epilogue
+  const signed char* ck;  // BK: the 8-bit states' codes, their row stride, and their scale bytes [block][row]
+  const unsigned char* cks;
+  long long ld_ck;
 };
 
 // ------------------------------------------------------------ PTX helpers
@@ -363,6 +368,26 @@ __device__ __forceinline__ uint4 pack_vec(const uint32_t* acc8) {
   for (int j = 0; j < 8; ++j) oh[j] = St<T>::st(__uint_as_float(acc8[j]));
   return o;
 }
+// G: 8 scaled accumulators
+template <typename T>
+__device__ __forceinline__ uint4 pack_scaled(const uint32_t* acc8, float scale) {
+  uint4 o;
+  T* oh = reinterpret_cast<T*>(&o);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) oh[j] = St<T>::st(scale * __uint_as_float(acc8[j]));
+  return o;
+}
+// BK: cast(f'(x) acc) for 8 columns whose states are the lower or upper 8 codes of `codes`, f' in its MUFU form
+template <typename T, int ACT>
+__device__ __forceinline__ uint4 epi_vec_bk(const uint4& codes, int half, float step, const uint32_t* acc8) {
+  const uint32_t c2[2] = {half ? codes.z : codes.x, half ? codes.w : codes.y};
+  const signed char* c = reinterpret_cast<const signed char*>(c2);
+  uint4 o;
+  T* oh = reinterpret_cast<T*>(&o);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) oh[j] = St<T>::st(act_df_hw<ACT>((float)c[j] * step) * __uint_as_float(acc8[j]));
+  return o;
+}
 // ... and the coalesced pass stores it and cast(f(x)) of the stored x (the A_out of the forward sweep)
 template <typename T, int ACT>
 __device__ __forceinline__ uint4 act_vec(uint4 x) {
@@ -403,8 +428,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
                    const __grid_constant__ CUtensorMap tmE0, const __grid_constant__ CUtensorMap tmE1,
                    const __grid_constant__ CUtensorMap tmE2, const __grid_constant__ TcParams p) {
   // tmE0..2: the I epilogue's operand maps (E, X, A_out)
-  constexpr bool A_MN = (MODE == MODE_I);
-  constexpr bool B_MN = (MODE == MODE_P || MODE == MODE_I || MODE == MODE_F);
+  constexpr bool A_MN = (MODE == MODE_I || MODE == MODE_BK);
+  constexpr bool B_MN = (MODE == MODE_P || MODE == MODE_I || MODE == MODE_F || MODE == MODE_BK);
   constexpr int NCTA = PAIR ? 2 : 1;
   constexpr int TM = TC_BM * NCTA;    // rows of a tile
   constexpr int BNL = BN / NCTA;      // columns of B this CTA loads
@@ -423,7 +448,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   constexpr bool EPI_STAGED =
-      (MODE == MODE_P || MODE == MODE_W || MODE == MODE_I || MODE == MODE_F || MODE == MODE_WD);
+      (MODE == MODE_P || MODE == MODE_W || MODE == MODE_I || MODE == MODE_F || MODE == MODE_WD || MODE == MODE_G ||
+       MODE == MODE_BK);
   constexpr uint32_t EPI_REGION = EPI_STAGED ? epi_bytes(MODE, PAIR) : 0;
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + STAGES * STAGE_BYTES + EPI_REGION);
   // bars: full[S], empty[S], tfull[2], tempty[2], epilogue slots[NSL per epilogue warp]
@@ -593,7 +619,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     uint32_t aphase = 0;
     bool staged = false;
     if constexpr (EPI_STAGED) staged = p.staged != 0;
-    const bool xpose = (MODE == MODE_P || MODE == MODE_W || MODE == MODE_F) && staged;
+    const bool xpose =
+        (MODE == MODE_P || MODE == MODE_W || MODE == MODE_F || MODE == MODE_G || MODE == MODE_BK) && staged;
     if (xpose) {
       {
         // P / W: the warp's 32 x HC block of the in/out operand (X_lo or W) is read with coalesced
@@ -602,8 +629,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         // buffer, each row thread applies the epilogue to its row in place, and the chunk leaves
         // with coalesced 16-byte stores (a warp instruction covers 4 rows x 128 bytes).
         // F has no input block: the row threads write cast(acc) into the buffer, and the coalesced
-        // pass stores it and, when A_out is given, cast(f(x)) beside it.
-        constexpr bool HAS_IN = (MODE != MODE_F);
+        // pass stores it and, when A_out is given, cast(f(x)) beside it.  G: the same with scale acc.
+        // BK: a row thread reads the 8-bit states of its own row (HC bytes, whole sectors) into registers
+        // before the accumulator is ready and writes cast(f'(x) acc).
+        constexpr bool HAS_IN = (MODE == MODE_P || MODE == MODE_W);
         constexpr int NCH = HC / 64;        // 64-column chunks per warp and tile
         constexpr int NPRE = 8 * NCH;       // prefetched 16-byte vectors per thread
         const uint32_t xb = saddr(smem + STAGES * STAGE_BYTES) + (warp - 2) * EPI_WARP_BYTES;
@@ -631,6 +660,19 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
           int g, m0, n0, sp;
           tile_coords(p, t, BN, g, m0, n0, sp, TM, rank);
           const int r0 = m0 + 32 * q, nw = n0 + c_lo;
+          uint4 ckv[MODE == MODE_BK ? HC / 16 : 1];
+          uint32_t ckb[MODE == MODE_BK ? HC / 32 : 1];
+          if constexpr (MODE == MODE_BK) {
+            const bool in = r0 + lane < p.Mg;
+            const signed char* row = p.ck + (long long)(r0 + lane) * p.ld_ck;
+#pragma unroll
+            for (int i = 0; i < HC / 16; ++i)
+              ckv[i] = (in && nw + 16 * i < p.Ng) ? __ldg(reinterpret_cast<const uint4*>(row + nw + 16 * i))
+                                                  : make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int i = 0; i < HC / 32; ++i)
+              ckb[i] = (in && nw + 32 * i < p.Ng) ? p.cks[(long long)((nw + 32 * i) / 32) * p.Mg + r0 + lane] : 0u;
+          }
           const bool ok = mbar_wait(tfull0 + 8 * acc, aphase, abort_flag);
           __syncwarp();
           if (!ok) break;
@@ -657,6 +699,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
                 const uint32_t a = xb + lane * 128 + (((4 * hf + j) ^ (lane & 7)) << 4);
                 if constexpr (HAS_IN)
                   sts128(a, epi_vec_pw<T, MODE>(lds128(a), raw + 8 * j, p.scale));
+                else if constexpr (MODE == MODE_BK)
+                  sts128(a, epi_vec_bk<T, ACT>(ckv[4 * cc + 2 * hf + j / 2], j & 1, mx_scale(ckb[2 * cc + hf]), raw + 8 * j));
+                else if constexpr (MODE == MODE_G)
+                  sts128(a, pack_scaled<T>(raw + 8 * j, p.scale));
                 else
                   sts128(a, pack_vec<T>(raw + 8 * j));
               }
@@ -968,6 +1014,12 @@ __global__ void ws_reduce_kernel(const float* __restrict__ ws, int splits, long 
       w[1] = St<T>::st(opt_step(opt, St<T>::ld(w[1]), -acc.y, 4 * i + 1));
       w[2] = St<T>::st(opt_step(opt, St<T>::ld(w[2]), -acc.z, 4 * i + 2));
       w[3] = St<T>::st(opt_step(opt, St<T>::ld(w[3]), -acc.w, 4 * i + 3));
+    } else if constexpr (MODE == MODE_G) {
+      T* w = reinterpret_cast<T*>(out) + 4 * i;
+      w[0] = St<T>::st(scale * acc.x);
+      w[1] = St<T>::st(scale * acc.y);
+      w[2] = St<T>::st(scale * acc.z);
+      w[3] = St<T>::st(scale * acc.w);
     } else {
       T* w = reinterpret_cast<T*>(out) + 4 * i;
       w[0] = St<T>::st(St<T>::ld(w[0]) + scale * acc.x);
@@ -980,8 +1032,8 @@ __global__ void ws_reduce_kernel(const float* __restrict__ ws, int splits, long 
 
 template <typename T, int ACT, int MODE, int BN, int PAIR>
 int launch_tc_t(const GemmArgs& a, int dtype, cudaStream_t s, float* ws, size_t ws_bytes, const TcTune* tune) {
-  constexpr bool A_MN = (MODE == MODE_I);
-  constexpr bool B_MN = (MODE == MODE_P || MODE == MODE_I || MODE == MODE_F);
+  constexpr bool A_MN = (MODE == MODE_I || MODE == MODE_BK);
+  constexpr bool B_MN = (MODE == MODE_P || MODE == MODE_I || MODE == MODE_F || MODE == MODE_BK);
   constexpr int TM = PAIR ? 2 * TC_BM : TC_BM;  // rows of a tile
   constexpr int BNL = PAIR ? BN / 2 : BN;       // B columns one CTA loads
   CUtensorMap ta, tb;
@@ -1011,6 +1063,7 @@ int launch_tc_t(const GemmArgs& a, int dtype, cudaStream_t s, float* ws, size_t 
   // a roughly square block of output tiles and re-reads each operand block about as often as the other
   p.raster = (tune != nullptr && tune->raster > 0) ? tune->raster : (PAIR ? TC_RASTER / 2 : TC_RASTER);
   p.opt = a.opt;
+  p.ck = a.ck; p.cks = a.cks; p.ld_ck = a.ld_ck;
   // split-K: a weight update with fewer output tiles than half the SMs and a long batch reduction
   const int nk = (a.Kg + TC_BK - 1) / TC_BK;
   p.splits = 1;
@@ -1020,7 +1073,7 @@ int launch_tc_t(const GemmArgs& a, int dtype, cudaStream_t s, float* ws, size_t 
   if (tune != nullptr && tune->max_ctas > 0 && tune->max_ctas < cap) cap = tune->max_ctas;
   const int want = tune != nullptr ? tune->splits : 0;  // 0: heuristic, 1: never, >= 2: requested
   const int units = PAIR ? max(1, cap / 2) : cap;  // tiles walked at once: CTAs, or CTA pairs
-  if ((MODE == MODE_W || MODE == MODE_WD || MODE == MODE_WO) && ws != nullptr && want != 1 &&
+  if ((MODE == MODE_W || MODE == MODE_WD || MODE == MODE_WO || MODE == MODE_G) && ws != nullptr && want != 1 &&
       (want >= 2 || (p.tiles < units / 2 && nk >= 8)) &&
       a.gsOut == (long long)a.Mg * a.Ng) {  // the reduce pass walks out as one dense [groups][M][N] array
     const long long tile_bytes = (long long)a.groups * a.Mg * a.Ng * 4;
@@ -1052,7 +1105,8 @@ int launch_tc_t(const GemmArgs& a, int dtype, cudaStream_t s, float* ws, size_t 
   // staged epilogue (no split-K): P / W through the transpose buffer, I through TMA with three maps
   // (E, X, A_out) of 32-row x 16-column boxes, 32-byte swizzle
   constexpr bool EPI_STAGED =
-      (MODE == MODE_P || MODE == MODE_W || MODE == MODE_I || MODE == MODE_F || MODE == MODE_WD);
+      (MODE == MODE_P || MODE == MODE_W || MODE == MODE_I || MODE == MODE_F || MODE == MODE_WD || MODE == MODE_G ||
+       MODE == MODE_BK);
   CUtensorMap te[3];
   memset(te, 0, sizeof(te));
   // WD accumulating into dw reads dw back per element: the row-per-thread path
@@ -1103,7 +1157,7 @@ int launch_tc_t(const GemmArgs& a, int dtype, cudaStream_t s, float* ws, size_t 
   count_launch();
   int rc2 = check_launch("tcgen05 GEMM");
   if (rc2 || p.splits == 1 || p.atomic) return rc2;
-  if constexpr (MODE == MODE_W || MODE == MODE_WD || MODE == MODE_WO) {
+  if constexpr (MODE == MODE_W || MODE == MODE_WD || MODE == MODE_WO || MODE == MODE_G) {
     const long long n4 = (long long)a.groups * a.Mg * a.Ng / 4;
     long long blocks = (n4 + 255) / 256;
     if (blocks > 148LL * 16) blocks = 148LL * 16;
@@ -1117,8 +1171,8 @@ int launch_tc_t(const GemmArgs& a, int dtype, cudaStream_t s, float* ws, size_t 
 template <typename T, int MODE, int BN, int PAIR>
 int dispatch_act(const GemmArgs& a, int act, int dtype, cudaStream_t s, float* ws, size_t ws_bytes,
                  const TcTune* tune) {
-  if constexpr (MODE == MODE_P || MODE == MODE_W || MODE == MODE_WD || MODE == MODE_WO) {
-    return launch_tc_t<T, IPC_ACT_IDENTITY, MODE, BN, PAIR>(a, dtype, s, ws, ws_bytes, tune);  // f only in I / F
+  if constexpr (MODE == MODE_P || MODE == MODE_W || MODE == MODE_WD || MODE == MODE_WO || MODE == MODE_G) {
+    return launch_tc_t<T, IPC_ACT_IDENTITY, MODE, BN, PAIR>(a, dtype, s, ws, ws_bytes, tune);  // f only in I / F / BK
   } else {
     IPC_DISPATCH_ACT(act, AC, { return launch_tc_t<T, AC, MODE, BN, PAIR>(a, dtype, s, ws, ws_bytes, tune); });
   }
@@ -1135,6 +1189,8 @@ int dispatch_mode(const GemmArgs& a, int mode, int act, int dtype, cudaStream_t 
     case MODE_WD: return dispatch_act<T, MODE_WD, BN, PAIR>(a, act, dtype, s, ws, ws_bytes, tune);
     case MODE_F: return dispatch_act<T, MODE_F, BN, PAIR>(a, act, dtype, s, ws, ws_bytes, tune);
     case MODE_WO: return dispatch_act<T, MODE_WO, BN, PAIR>(a, act, dtype, s, ws, ws_bytes, tune);
+    case MODE_G: return dispatch_act<T, MODE_G, BN, PAIR>(a, act, dtype, s, ws, ws_bytes, tune);
+    case MODE_BK: return dispatch_act<T, MODE_BK, BN, PAIR>(a, act, dtype, s, ws, ws_bytes, tune);
     default: return set_error(IPC_ERR_ARG, "bad GEMM mode %d", mode);
   }
 }
@@ -1146,7 +1202,7 @@ bool tc_eligible(int mode, int M, int K, int B, int dtype, int algo, bool b_acti
   if (dtype != IPC_DT_F16 && dtype != IPC_DT_BF16) return false;
   if (b_activated) return false;  // f on the B operand is materialised once by the caller
   int Mg = M, Ng = B, Kg = K;
-  const bool weight = (mode == MODE_W || mode == MODE_WD || mode == MODE_WO);
+  const bool weight = (mode == MODE_W || mode == MODE_WD || mode == MODE_WO || mode == MODE_G);
   if (weight) { Ng = K; Kg = B; }
   if (Mg < 1 || Ng < 1 || Kg < 1) return false;
   if (M % 8 || K % 8 || B % 8) return false;  // 16-byte row strides for TMA and the epilogue vectors
@@ -1169,7 +1225,7 @@ int launch_tc(const GemmArgs& a, int mode, int act, int dtype, cudaStream_t s, f
   // takes the generic kernel
   const uintptr_t mis = reinterpret_cast<uintptr_t>(a.A) | reinterpret_cast<uintptr_t>(a.Bm) |
                         reinterpret_cast<uintptr_t>(a.out) | reinterpret_cast<uintptr_t>(a.aux) |
-                        reinterpret_cast<uintptr_t>(a.aux2);
+                        reinterpret_cast<uintptr_t>(a.aux2) | reinterpret_cast<uintptr_t>(a.ck);
   if (mis & 15) {
     if (a.mcast) return set_error(IPC_ERR_ARG, "IPC_FLAG_MULTIMEM_RED: operands must be 16-byte aligned");
     return launch_generic(a, mode, false, act, dtype, s);
@@ -1183,7 +1239,7 @@ int launch_tc(const GemmArgs& a, int mode, int act, int dtype, cudaStream_t s, f
   const long long tm = (a.Mg + TC_BM - 1) / TC_BM;
   const long long t256 = tm * ((a.Ng + 255) / 256) * a.groups, t128 = tm * ((a.Ng + 127) / 128) * a.groups;
   const long long cap = grid_cap();
-  const bool splitk = (mode == MODE_W || mode == MODE_WD || mode == MODE_WO) && ws != nullptr && t256 < cap / 2 &&
+  const bool splitk = (mode == MODE_W || mode == MODE_WD || mode == MODE_WO || mode == MODE_G) && ws != nullptr && t256 < cap / 2 &&
                       (a.Kg + TC_BK - 1) / TC_BK >= 8 && a.gsOut == (long long)a.Mg * a.Ng &&
                       ws_bytes >= (size_t)(2LL * a.groups * a.Mg * a.Ng * 4);
   const long long cost256 = ((t256 + cap - 1) / cap) * (256 + 416), cost128 = ((t128 + cap - 1) / cap) * (128 + 416);

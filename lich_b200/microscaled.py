@@ -1,0 +1,309 @@
+"""Microscaled layers: 8-bit checkpoints of states with the backward products that read them, and 4-bit operands
+with their product.
+
+Blocks of 32 numbers share one power of two (formats and layouts: ``include/ipc_b200.h``).  Like the builders of
+``lich_b200.tilelang_kernels`` each ``build_*`` returns a cached callable specialised for its shape, activation and
+dtype that writes its output tensors in place on the current CUDA stream, raises ``ValueError`` for tensors of another
+shape, dtype, device or layout before anything is launched, and owns (per device and stream) whatever workspace it
+needs.
+
+    codes, scales = empty_checkpoint(D, B, device=dev)                       # states x [D, B] kept in 8 bits
+    build_checkpoint(D, B, "bfloat16")(x, codes, scales)
+    build_checkpoint_restore(D, B, "tanh", "bfloat16")(codes, scales, out)   # out = f(x^)
+    build_weight_update_checkpoint(M, K, B, "tanh", "bfloat16", alpha)(w, e, codes, scales)       # W += alpha E f(x^)^T
+    build_weight_delta_checkpoint(M, K, B, "tanh", "bfloat16", alpha)(dw, e, codes, scales)       # dW, W untouched
+    build_error_backward_checkpoint(M, K, B, "tanh", "bfloat16")(w, e, codes, scales, e_up)       # f'(x^) * (W^T E)
+
+    wq, ws = empty_mxfp4(M, K, device=dev)                                   # weights [M, K] in 4 bits
+    build_mxfp4_quantize(M, K, "identity", "bfloat16")(w, wq, ws)
+    aq, as_ = empty_mxfp4(B, K, device=dev)                                  # f(x) of states [K, B], turned to [B, K]
+    build_mxfp4_quantize(B, K, "tanh", "bfloat16", True)(x, aq, as_)
+    build_mxfp4_forward(M, K, B, "bfloat16")(wq, ws, aq, as_, out)           # out [M, B] = W4 @ A4^T
+
+The reference has no counterpart: it keeps and multiplies fp16 only (``tilelang_kernels.py:8-17``).
+"""
+from __future__ import annotations
+
+from ctypes import byref, c_size_t
+from functools import lru_cache
+
+import torch
+
+from . import _native as N
+from .tilelang_kernels import KernelConfig, _algo
+
+N.load()
+
+BLOCK = 32
+
+
+def checkpoint_shapes(D: int, B: int) -> tuple[tuple[int, int], tuple[int, int]]:
+    """Shapes of a checkpoint's codes (int8) and scale bytes (uint8) for states ``[D, B]``."""
+    nb = -(-int(B) // BLOCK)
+    return (int(D), nb * BLOCK), (nb, int(D))
+
+
+def mxfp4_shapes(R: int, K: int) -> tuple[tuple[int, int], tuple[int, ...]]:
+    """Shapes of a 4-bit operand's codes and scale bytes (both uint8) for ``R`` rows and ``K`` columns."""
+    ka = -(-int(K) // 128)
+    return (int(R), ka * 64), (-(-int(R) // 128), ka, 32, 4, 4)
+
+
+def empty_checkpoint(D: int, B: int, *, device) -> tuple[torch.Tensor, torch.Tensor]:
+    c, s = checkpoint_shapes(D, B)
+    return torch.empty(c, device=device, dtype=torch.int8), torch.empty(s, device=device, dtype=torch.uint8)
+
+
+def empty_mxfp4(R: int, K: int, *, device) -> tuple[torch.Tensor, torch.Tensor]:
+    c, s = mxfp4_shapes(R, K)
+    return torch.empty(c, device=device, dtype=torch.uint8), torch.empty(s, device=device, dtype=torch.uint8)
+
+
+class _MxOp:
+    """Shape-specialised callable over the C ABI: ``spec`` names each tensor argument's shape and dtype."""
+
+    kind = "op"
+
+    def __init__(self, entry: str, spec):
+        self.spec = tuple((torch.Size(s), d) for s, d in spec)
+        self._fn = getattr(N.load(), entry)
+        self._ws: dict = {}
+
+    def _stream(self, tensors) -> int:
+        """The current stream of the tensors' device, after checking the tensors against ``spec``."""
+        try:
+            dev = tensors[0].get_device()
+            for t, (shape, dtype) in zip(tensors, self.spec):
+                if t.shape != shape or t.dtype is not dtype or t.get_device() != dev or not t.is_contiguous():
+                    break
+            else:
+                if dev >= 0:
+                    return torch._C._cuda_getCurrentRawStream(dev)
+        except AttributeError:
+            pass
+        raise ValueError(self._refusal(tensors))
+
+    def _refusal(self, tensors) -> str:
+        for i, (t, (shape, dtype)) in enumerate(zip(tensors, self.spec)):
+            if not isinstance(t, torch.Tensor):
+                return f"{self.kind}: argument {i} is not a tensor"
+            if t.shape != shape:
+                return f"{self.kind}: argument {i} has shape {tuple(t.shape)}, kernel was built for {tuple(shape)}"
+            if t.dtype != dtype:
+                return f"{self.kind}: argument {i} is {t.dtype}, kernel was built for {dtype}"
+            if not t.is_cuda:
+                return f"{self.kind}: argument {i} is not a CUDA tensor"
+            if not t.is_contiguous():
+                return f"{self.kind}: argument {i} is not contiguous"
+        return f"{self.kind}: tensors on different devices"
+
+    def _launch(self, tensors, *args) -> None:
+        """The C entry on the tensors' device and its current stream; its error as an exception."""
+        dev = tensors[0].get_device()
+        if dev == torch._C._cuda_getDevice():
+            rc = self._fn(*args)
+        else:
+            with torch.cuda.device(dev):
+                rc = self._fn(*args)
+        if rc:
+            N.check(rc)
+
+    def get_kernel_source(self) -> str:
+        return f"lich_b200 {self.kind} {self.spec} (prebuilt sm_100a kernel, include/ipc_b200.h)"
+
+
+class CheckpointKernel(_MxOp):
+    kind = "checkpoint"
+
+    def __init__(self, D, B, dtype):
+        c, s = checkpoint_shapes(D, B)
+        super().__init__("ipc_mx8_store", [((D, B), N.torch_dtype(dtype)), (c, torch.int8), (s, torch.uint8)])
+        self.D, self.B, self.dt = int(D), int(B), N.dtype_code(dtype)
+
+    def __call__(self, x, codes, scales):
+        t = (x, codes, scales)
+        s = self._stream(t)
+        self._launch(t, x.data_ptr(), codes.data_ptr(), scales.data_ptr(), self.D, self.B, self.dt, s)
+
+
+class CheckpointRestoreKernel(_MxOp):
+    kind = "checkpoint_restore"
+
+    def __init__(self, D, B, activation, dtype):
+        c, s = checkpoint_shapes(D, B)
+        super().__init__("ipc_mx8_restore", [(c, torch.int8), (s, torch.uint8), ((D, B), N.torch_dtype(dtype))])
+        self.D, self.B, self.act, self.dt = int(D), int(B), N.act_code(activation), N.dtype_code(dtype)
+
+    def __call__(self, codes, scales, out):
+        t = (codes, scales, out)
+        s = self._stream(t)
+        self._launch(t, codes.data_ptr(), scales.data_ptr(), out.data_ptr(), self.D, self.B, self.act, self.dt, s)
+
+
+class CheckpointWeightKernel(_MxOp):
+    kind = "weight_checkpoint"
+
+    def __init__(self, mode, M, K, B, activation, dtype, alpha, out_dtype, cfg):
+        c, s = checkpoint_shapes(K, B)
+        dt = N.torch_dtype(dtype)
+        super().__init__("ipc_mx8_weight", [((M, K), out_dtype), ((M, B), dt), (c, torch.int8), (s, torch.uint8)])
+        self.mode, self.M, self.K, self.B = mode, int(M), int(K), int(B)
+        self.act, self.dt, self.alpha, self.algo = N.act_code(activation), N.dtype_code(dtype), float(alpha), _algo(cfg)
+
+    def _workspace(self, dev: int, stream: int):
+        """This operator's workspace for one stream of a device: calls on two streams may overlap."""
+        ws = self._ws.get((dev, stream))
+        if ws is None:
+            n = c_size_t(0)
+            with torch.cuda.device(dev):
+                N.check(N.load().ipc_mx8_weight_ws_bytes(self.mode, self.M, self.K, self.B, self.dt, self.algo, byref(n)))
+                buf = torch.empty(max(int(n.value), 16), device=f"cuda:{dev}", dtype=torch.uint8)
+            ws = self._ws[dev, stream] = (buf, buf.data_ptr(), int(n.value))
+        return ws
+
+    def __call__(self, out, e, codes, scales, *, accumulate: bool = False):
+        t = (out, e, codes, scales)
+        s = self._stream(t)
+        if accumulate and self.mode != N.MODE_WDELTA:
+            raise ValueError(f"{self.kind}: only a weight delta in float32 accumulates")
+        _, ws, n = self._workspace(out.get_device(), s)
+        self._launch(t, self.mode, out.data_ptr(), e.data_ptr(), codes.data_ptr(), scales.data_ptr(), self.M, self.K,
+                     self.B, self.alpha, N.FLAG_ACCUMULATE if accumulate else 0, self.act, self.dt, self.algo, ws, n, s)
+
+
+class CheckpointBackwardKernel(_MxOp):
+    kind = "error_backward_checkpoint"
+
+    def __init__(self, M, K, B, activation, dtype, cfg):
+        c, s = checkpoint_shapes(K, B)
+        dt = N.torch_dtype(dtype)
+        super().__init__("ipc_mx8_backward",
+                         [((M, K), dt), ((M, B), dt), (c, torch.int8), (s, torch.uint8), ((K, B), dt)])
+        self.M, self.K, self.B = int(M), int(K), int(B)
+        self.act, self.dt, self.algo = N.act_code(activation), N.dtype_code(dtype), _algo(cfg)
+
+    def __call__(self, w, e, codes, scales, e_up):
+        t = (w, e, codes, scales, e_up)
+        s = self._stream(t)
+        self._launch(t, e_up.data_ptr(), w.data_ptr(), e.data_ptr(), codes.data_ptr(), scales.data_ptr(), self.M, self.K,
+                     self.B, self.act, self.dt, self.algo, s)
+
+
+class Mxfp4QuantizeKernel(_MxOp):
+    kind = "mxfp4_quantize"
+
+    def __init__(self, R, K, activation, dtype, turned):
+        c, s = mxfp4_shapes(R, K)
+        super().__init__("ipc_mxfp4_quantize", [((K, R) if turned else (R, K), N.torch_dtype(dtype)),
+                                                (c, torch.uint8), (s, torch.uint8)])
+        self.R, self.K, self.turned = int(R), int(K), int(bool(turned))
+        self.act, self.dt = N.act_code(activation), N.dtype_code(dtype)
+
+    def __call__(self, x, codes, scales):
+        t = (x, codes, scales)
+        s = self._stream(t)
+        self._launch(t, x.data_ptr(), codes.data_ptr(), scales.data_ptr(), self.R, self.K, self.turned, self.act, self.dt,
+                     s)
+
+
+class Mxfp4RestoreKernel(_MxOp):
+    kind = "mxfp4_restore"
+
+    def __init__(self, R, K, dtype):
+        c, s = mxfp4_shapes(R, K)
+        super().__init__("ipc_mxfp4_restore", [(c, torch.uint8), (s, torch.uint8), ((R, K), N.torch_dtype(dtype))])
+        self.R, self.K, self.dt = int(R), int(K), N.dtype_code(dtype)
+
+    def __call__(self, codes, scales, out):
+        t = (codes, scales, out)
+        s = self._stream(t)
+        self._launch(t, codes.data_ptr(), scales.data_ptr(), out.data_ptr(), self.R, self.K, self.dt, s)
+
+
+class Mxfp4ForwardKernel(_MxOp):
+    kind = "mxfp4_forward"
+
+    def __init__(self, M, K, B, dtype):
+        wc, ws = mxfp4_shapes(M, K)
+        ac, as_ = mxfp4_shapes(B, K)
+        super().__init__("ipc_mxfp4_forward", [(wc, torch.uint8), (ws, torch.uint8), (ac, torch.uint8),
+                                               (as_, torch.uint8), ((M, B), N.torch_dtype(dtype))])
+        self.M, self.K, self.B, self.dt = int(M), int(K), int(B), N.dtype_code(dtype)
+
+    def __call__(self, w, w_scales, a, a_scales, out):
+        t = (w, w_scales, a, a_scales, out)
+        s = self._stream(t)
+        self._launch(t, w.data_ptr(), w_scales.data_ptr(), a.data_ptr(), a_scales.data_ptr(), out.data_ptr(), self.M,
+                     self.K, self.B, self.dt, s)
+
+
+def _validate(*sizes, activation="identity", dtype):
+    if min(int(n) for n in sizes) < 0:
+        raise ValueError(f"negative size in {sizes}")
+    N.act_code(activation)
+    N.dtype_code(N.torch_dtype(dtype))
+
+
+@lru_cache(maxsize=256)
+def build_checkpoint(D: int, B: int, dtype: str):
+    """``kernel(x [D, B], codes, scales)``: the states in 8 bits."""
+    _validate(D, B, dtype=dtype)
+    return CheckpointKernel(D, B, dtype)
+
+
+@lru_cache(maxsize=256)
+def build_checkpoint_restore(D: int, B: int, activation: str, dtype: str):
+    """``kernel(codes, scales, out [D, B])``: ``out = f(x^)``."""
+    _validate(D, B, activation=activation, dtype=dtype)
+    return CheckpointRestoreKernel(D, B, activation, dtype)
+
+
+@lru_cache(maxsize=256)
+def build_weight_update_checkpoint(M: int, K: int, B: int, activation: str, dtype: str, alpha: float,
+                                   cfg: KernelConfig = KernelConfig()):
+    """``kernel(w [M, K], e [M, B], codes, scales)``: ``W += alpha * E @ f(x^)^T`` in place."""
+    _validate(M, K, B, activation=activation, dtype=dtype)
+    return CheckpointWeightKernel(N.MODE_WEIGHT, M, K, B, activation, dtype, alpha, N.torch_dtype(dtype), cfg)
+
+
+@lru_cache(maxsize=256)
+def build_weight_delta_checkpoint(M: int, K: int, B: int, activation: str, dtype: str, alpha: float,
+                                  delta_dtype: str = "float32", cfg: KernelConfig = KernelConfig()):
+    """``kernel(dw [M, K], e [M, B], codes, scales, accumulate=False)``: ``dw = alpha * E @ f(x^)^T``, in float32 (which
+    alone can accumulate) or in ``dtype``."""
+    _validate(M, K, B, activation=activation, dtype=dtype)
+    out = N.torch_dtype(delta_dtype)
+    if out is not torch.float32 and out is not N.torch_dtype(dtype):
+        raise ValueError(f"a weight delta is kept in float32 or in {dtype}, not in {delta_dtype}")
+    mode = N.MODE_WDELTA if out is torch.float32 else N.MODE_WGRAD
+    return CheckpointWeightKernel(mode, M, K, B, activation, dtype, alpha, out, cfg)
+
+
+@lru_cache(maxsize=256)
+def build_error_backward_checkpoint(M: int, K: int, B: int, activation: str, dtype: str,
+                                    cfg: KernelConfig = KernelConfig()):
+    """``kernel(w [M, K], e [M, B], codes, scales, e_up [K, B])``: ``e_up = f'(x^) * (W^T @ E)``."""
+    _validate(M, K, B, activation=activation, dtype=dtype)
+    return CheckpointBackwardKernel(M, K, B, activation, dtype, cfg)
+
+
+@lru_cache(maxsize=256)
+def build_mxfp4_quantize(R: int, K: int, activation: str, dtype: str, turned: bool = False):
+    """``kernel(x, codes, scales)``: ``f(x)`` as a 4-bit operand of ``R`` rows; ``x`` is ``[R, K]``, or with ``turned``
+    the feature-major ``[K, R]``."""
+    _validate(R, K, activation=activation, dtype=dtype)
+    return Mxfp4QuantizeKernel(R, K, activation, dtype, turned)
+
+
+@lru_cache(maxsize=256)
+def build_mxfp4_restore(R: int, K: int, dtype: str):
+    """``kernel(codes, scales, out [R, K])``: the values a 4-bit operand stands for."""
+    _validate(R, K, dtype=dtype)
+    return Mxfp4RestoreKernel(R, K, dtype)
+
+
+@lru_cache(maxsize=256)
+def build_mxfp4_forward(M: int, K: int, B: int, dtype: str):
+    """``kernel(w, w_scales, a, a_scales, out [M, B])``: ``out = W4 @ A4^T``, sums in float32, stored in ``dtype``."""
+    _validate(M, K, B, dtype=dtype)
+    return Mxfp4ForwardKernel(M, K, B, dtype)

@@ -1,0 +1,372 @@
+"""GPU parity of the microscaled operators against their definition in 64 bits (``oracle/mx_oracle.py``).
+
+Codes and scale bytes are equal to the oracle's.  Bounds of the products, element by element, with S = |A| |B| (the
+product of magnitudes), u the unit roundoff of the storage type (2^-11 fp16, 2^-8 bf16, 2^-24 fp32):
+
+* the stored operand f(x^) is rounded once: S u; where f is a 16-bit MUFU form, tanh.approx adds a relative 2^-10.9
+  (sigmoid, silu 2^-20; gelu through tanh at most 0.5 |x| 2^-10.9);
+* fp32 sums of n products: S n 2^-23 (accumulators may truncate, which doubles the unit roundoff);
+* the result is rounded once: u |result|; 16-bit results below the smallest normal number: half of the smallest
+  subnormal;
+* the slope f' in its MUFU form is off by at most 2 * 2^-10.9 (tanh), 2^-18 (sigmoid, silu), and for gelu, whose
+  derivative holds x (1 - t^2), by (0.5 + |x| g(x)) 2^-10.9 with g the inner derivative.
+"""
+import math
+
+import pytest
+import torch
+
+from oracle import ipc_oracle as O
+from oracle import mx_oracle as X
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda", 0)
+HALF = [torch.float16, torch.bfloat16]
+ALL = HALF + [torch.float32]
+NAME = {torch.float16: "float16", torch.bfloat16: "bfloat16", torch.float32: "float32"}
+U = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8, torch.float32: 2.0 ** -24}
+TINY = {torch.float16: 2.0 ** -25, torch.bfloat16: 2.0 ** -134, torch.float32: 2.0 ** -150}
+MUFU = 2.0 ** -10.9
+ACTS = ["relu", "tanh", "sigmoid", "silu", "gelu", "identity"]
+
+
+def _mx():
+    from lich_b200 import microscaled as mx
+    return mx
+
+
+def _rand(shape, seed, scale=1.0, dt=torch.float32):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(*shape, generator=g) * scale).to(dt)
+
+
+def _states(D, B, seed, dt):
+    """Rows of very different size, a row of zeros, tiny and (in fp32, bf16) very large rows."""
+    x = torch.randn(D, B, generator=torch.Generator().manual_seed(seed))
+    x *= torch.exp2(torch.randint(-6, 7, (D, 1), generator=torch.Generator().manual_seed(seed + 1)).float())
+    x[D // 2] = 0
+    x[0, ::2] = 0
+    if D > 3:
+        x[1] *= 2.0 ** -20 if dt is torch.float16 else 2.0 ** -120
+        if dt is not torch.float16:
+            x[2] *= 2.0 ** 110
+    return x.to(dt)
+
+
+def _ckpt(x):
+    c, s = X.store8(x)
+    return c.to(DEV), s.to(DEV)
+
+
+def _act_err(act, x, dt):
+    """Bound of |f_device(x) - f(x)| before rounding, for 16-bit storage (fp32 uses CUDA's own functions, 4 ulp)."""
+    y = O.act_forward(act, x).abs()
+    if act in ("relu", "identity"):
+        return torch.zeros_like(y)
+    if dt is torch.float32:
+        return 2.0 ** -21 * y + (2.0 ** -21 * x.abs() if act == "gelu" else 0)
+    if act == "tanh":
+        return MUFU * y
+    if act == "gelu":
+        return 0.5 * x.abs() * MUFU + 2.0 ** -20 * y
+    return 2.0 ** -20 * (y + 2.0 ** -20)
+
+
+def _slope_err(act, x, dt):
+    if act in ("relu", "identity"):
+        return torch.zeros_like(x)
+    g = math.sqrt(2 / math.pi) * (1 + 3 * 0.044715 * x * x)
+    if dt is torch.float32:
+        return 2.0 ** -20 * (1 + x.abs() * (g if act == "gelu" else 1))
+    if act == "tanh":
+        return torch.full_like(x, 2 * MUFU)
+    if act == "gelu":
+        return (0.5 + x.abs() * g) * MUFU + 2.0 ** -20
+    return 2.0 ** -18 * (1 + x.abs())
+
+
+def _within(got, ref, tol):
+    got = got.double().cpu()
+    assert got.shape == ref.shape
+    over = (got - ref).abs() - tol
+    assert not torch.isnan(got).any()
+    assert (over <= 0).all(), f"{int((over > 0).sum())} of {over.numel()} over by up to {over.max():.3e}"
+
+
+# ----------------------------------------------------------------------------------------------- 8-bit checkpoint
+@pytest.mark.parametrize("dt", ALL)
+@pytest.mark.parametrize("D,B", [(1, 1), (4, 31), (5, 32), (33, 33), (10, 128), (70, 264), (784, 128), (100, 777)])
+def test_store_and_restore(D, B, dt):
+    mx = _mx()
+    x = _states(D, B, 3, dt)
+    c, s = mx.empty_checkpoint(D, B, device=DEV)
+    c.fill_(77), s.fill_(77)
+    mx.build_checkpoint(D, B, NAME[dt])(x.to(DEV), c, s)
+    rc, rs = X.store8(x)
+    assert torch.equal(c.cpu(), rc) and torch.equal(s.cpu(), rs)
+    xhat = X.load8(rc, rs, B)
+    assert ((xhat - x.double()).abs() <= torch.exp2(rs.double() - 128).repeat_interleave(32, 0)[:B].t()).all()
+    for act in ACTS:
+        out = torch.full((D, B), 9.0, device=DEV, dtype=dt)
+        mx.build_checkpoint_restore(D, B, act, NAME[dt])(c, s, out)
+        ref = O.act_forward(act, xhat)
+        ref = torch.where(ref.abs() > torch.finfo(dt).max, ref.sign() * float("inf"), ref)
+        big = torch.isinf(ref) | (ref.abs() > torch.finfo(dt).max * (1 - U[dt]))  # rounds to the largest, or over it
+        got = out.cpu().double()
+        assert (got[big].abs() >= torch.finfo(dt).max).all()
+        got[big], ref[big] = 0, 0
+        _within(got, ref, _act_err(act, xhat, dt) * (~big) + U[dt] * ref.abs() * (1 + 2.0 ** -9) + TINY[dt])
+
+
+@pytest.mark.parametrize("dt", ALL)
+def test_store_blocks_that_are_not_finite(dt):
+    mx = _mx()
+    x = torch.ones(3, 70, dtype=dt)
+    x[0, 3], x[1, 40], x[2, 69] = float("nan"), float("inf"), -float("inf")
+    c, s = mx.empty_checkpoint(3, 70, device=DEV)
+    mx.build_checkpoint(3, 70, NAME[dt])(x.to(DEV), c, s)
+    rc, rs = X.store8(x)
+    assert torch.equal(c.cpu(), rc) and torch.equal(s.cpu(), rs)
+    out = torch.zeros(3, 70, device=DEV, dtype=dt)
+    mx.build_checkpoint_restore(3, 70, "identity", NAME[dt])(c, s, out)
+    assert torch.equal(out.isnan().cpu(), X.load8(rc, rs, 70).isnan())
+
+
+def test_store_takes_tensors_that_start_between_vectors():
+    mx = _mx()
+    flat = _rand((1 + 6 * 64,), 5, dt=torch.bfloat16).to(DEV)
+    x = flat[1:].view(6, 64)  # contiguous, two bytes past a 16-byte boundary
+    c, s = mx.empty_checkpoint(6, 64, device=DEV)
+    mx.build_checkpoint(6, 64, "bfloat16")(x, c, s)
+    rc, rs = X.store8(x.cpu())
+    assert torch.equal(c.cpu(), rc) and torch.equal(s.cpu(), rs)
+    out = torch.zeros(1 + 6 * 64, device=DEV, dtype=torch.bfloat16)
+    mx.build_checkpoint_restore(6, 64, "relu", "bfloat16")(c, s, out[1:].view(6, 64))
+    assert torch.equal(out[1:].cpu().double().view(6, 64), X.load8(rc, rs, 64).clamp(min=0)) and out[0] == 0
+
+
+# ----------------------------------------------------------------------------------- products with a checkpoint
+SIZES = [(1, 1, 1), (10, 64, 1), (64, 784, 128), (10, 65, 17), (5, 8, 33), (128, 256, 256), (136, 264, 520),
+         (100, 129, 777), (72, 1000, 96), (256, 512, 1024), (48, 40, 2048), (384, 512, 264)]
+
+
+def _delta_case(M, K, B, dt, act, seed=0):
+    e = _rand((M, B), seed, 0.3, dt)
+    x = _rand((K, B), seed + 1, 1.5, dt)
+    c, s = _ckpt(x)
+    xhat = X.load8(c.cpu(), s.cpu(), B)
+    a = O.act_forward(act, xhat)
+    u = U[dt]
+    S = e.double().abs() @ a.abs().t()
+    err = (e.double().abs() @ (_act_err(act, xhat, dt) + u * a.abs() + TINY[dt]).t()) * (1 + 2.0 ** -8)
+    return e, c, s, e.double() @ a.t(), err + S * B * 2.0 ** -23
+
+
+@pytest.mark.parametrize("dt", ALL)
+@pytest.mark.parametrize("M,K,B", SIZES)
+def test_weight_delta(M, K, B, dt):
+    mx = _mx()
+    act = ACTS[(M + K + B) % 6]
+    e, c, s, ref, err = _delta_case(M, K, B, dt, act)
+    alpha = 1.0 / B
+    dw = torch.full((M, K), 7.0, device=DEV)
+    k = mx.build_weight_delta_checkpoint(M, K, B, act, NAME[dt], alpha)
+    k(dw, e.to(DEV), c, s)
+    _within(dw, alpha * ref, alpha * err + 2.0 ** -23 * alpha * ref.abs())
+    first = dw.clone()
+    k(dw, e.to(DEV), c, s, accumulate=True)
+    _within(dw, 2 * alpha * ref, 2 * alpha * err + 2.0 ** -22 * 2 * alpha * ref.abs())
+    k(dw, e.to(DEV), c, s)
+    assert torch.equal(dw, first)  # nothing left over from a call before
+    if dt is not torch.float32:
+        g = torch.full((M, K), 7.0, device=DEV, dtype=dt)
+        mx.build_weight_delta_checkpoint(M, K, B, act, NAME[dt], alpha, NAME[dt])(g, e.to(DEV), c, s)
+        _within(g, alpha * ref, (alpha * err) * (1 + U[dt]) + U[dt] * alpha * ref.abs() + TINY[dt])
+
+
+@pytest.mark.parametrize("dt", ALL)
+@pytest.mark.parametrize("M,K,B", SIZES)
+def test_weight_update(M, K, B, dt):
+    mx = _mx()
+    act = ACTS[(M + 2 * K + B) % 6]
+    e, c, s, ref, err = _delta_case(M, K, B, dt, act, 10)
+    w0 = _rand((M, K), 12, 0.05, dt)
+    w = w0.to(DEV)
+    mx.build_weight_update_checkpoint(M, K, B, act, NAME[dt], 0.01)(w, e.to(DEV), c, s)
+    want = w0.double() + 0.01 * ref
+    _within(w, want, (0.01 * err) * (1 + U[dt]) + (U[dt] + 2.0 ** -22) * (want.abs() + 0.01 * ref.abs()) + TINY[dt])
+
+
+@pytest.mark.parametrize("dt", ALL)
+@pytest.mark.parametrize("M,K,B", SIZES)
+@pytest.mark.parametrize("act", ACTS)
+def test_error_backward(M, K, B, dt, act):
+    mx = _mx()
+    w, e = _rand((M, K), 1, K ** -0.5, dt), _rand((M, B), 2, 0.3, dt)
+    c, s = _ckpt(_rand((K, B), 3, 1.5, dt))
+    xhat = X.load8(c.cpu(), s.cpu(), B)
+    up = torch.full((K, B), 7.0, device=DEV, dtype=dt)
+    mx.build_error_backward_checkpoint(M, K, B, act, NAME[dt])(w.to(DEV), e.to(DEV), c, s, up)
+    acc = w.double().t() @ e.double()
+    S = w.double().abs().t() @ e.double().abs()
+    ref = X.backward(w, e, xhat, act)
+    slope = X.slope(act, xhat).abs()
+    tol = _slope_err(act, xhat, dt) * (acc.abs() + S * M * 2.0 ** -23) + slope * S * M * 2.0 ** -23
+    _within(up, ref, tol * (1 + U[dt]) + (U[dt] + 2.0 ** -23) * ref.abs() + TINY[dt])
+
+
+def test_gradient_against_differences():
+    """The error sent up is the derivative of the layer's energy with respect to the states the checkpoint holds:
+    d/dx_j sum_i e_i (W f(x))_i, by central differences in 64 bits."""
+    mx = _mx()
+    M, K, B = 20, 24, 40
+    w, e = _rand((M, K), 4, 0.3), _rand((M, B), 5, 0.5)
+    c, s = _ckpt(_rand((K, B), 6, 1.0))
+    xhat = X.load8(c.cpu(), s.cpu(), B)
+    for act in ("tanh", "sigmoid", "silu", "gelu"):
+        up = torch.empty(K, B, device=DEV)
+        mx.build_error_backward_checkpoint(M, K, B, act, "float32")(w.to(DEV), e.to(DEV), c, s, up)
+        dw = torch.empty(M, K, device=DEV)
+        mx.build_weight_delta_checkpoint(M, K, B, act, "float32", 1.0)(dw, e.to(DEV), c, s)
+
+        def energy(ww, xx):
+            return (e.double() * (ww @ O.act_forward(act, xx))).sum()
+
+        h = 2.0 ** -17  # truncation h^2 |f'''| / 6 < 2^-34, rounding 2^-53 |energy| / h < 2^-28
+        for k, b in ((0, 0), (7, 13), (23, 39)):
+            d = torch.zeros(K, B, dtype=torch.float64)
+            d[k, b] = h
+            num = (energy(w.double(), xhat + d) - energy(w.double(), xhat - d)) / (2 * h)
+            assert abs(num - up[k, b].double().cpu()) < 2.0 ** -16
+            d = torch.zeros(M, K, dtype=torch.float64)
+            d[k % M, k] = h
+            num = (energy(w.double() + d, xhat) - energy(w.double() - d, xhat)) / (2 * h)
+            assert abs(num - dw[k % M, k].double().cpu()) < 2.0 ** -14
+
+
+def test_products_mark_states_that_were_not_finite():
+    mx = _mx()
+    M, K, B = 128, 256, 256
+    x = _rand((K, B), 1, 1.0, torch.bfloat16)
+    x[5, 40] = float("nan")
+    c, s = _ckpt(x)
+    w, e = _rand((M, K), 2, 0.1, torch.bfloat16).to(DEV), _rand((M, B), 3, 0.1, torch.bfloat16).to(DEV)
+    up = torch.zeros(K, B, device=DEV, dtype=torch.bfloat16)
+    mx.build_error_backward_checkpoint(M, K, B, "tanh", "bfloat16")(w, e, c, s, up)
+    want = torch.zeros(K, B, dtype=torch.bool)
+    want[5, 32:64] = True
+    assert torch.equal(up.isnan().cpu(), want)
+    dw = torch.zeros(M, K, device=DEV)
+    mx.build_weight_delta_checkpoint(M, K, B, "tanh", "bfloat16", 1.0)(dw, e, c, s)
+    assert dw[:, 5].isnan().all() and not dw[:, :5].isnan().any() and not dw[:, 6:].isnan().any()
+
+
+def test_empty_and_other_streams():
+    mx = _mx()
+    c, s = mx.empty_checkpoint(8, 0, device=DEV)
+    dw = torch.full((4, 8), 3.0, device=DEV)
+    mx.build_weight_delta_checkpoint(4, 8, 0, "tanh", "float16", 1.0)(
+        dw, torch.empty(4, 0, device=DEV, dtype=torch.float16), c, s)
+    assert not dw.any()  # an empty batch: no gradient
+    e, c, s, ref, err = _delta_case(128, 256, 512, torch.bfloat16, "tanh")
+    k = mx.build_weight_delta_checkpoint(128, 256, 512, "tanh", "bfloat16", 1.0)
+    outs = []
+    ed = e.to(DEV)
+    torch.cuda.synchronize()
+    for _ in range(3):  # one workspace a stream: calls on several streams at once do not meet
+        st = torch.cuda.Stream(DEV)
+        with torch.cuda.stream(st):
+            dw = torch.empty(128, 256, device=DEV)
+            k(dw, ed, c, s)
+            outs.append(dw)
+    torch.cuda.synchronize()
+    for dw in outs:
+        _within(dw, ref, err + 2.0 ** -23 * ref.abs())
+
+
+# ----------------------------------------------------------------------------------------------- 4-bit operands
+@pytest.mark.parametrize("dt", ALL)
+@pytest.mark.parametrize("turned", [False, True])
+@pytest.mark.parametrize("R,K", [(1, 1), (1, 784), (3, 31), (130, 33), (128, 128), (65, 300), (300, 777), (17, 1024)])
+def test_quantize_and_restore(R, K, turned, dt):
+    mx = _mx()
+    x = _states(K, R, 8, dt) if turned else _states(K, R, 8, dt).t().contiguous()
+    for act in ("identity", "relu"):
+        q, sc = mx.empty_mxfp4(R, K, device=DEV)
+        q.fill_(77), sc.fill_(77)
+        mx.build_mxfp4_quantize(R, K, act, NAME[dt], turned)(x.to(DEV), q, sc)
+        v = O.act_forward(act, x.double())
+        val, rq, rsc = X.quant4(v.t().contiguous() if turned else v)
+        assert torch.equal(sc.cpu(), rsc)  # padding rows and blocks too
+        out = torch.full((R, K), 9.0, device=DEV)
+        mx.build_mxfp4_restore(R, K, "float32")(q, sc, out)
+        assert torch.equal(out.cpu().double(), val)
+        differ = (q.cpu() != rq)  # a zero's sign bit may differ and stands for the same
+        assert ((q.cpu()[differ] & 0x77) == (rq[differ] & 0x77)).all()
+        for odt in HALF:
+            o = torch.full((R, K), 9.0, device=DEV, dtype=odt)
+            mx.build_mxfp4_restore(R, K, NAME[odt])(q, sc, o)
+            assert torch.equal(o.cpu(), val.to(odt))
+
+
+def test_quantize_of_other_activations():
+    """f(x) in 32 bits is off by a few ulp, so a code can only differ where f(x) is that near to a rounding boundary:
+    every value is one of the two neighbours of f(x) on its grid."""
+    mx = _mx()
+    R, K = 40, 200
+    x = _rand((K, R), 9, 1.5)
+    for act in ("tanh", "sigmoid", "silu", "gelu"):
+        q, sc = mx.empty_mxfp4(R, K, device=DEV)
+        mx.build_mxfp4_quantize(R, K, act, "float32", True)(x.to(DEV), q, sc)
+        out = torch.empty(R, K, device=DEV)
+        mx.build_mxfp4_restore(R, K, "float32")(q, sc, out)
+        v = O.act_forward(act, x.double()).t().contiguous()
+        val, _, _ = X.quant4(v)
+        same = out.cpu().double() == val
+        assert same.double().mean() > 1 - 2.0 ** -10
+        lo, hi = X.quant4(v * (1 - 2.0 ** -19))[0], X.quant4(v * (1 + 2.0 ** -19))[0]
+        o = out.cpu().double()
+        assert ((o == lo) | (o == hi) | same).all()
+
+
+def test_quantize_blocks_that_are_not_finite():
+    mx = _mx()
+    for turned in (False, True):
+        x = _rand((40, 200), 3, 1.0, torch.bfloat16)
+        x[7, 50], x[8, 199], x[39, 0] = float("nan"), float("inf"), -float("inf")
+        q, sc = mx.empty_mxfp4(40, 200, device=DEV)
+        mx.build_mxfp4_quantize(40, 200, "identity", "bfloat16", turned)((x.t().contiguous() if turned else x).to(DEV), q, sc)
+        val, _, rsc = X.quant4(x)
+        assert torch.equal(sc.cpu(), rsc)
+        out = torch.zeros(40, 200, device=DEV)
+        mx.build_mxfp4_restore(40, 200, "float32")(q, sc, out)
+        assert torch.equal(out.isnan().cpu(), val.isnan())
+
+
+FSIZES = [(1, 1, 1), (10, 64, 1), (1024, 1024, 1), (64, 784, 7), (129, 300, 16), (128, 128, 17), (10, 1024, 33),
+          (1000, 777, 300), (256, 256, 256), (130, 2000, 129), (300, 513, 520), (64, 40, 1000), (512, 1024, 264)]
+
+
+@pytest.mark.parametrize("dt", ALL)
+@pytest.mark.parametrize("M,K,B", FSIZES)
+def test_forward(M, K, B, dt):
+    mx = _mx()
+    w, wq, wsc = X.quant4(_rand((M, K), 1, K ** -0.5))
+    a, aq, asc = X.quant4(_rand((B, K), 2, 1.0))
+    out = torch.full((M, B), 9.0, device=DEV, dtype=dt)
+    mx.build_mxfp4_forward(M, K, B, NAME[dt])(wq.to(DEV), wsc.to(DEV), aq.to(DEV), asc.to(DEV), out)
+    ref = w @ a.t()
+    _within(out, ref, (w.abs() @ a.abs().t()) * K * 2.0 ** -23 + U[dt] * ref.abs() * (1 + 2.0 ** -8) + TINY[dt])
+
+
+@pytest.mark.parametrize("M,K,B", [(64, 256, 1), (256, 512, 256)])
+def test_forward_marks_what_was_not_finite(M, K, B):
+    mx = _mx()
+    w, a = _rand((M, K), 1), _rand((B, K), 2)
+    w[3, 100] = float("nan")
+    _, wq, wsc = X.quant4(w)
+    _, aq, asc = X.quant4(a)
+    out = torch.zeros(M, B, device=DEV)
+    mx.build_mxfp4_forward(M, K, B, "float32")(wq.to(DEV), wsc.to(DEV), aq.to(DEV), asc.to(DEV), out)
+    bad = out.isnan().cpu()
+    assert bad[3].all() and bad.sum() == B
