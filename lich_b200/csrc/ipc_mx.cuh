@@ -82,5 +82,7 @@ int launch_mx4_restore(const unsigned char* codes, const unsigned char* scales, 
                        cudaStream_t s);
 int launch_mx4_gemm(const unsigned char* w, const unsigned char* ws, const unsigned char* a, const unsigned char* as,
                     void* out, int M, int K, int B, int dtype, cudaStream_t s);
+// First error a bounded wait of the 4-bit product recorded (0 = none); clear != 0 resets it.
+int read_mx_status(int* status, int clear);
 
 }  // namespace ipc
