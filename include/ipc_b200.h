@@ -343,8 +343,11 @@ int ipc_mx8_restore(const signed char* codes, const unsigned char* scales, void*
  *   IPC_MODE_WEIGHT  W = cast(W + scale * E @ A^T)          (out = W [M, K], in/out)
  *   IPC_MODE_WDELTA  dw = scale * E @ A^T in fp32; IPC_FLAG_ACCUMULATE adds into dw
  *   IPC_MODE_WGRAD   out = cast(scale * E @ A^T) in `dtype`
- * The workspace (16-byte aligned; ipc_mx8_weight_ws_bytes gives its size) follows
- * the rules of ipc_fused_gemm_ws.  IPC_ALGO_OUTER is IPC_ERR_ARG.
+ * The workspace (16-byte aligned; *_ws_bytes gives its size, which may be 0) need
+ * not be initialised; calls that share one must be ordered on one stream.
+ * IPC_ALGO_AUTO runs large products on the tcgen05 GEMMs and the rest, of any
+ * size and alignment, in one launch of an mma.sync kernel (IPC_ALGO_SIMT asks for
+ * it); fp32 storage runs on the generic kernel.  IPC_ALGO_OUTER is IPC_ERR_ARG.
  */
 #define IPC_MODE_WGRAD 6
 int ipc_mx8_weight(int mode, void* out, const void* e, const signed char* codes, const unsigned char* scales, int M,
@@ -354,9 +357,12 @@ int ipc_mx8_weight_ws_bytes(int mode, int M, int K, int B, int dtype, int algo, 
 /*
  * Error of the layer above from its checkpoint (backpropagation through
  * mu = W f(x_up)):  e_up [K, B] = cast(f'(x^) * (W^T @ E)), w [M, K], e [M, B].
+ * Workspace and algorithms as for ipc_mx8_weight.
  */
 int ipc_mx8_backward(void* e_up, const void* w, const void* e, const signed char* codes, const unsigned char* scales,
-                     int M, int K, int B, int act, int dtype, int algo, void* stream);
+                     int M, int K, int B, int act, int dtype, int algo, void* workspace, size_t workspace_bytes,
+                     void* stream);
+int ipc_mx8_backward_ws_bytes(int M, int K, int B, int dtype, int algo, size_t* bytes);
 /*
  * codes, scales = the 4-bit operand of f(x) (f in fp32, not rounded before it
  * is stored): turned == 0 takes x [R, K] (weights), turned != 0 x [K, R]

@@ -49,6 +49,7 @@ EXPORTED = (
     "ipc_fused_gemm_ws", "ipc_weight_update_noalloc", "ipc_selftest_barrier_timeout", "ipc_set_max_ctas",
     "ipc_fused_gemm_ws_bytes", "ipc_fused_gemm_tuned", "ipc_weight_update_opt", "ipc_count_correct",
     "ipc_mx8_store", "ipc_mx8_restore", "ipc_mx8_weight", "ipc_mx8_weight_ws_bytes", "ipc_mx8_backward",
+    "ipc_mx8_backward_ws_bytes",
     "ipc_mxfp4_quantize", "ipc_mxfp4_restore", "ipc_mxfp4_forward",
 )
 
@@ -151,7 +152,8 @@ def load() -> ctypes.CDLL:
         "ipc_mx8_restore": (i, [vp, vp, vp, i, i, i, i, vp]),
         "ipc_mx8_weight": (i, [i, vp, vp, vp, vp, i, i, i, f, i, i, i, i, vp, c_size_t, vp]),
         "ipc_mx8_weight_ws_bytes": (i, [i, i, i, i, i, i, POINTER(c_size_t)]),
-        "ipc_mx8_backward": (i, [vp, vp, vp, vp, vp, i, i, i, i, i, i, vp]),
+        "ipc_mx8_backward": (i, [vp, vp, vp, vp, vp, i, i, i, i, i, i, vp, c_size_t, vp]),
+        "ipc_mx8_backward_ws_bytes": (i, [i, i, i, i, i, POINTER(c_size_t)]),
         "ipc_mxfp4_quantize": (i, [vp, vp, vp, i, i, i, i, i, vp]),
         "ipc_mxfp4_restore": (i, [vp, vp, vp, i, i, i, vp]),
         "ipc_mxfp4_forward": (i, [vp, vp, vp, vp, vp, i, i, i, i, vp]),

@@ -442,12 +442,43 @@ int ipc_mx8_restore(const signed char* codes, const unsigned char* scales, void*
   if (D == 0 || B == 0) return IPC_OK;
   IPC_REQUIRE(codes && scales && out, "null operand pointer");
   IPC_REQUIRE(aligned16(codes), "checkpoint codes must be 16-byte aligned");
-  return launch_mx8_restore(codes, scales, out, D, B, B, B, act, dtype, reinterpret_cast<cudaStream_t>(stream));
+  return launch_mx8_restore(codes, scales, out, D, B, B, act, dtype, reinterpret_cast<cudaStream_t>(stream));
 }
 
-// f(x) of a checkpoint read back into the head of the workspace (a multiple of 256 bytes)
-static size_t mx8_values_bytes(int K, int B, int dtype) {
-  return ((size_t)K * B * dt_size(dtype) + 255) / 256 * 256;
+// Products with a checkpoint.  Large ones run on the tcgen05 GEMMs, whose operands TMA loads: rows on 16-byte
+// boundaries.  So f(x^) is restored, and an operand with a row stride that is no multiple of 8 copied, into rows of the
+// workspace that are.  The rest (16-bit storage) is one launch of mx8_small_kernel, which needs none.
+constexpr double MX8_LARGE_WEIGHT = 3e8, MX8_LARGE_BACKWARD = 3e8;
+static bool mx8_large(int mode, int M, int K, int B, int dtype, int algo) {
+  if (dtype == IPC_DT_F32 || (algo != IPC_ALGO_AUTO && algo != IPC_ALGO_TCGEN05)) return false;
+  if (M < 1 || K < 1 || B < 1) return false;
+  if (algo == IPC_ALGO_TCGEN05) return true;
+  return (double)M * K * B >= (mode == MODE_BK ? MX8_LARGE_BACKWARD : MX8_LARGE_WEIGHT);
+}
+static long long up8(long long n) { return (n + 7) / 8 * 8; }
+static size_t up256(size_t n) { return (n + 255) / 256 * 256; }
+
+// workspace of a weight product: f(x^) [K][ld], E [M][ld] when B is no multiple of 8, the fp32 delta of a W update with
+// ragged rows, split-K partials
+struct Mx8WeightWs {
+  size_t values, e, delta, partial, total;
+  long long ld;
+};
+static Mx8WeightWs mx8_weight_ws(int mode, int M, int K, int B, int dtype, int algo) {
+  Mx8WeightWs w{};
+  if (M == 0 || K == 0 || B == 0) return w;
+  if (dtype == IPC_DT_F32) {
+    w.ld = B;
+    w.values = up256((size_t)K * B * 4);
+  } else if (mx8_large(mode, M, K, B, dtype, algo)) {
+    w.ld = up8(B);
+    w.values = up256((size_t)K * w.ld * 2);
+    w.e = B % 8 ? up256((size_t)M * w.ld * 2) : 0;
+    w.delta = (mode == MODE_W && K % 8) ? up256((size_t)M * K * 4) : 0;
+    w.partial = IPC_SPLITK_WS_BYTES;
+  }
+  w.total = w.values + w.e + w.delta + w.partial;
+  return w;
 }
 
 int ipc_mx8_weight_ws_bytes(int mode, int M, int K, int B, int dtype, int algo, size_t* bytes) {
@@ -455,8 +486,7 @@ int ipc_mx8_weight_ws_bytes(int mode, int M, int K, int B, int dtype, int algo, 
   if (rc) return rc;
   IPC_REQUIRE(mode == IPC_MODE_WEIGHT || mode == IPC_MODE_WDELTA || mode == IPC_MODE_WGRAD, "not a weight mode: %d", mode);
   IPC_REQUIRE(bytes != nullptr, "null result pointer");
-  *bytes = mx8_values_bytes(K, B, dtype);
-  if (B > 16 && tc_eligible(mode, M, K, B, dtype, algo, false, true)) *bytes += IPC_SPLITK_WS_BYTES;
+  *bytes = mx8_weight_ws(mode, M, K, B, dtype, algo).total;
   return IPC_OK;
 }
 
@@ -472,38 +502,81 @@ int ipc_mx8_weight(int mode, void* out, const void* e, const signed char* codes,
   if (M == 0 || K == 0) return IPC_OK;
   IPC_REQUIRE(out && (B == 0 || (e && codes && scales)), "null operand pointer");
   IPC_REQUIRE(aligned16(codes), "checkpoint codes must be 16-byte aligned");
-  const size_t need = mx8_values_bytes(K, B, dtype);
-  IPC_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), "workspace of %lld bytes, %lld needed (ipc_mx8_weight_ws_bytes)",
-              (long long)workspace_bytes, (long long)need);
+  const Mx8WeightWs w = mx8_weight_ws(mode, M, K, B, dtype, algo);
+  IPC_REQUIRE(w.total == 0 || (workspace && workspace_bytes >= w.total),
+              "workspace of %lld bytes, %lld needed (ipc_mx8_weight_ws_bytes)", (long long)workspace_bytes, (long long)w.total);
   IPC_REQUIRE(aligned16(workspace), "workspace must be 16-byte aligned");
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  if (B > 0) {
-    rc = launch_mx8_restore(codes, scales, workspace, K, B, B, B, act, dtype, s);
-    if (rc) return rc;
-  }
   GemmArgs p{};
   p.A = e; p.lda = B; p.gsA = (long long)M * B;
-  p.Bm = workspace; p.ldb = B; p.gsB = (long long)K * B;
   p.Mg = M; p.Ng = K; p.Kg = B; p.groups = 1;
   p.out = out; p.gsOut = (long long)M * K;
   p.scale = scale;
   p.accumulate = (flags & IPC_FLAG_ACCUMULATE) != 0;
-  const size_t rest = workspace_bytes - need;
-  if (B > 16 && tc_eligible(mode, M, K, B, dtype, algo, false, rest > 0))
-    return launch_tc(p, mode, act, dtype, s, rest ? reinterpret_cast<float*>(static_cast<char*>(workspace) + need) : nullptr, rest);
-  if (algo == IPC_ALGO_TCGEN05)
-    return set_error(IPC_ERR_UNSUPPORTED, "tcgen05 path: not eligible (M=%d K=%d B=%d dtype=%d)", M, K, B, dtype);
-  return launch_generic(p, mode, false, act, dtype, s);
+  p.ck = codes; p.cks = scales; p.ld_ck = mx8_ld(B);
+  if (dtype == IPC_DT_F32) {
+    if (algo == IPC_ALGO_TCGEN05) return set_error(IPC_ERR_UNSUPPORTED, "tcgen05 path: 16-bit storage only");
+    if (B > 0) rc = launch_mx8_restore(codes, scales, workspace, K, B, B, act, dtype, s);
+    if (rc) return rc;
+    p.Bm = workspace; p.ldb = B; p.gsB = (long long)K * B;
+    return launch_generic(p, mode, false, act, dtype, s);
+  }
+  const bool direct = B % 8 == 0;
+  // (tensors that start between 16-byte boundaries though their rows would not: rare, and no copy is planned for them)
+  if (w.values == 0 || (direct && !aligned16(e)) || (mode == MODE_W && K % 8 == 0 && !aligned16(out)))
+    return launch_mx8_small(p, mode, act, dtype, s);
+  char* ws = static_cast<char*>(workspace);
+  rc = launch_mx8_restore(codes, scales, ws, K, B, w.ld, act, dtype, s);
+  if (rc) return rc;
+  if (!direct) {
+    rc = launch_mx8_pack(e, ws + w.values, M, B, w.ld, s);
+    if (rc) return rc;
+    p.A = ws + w.values;
+  }
+  p.lda = w.ld; p.gsA = (long long)M * w.ld;
+  p.Bm = ws; p.ldb = w.ld; p.gsB = (long long)K * w.ld;
+  p.ck = nullptr;
+  float* part = reinterpret_cast<float*>(ws + w.values + w.e + w.delta);
+  if (aligned16(out) && K % 8 == 0) return launch_tc(p, mode, act, dtype, s, part, w.partial);
+  p.ragged = 1;
+  if (mode != MODE_W) return launch_tc(p, mode, act, dtype, s, part, w.partial);
+  p.out = ws + w.values + w.e;  // W with ragged rows: the fp32 delta, then W += delta
+  rc = launch_tc(p, MODE_WD, act, dtype, s, part, w.partial);
+  if (rc) return rc;
+  return launch_apply(out, static_cast<const float*>(p.out), (long long)M * K, dtype, s);
+}
+
+// workspace of the error product: W [M][lw] when K is no multiple of 8, E [M][le] when B is none
+static size_t mx8_backward_ws(int M, int K, int B, int dtype, int algo, size_t* w_bytes) {
+  *w_bytes = 0;
+  if (!mx8_large(MODE_BK, M, K, B, dtype, algo)) return 0;
+  *w_bytes = K % 8 ? up256((size_t)M * up8(K) * 2) : 0;
+  return *w_bytes + (B % 8 ? up256((size_t)M * up8(B) * 2) : 0);
+}
+
+int ipc_mx8_backward_ws_bytes(int M, int K, int B, int dtype, int algo, size_t* bytes) {
+  int rc = common_checks(M, K, B, 1, IPC_ACT_IDENTITY, dtype, algo);
+  if (rc) return rc;
+  IPC_REQUIRE(bytes != nullptr, "null result pointer");
+  size_t w;
+  *bytes = mx8_backward_ws(M, K, B, dtype, algo, &w);
+  return IPC_OK;
 }
 
 int ipc_mx8_backward(void* e_up, const void* w, const void* e, const signed char* codes, const unsigned char* scales,
-                     int M, int K, int B, int act, int dtype, int algo, void* stream) {
+                     int M, int K, int B, int act, int dtype, int algo, void* workspace, size_t workspace_bytes,
+                     void* stream) {
   int rc = common_checks(M, K, B, 1, act, dtype, algo);
   if (rc) return rc;
   IPC_REQUIRE(algo != IPC_ALGO_OUTER, "IPC_ALGO_OUTER applies to the weight update only");
   if (K == 0 || B == 0) return IPC_OK;
   IPC_REQUIRE(e_up && codes && scales && (M == 0 || (w && e)), "null operand pointer");
   IPC_REQUIRE(aligned16(codes), "checkpoint codes must be 16-byte aligned");
+  size_t w_bytes;
+  const size_t need = mx8_backward_ws(M, K, B, dtype, algo, &w_bytes);
+  IPC_REQUIRE(need == 0 || (workspace && workspace_bytes >= need),
+              "workspace of %lld bytes, %lld needed (ipc_mx8_backward_ws_bytes)", (long long)workspace_bytes, (long long)need);
+  IPC_REQUIRE(aligned16(workspace), "workspace must be 16-byte aligned");
   GemmArgs p{};
   p.A = w; p.lda = K; p.gsA = (long long)M * K;
   p.Bm = e; p.ldb = B; p.gsB = (long long)M * B;
@@ -511,11 +584,25 @@ int ipc_mx8_backward(void* e_up, const void* w, const void* e, const signed char
   p.out = e_up; p.gsOut = (long long)K * B;
   p.ck = codes; p.cks = scales; p.ld_ck = mx8_ld(B);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  if (tc_eligible(MODE_BK, K, M, B, dtype, algo, false)) return launch_tc(p, MODE_BK, act, dtype, s);
-  if (algo == IPC_ALGO_TCGEN05)
-    return set_error(IPC_ERR_UNSUPPORTED, "tcgen05 path: not eligible (M=%d K=%d B=%d dtype=%d)", M, K, B, dtype);
-  if (skinny_eligible(MODE_BK, K, M, B, dtype, algo)) return launch_skinny(p, MODE_BK, false, act, dtype, s);
-  return launch_generic(p, MODE_BK, false, act, dtype, s);
+  if (dtype == IPC_DT_F32) {
+    if (algo == IPC_ALGO_TCGEN05) return set_error(IPC_ERR_UNSUPPORTED, "tcgen05 path: 16-bit storage only");
+    return launch_generic(p, MODE_BK, false, act, dtype, s);
+  }
+  const bool wide = mx8_large(MODE_BK, M, K, B, dtype, algo) && (K % 8 || aligned16(w)) && (B % 8 || aligned16(e));
+  if (!wide) return launch_mx8_small(p, MODE_BK, act, dtype, s);
+  char* ws = static_cast<char*>(workspace);
+  if (K % 8) {
+    rc = launch_mx8_pack(w, ws, M, K, up8(K), s);
+    if (rc) return rc;
+    p.A = ws; p.lda = up8(K); p.gsA = M * p.lda;
+  }
+  if (B % 8) {
+    rc = launch_mx8_pack(e, ws + w_bytes, M, B, up8(B), s);
+    if (rc) return rc;
+    p.Bm = ws + w_bytes; p.ldb = up8(B); p.gsB = M * p.ldb;
+  }
+  p.ragged = B % 8 != 0 || !aligned16(e_up);
+  return launch_tc(p, MODE_BK, act, dtype, s);
 }
 
 int ipc_mxfp4_quantize(const void* x, unsigned char* codes, unsigned char* scales, int R, int K, int turned, int act,

@@ -68,6 +68,7 @@ struct GemmArgs {
   const signed char* ck;     // BK: 8-bit checkpoint of the [Mg, Ng] states, codes ld_ck apart, 16-byte aligned ...
   const unsigned char* cks;  // ... and its scale bytes [ceil(Ng / 32)][Mg]  (ipc_mx.cuh)
   long long ld_ck;
+  int ragged;       // WD, G, BK: rows of out start anywhere (odd Ng, or a view); lda and ldb still suit TMA
 };
 
 int launch_generic(const GemmArgs& p, int mode, bool bact, int act, int dtype, cudaStream_t s);

@@ -1,8 +1,10 @@
 // Storing and reading back microscaled operands (formats and layouts: ipc_mx.cuh).
 //
-// All four kernels are bound by memory: every input element is read once, every code and scale byte written
-// once.  A CTA owns a tile of 32 rows x 256 columns, so that the scale bytes of a tile, which lie across the rows in
-// both layouts, leave as whole sectors.
+// These kernels are bound by memory: every input element is read once, every code and scale byte written once.  A CTA
+// owns a tile of 32 rows x 256 columns, so that the scale bytes of a tile, which lie across the rows in both layouts,
+// leave as whole sectors.  A thread moves one 16-byte vector of the 16- or 32-bit side, so that a warp instruction covers
+// whole sectors (with two vectors a thread the stores of a restore reach L2 as half sectors: 22 us against 17 us for 8-bit
+// codes at 4096 x 8192 in bf16).  Rows that do not start on 16-byte boundaries take a lane per element.
 #include "ipc_mx.cuh"
 
 namespace ipc {
@@ -14,26 +16,37 @@ constexpr int THREADS = 256;
 constexpr int TB = TCOL / MX_BLOCK;
 
 template <typename T>
-struct Vec16 {  // 16 consecutive elements
-  static __device__ __forceinline__ void load(const T* p, float (&v)[16]) {
-    constexpr int N = 16 / sizeof(T);
-    uint4 raw[16 / N];
+struct Vec {  // one 16-byte vector
+  static constexpr int N = 16 / sizeof(T);
+  static __device__ __forceinline__ void load(const T* p, float (&v)[N]) {
+    const uint4 raw = __ldg(reinterpret_cast<const uint4*>(p));
+    const T* h = reinterpret_cast<const T*>(&raw);
 #pragma unroll
-    for (int i = 0; i < 16 / N; ++i) raw[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
-    const T* h = reinterpret_cast<const T*>(raw);
-#pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] = St<T>::ld(h[j]);
+    for (int j = 0; j < N; ++j) v[j] = St<T>::ld(h[j]);
   }
-  static __device__ __forceinline__ void store(T* p, const float (&v)[16]) {
-    constexpr int N = 16 / sizeof(T);
-    uint4 raw[16 / N];
-    T* h = reinterpret_cast<T*>(raw);
+  static __device__ __forceinline__ void store(T* p, const float (&v)[N]) {
+    uint4 raw;
+    T* h = reinterpret_cast<T*>(&raw);
 #pragma unroll
-    for (int j = 0; j < 16; ++j) h[j] = St<T>::st(v[j]);
-#pragma unroll
-    for (int i = 0; i < 16 / N; ++i) reinterpret_cast<uint4*>(p)[i] = raw[i];
+    for (int j = 0; j < N; ++j) h[j] = St<T>::st(v[j]);
+    *reinterpret_cast<uint4*>(p) = raw;
   }
 };
+// N codes (bytes) moved at once
+__device__ __forceinline__ void ld_codes(const void* p, uint32_t (&w)[2]) {
+  const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
+  w[0] = v.x; w[1] = v.y;
+}
+__device__ __forceinline__ void ld_codes(const void* p, uint32_t (&w)[1]) { w[0] = __ldg(reinterpret_cast<const uint32_t*>(p)); }
+__device__ __forceinline__ void st_codes(void* p, const uint32_t (&w)[2]) { *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]); }
+__device__ __forceinline__ void st_codes(void* p, const uint32_t (&w)[1]) { *reinterpret_cast<uint32_t*>(p) = w[0]; }
+// the largest of a block's magnitudes, the block spread over G neighbouring lanes
+template <int G>
+__device__ __forceinline__ uint32_t group_max(uint32_t m) {
+#pragma unroll
+  for (int o = 1; o < G; o *= 2) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+  return m;
+}
 
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
@@ -59,8 +72,7 @@ __device__ __forceinline__ float act_for(float v) {
 }
 
 // ---------------------------------------------------------------------------- 8 bits
-// VEC: rows start on 16-byte boundaries; a thread takes 16 elements, two threads a block.  Otherwise a lane
-// takes one element of a block, so that loads and stores stay coalesced whatever the row stride.
+// VEC: rows start on 16-byte boundaries (so B is a multiple of a vector); 4 threads a block (8 in fp32).
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(THREADS) mx8_store_kernel(const T* __restrict__ x, signed char* __restrict__ codes,
                                                             unsigned char* __restrict__ scales, int D, int B, int nb) {
@@ -69,40 +81,31 @@ __global__ void __launch_bounds__(THREADS) mx8_store_kernel(const T* __restrict_
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const long long ldc = (long long)nb * MX_BLOCK;
   if constexpr (VEC) {
-    const int cj = tid & 15, r0 = tid >> 4;
+    constexpr int N = Vec<T>::N, TPR = TCOL / N, RPI = THREADS / TPR;  // threads a row, rows at a time
+    const int c = c0 + N * (tid % TPR);
 #pragma unroll
-    for (int it = 0; it < TR / 16; ++it) {
-      const int r = r0 + 16 * it, d = d0 + r, c = c0 + 16 * cj;
-      float v[16];
+    for (int it = 0; it < TR / RPI; ++it) {
+      const int r = tid / TPR + RPI * it, d = d0 + r;
+      float v[N];
+#pragma unroll
+      for (int j = 0; j < N; ++j) v[j] = 0.f;
+      if (d < D && c < B) Vec<T>::load(x + (long long)d * B + c, v);
       uint32_t m = 0;
-      if (d < D && c < B) {
-        if (c + 16 <= B) {
-          Vec16<T>::load(x + (long long)d * B + c, v);
-        } else {
 #pragma unroll
-          for (int j = 0; j < 16; ++j) v[j] = c + j < B ? St<T>::ld(x[(long long)d * B + c + j]) : 0.f;
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 16; ++j) v[j] = 0.f;
-      }
-#pragma unroll
-      for (int j = 0; j < 16; ++j) m = max(m, abs_bits(v[j]));
-      m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-      const uint32_t byte = mx8_scale_byte(m);
+      for (int j = 0; j < N; ++j) m = max(m, abs_bits(v[j]));
+      const uint32_t byte = mx8_scale_byte(group_max<MX_BLOCK / N>(m));
       const float inv = mx_inv_scale(byte);
-      if ((cj & 1) == 0) s_scale[cj >> 1][r] = (unsigned char)byte;
+      if (c % MX_BLOCK == 0) s_scale[(c - c0) / MX_BLOCK][r] = (unsigned char)byte;
       if (d < D && c < ldc) {
-        uint4 o;
-        uint32_t* w = reinterpret_cast<uint32_t*>(&o);
+        uint32_t w[N / 4];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
+        for (int q = 0; q < N / 4; ++q) {
           uint32_t t = 0;
 #pragma unroll
           for (int j = 0; j < 4; ++j) t |= ((uint32_t)mx8_code(v[4 * q + j], inv) & 0xffu) << (8 * j);
           w[q] = t;
         }
-        *reinterpret_cast<uint4*>(codes + (long long)d * ldc + c) = o;
+        st_codes(codes + (long long)d * ldc + c, w);
       }
     }
   } else {
@@ -131,34 +134,31 @@ __global__ void __launch_bounds__(THREADS) mx8_store_kernel(const T* __restrict_
 template <typename T, int ACT, bool VEC>
 __global__ void __launch_bounds__(THREADS)
     mx8_restore_kernel(const signed char* __restrict__ codes, const unsigned char* __restrict__ scales,
-                       T* __restrict__ out, int D, int B, int nb, long long ld_out, int pad_cols) {
+                       T* __restrict__ out, int D, int cols, int nb, long long ld_out) {
   const int d0 = blockIdx.y * TR, c0 = blockIdx.x * TCOL;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const long long ldc = (long long)nb * MX_BLOCK;
   if constexpr (VEC) {
-    const int cj = tid & 15, r0 = tid >> 4;
+    constexpr int N = Vec<T>::N, TPR = TCOL / N, RPI = THREADS / TPR;
+    const int c = c0 + N * (tid % TPR);
 #pragma unroll
-    for (int it = 0; it < TR / 16; ++it) {
-      const int d = d0 + r0 + 16 * it, c = c0 + 16 * cj;
-      if (d >= D || c >= pad_cols) continue;
-      float v[16];
-      if (c < ldc) {
-        const uint4 raw = __ldg(reinterpret_cast<const uint4*>(codes + (long long)d * ldc + c));
-        const float sc = mx_scale(scales[(long long)(c / MX_BLOCK) * D + d]);
-        const signed char* q = reinterpret_cast<const signed char*>(&raw);
+    for (int it = 0; it < TR / RPI; ++it) {
+      const int d = d0 + tid / TPR + RPI * it;
+      if (d >= D || c >= cols) continue;
+      uint32_t w[N / 4];
+      ld_codes(codes + (long long)d * ldc + c, w);
+      const float sc = mx_scale(scales[(long long)(c / MX_BLOCK) * D + d]);
+      const signed char* q = reinterpret_cast<const signed char*>(w);
+      float v[N];
 #pragma unroll
-        for (int j = 0; j < 16; ++j) v[j] = c + j < B ? act_for<T, ACT>((float)q[j] * sc) : 0.f;
-      } else {
-#pragma unroll
-        for (int j = 0; j < 16; ++j) v[j] = 0.f;
-      }
+      for (int j = 0; j < N; ++j) v[j] = act_for<T, ACT>((float)q[j] * sc);
       T* o = out + (long long)d * ld_out + c;
-      if (c + 16 <= pad_cols) {
-        Vec16<T>::store(o, v);
+      if (c + N <= cols) {
+        Vec<T>::store(o, v);
       } else {
 #pragma unroll
-        for (int j = 0; j < 16; ++j)
-          if (c + j < pad_cols) o[j] = St<T>::st(v[j]);
+        for (int j = 0; j < N; ++j)
+          if (c + j < cols) o[j] = St<T>::st(v[j]);
       }
     }
   } else {
@@ -168,12 +168,9 @@ __global__ void __launch_bounds__(THREADS)
 #pragma unroll
       for (int j = 0; j < TB; ++j) {
         const int c = c0 + MX_BLOCK * j + lane;
-        if (c >= pad_cols) continue;
-        float v = 0.f;
-        if (c < B)
-          v = act_for<T, ACT>((float)codes[(long long)d * ldc + c] *
-                              mx_scale(scales[(long long)(c / MX_BLOCK) * D + d]));
-        out[(long long)d * ld_out + c] = St<T>::st(v);
+        if (c >= cols) continue;
+        out[(long long)d * ld_out + c] = St<T>::st(act_for<T, ACT>(
+            (float)codes[(long long)d * ldc + c] * mx_scale(scales[(long long)(c / MX_BLOCK) * D + d])));
       }
     }
   }
@@ -186,40 +183,59 @@ __global__ void __launch_bounds__(THREADS) mx4_rows_kernel(const T* __restrict__
                                                            unsigned char* __restrict__ scales, int R, int K, int kp) {
   __shared__ __align__(16) unsigned char s_scale[TR][TB];
   const int r0 = blockIdx.y * TR, c0 = blockIdx.x * TCOL;
-  const int tid = threadIdx.x;
-  const int cj = tid & 15, rr = tid >> 4;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if constexpr (VEC) {
+    constexpr int N = 8, TPR = TCOL / N, RPI = THREADS / TPR;  // 8 codes: 4 bytes a thread
+    const int c = c0 + N * (tid % TPR);
 #pragma unroll
-  for (int it = 0; it < TR / 16; ++it) {
-    const int r = r0 + rr + 16 * it, c = c0 + 16 * cj;
-    float v[16];
+    for (int it = 0; it < TR / RPI; ++it) {
+      const int rr = tid / TPR + RPI * it, r = r0 + rr;
+      float v[N];
 #pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] = 0.f;
-    if (r < R && c < K) {
-      if (VEC && c + 16 <= K) {
-        Vec16<T>::load(x + (long long)r * K + c, v);
-      } else {
+      for (int j = 0; j < N; ++j) v[j] = 0.f;
+      if (r < R) {  // (K is a multiple of a vector)
 #pragma unroll
-        for (int j = 0; j < 16; ++j)
-          if (c + j < K) v[j] = St<T>::ld(x[(long long)r * K + c + j]);
+        for (int h = 0; h < N; h += Vec<T>::N)
+          if (c + h < K) {
+            float u[Vec<T>::N];
+            Vec<T>::load(x + (long long)r * K + c + h, u);
+#pragma unroll
+            for (int j = 0; j < Vec<T>::N; ++j) v[h + j] = act_full<ACT>(u[j]);
+          }
       }
+      uint32_t m = 0;
 #pragma unroll
-      for (int j = 0; j < 16; ++j) v[j] = c + j < K ? act_full<ACT>(v[j]) : 0.f;
+      for (int j = 0; j < N; ++j) m = max(m, abs_bits(v[j]));
+      const uint32_t byte = mx4_scale_byte(group_max<MX_BLOCK / N>(m));
+      if (c % MX_BLOCK == 0) s_scale[rr][(c - c0) / MX_BLOCK] = (unsigned char)byte;
+      if (r < R && c < kp) {
+        const float inv = mx_inv_scale(byte);
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[j] = byte == MX_NAN_BYTE ? 0.f : v[j] * inv;
+        *reinterpret_cast<uint32_t*>(codes + (long long)r * (kp / 2) + c / 2) = mx4_pack8(v);
+      }
     }
-    uint32_t m = 0;
+  } else {
+    for (int rr = warp; rr < TR; rr += THREADS / 32) {
+      const int r = r0 + rr;
+      float v[TB];
 #pragma unroll
-    for (int j = 0; j < 16; ++j) m = max(m, abs_bits(v[j]));
-    m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-    const uint32_t byte = mx4_scale_byte(m);
-    if ((cj & 1) == 0) s_scale[rr + 16 * it][cj >> 1] = (unsigned char)byte;
-    if (r < R && c < kp) {
-      const float inv = mx_inv_scale(byte);
-      float a[8], b[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        a[j] = byte == MX_NAN_BYTE ? 0.f : v[j] * inv;
-        b[j] = byte == MX_NAN_BYTE ? 0.f : v[8 + j] * inv;
+      for (int j = 0; j < TB; ++j) {
+        const int c = c0 + MX_BLOCK * j + lane;
+        v[j] = (r < R && c < K) ? St<T>::ld(x[(long long)r * K + c]) : 0.f;
       }
-      *reinterpret_cast<uint2*>(codes + (long long)r * (kp / 2) + c / 2) = make_uint2(mx4_pack8(a), mx4_pack8(b));
+#pragma unroll
+      for (int j = 0; j < TB; ++j) {
+        const int c = c0 + MX_BLOCK * j + lane;
+        if (ACT != IPC_ACT_RELU && ACT != IPC_ACT_IDENTITY) v[j] = (r < R && c < K) ? act_full<ACT>(v[j]) : 0.f;
+        else v[j] = act_full<ACT>(v[j]);
+        const uint32_t byte = mx4_scale_byte(__reduce_max_sync(0xffffffffu, abs_bits(v[j])));
+        if (lane == 0) s_scale[rr][j] = (unsigned char)byte;
+        const float lo = byte == MX_NAN_BYTE ? 0.f : v[j] * mx_inv_scale(byte);
+        const float hi = __shfl_down_sync(0xffffffffu, lo, 1);
+        if ((lane & 1) == 0 && r < R && c < kp)
+          codes[(long long)r * (kp / 2) + c / 2] = (unsigned char)mx4_pack2(lo, hi);
+      }
     }
   }
   __syncthreads();
@@ -234,10 +250,35 @@ __global__ void __launch_bounds__(THREADS) mx4_rows_kernel(const T* __restrict__
 }
 
 // Turned ([K, R] feature-major states -> R rows of K): a CTA takes 256 features x 64 samples; a warp a block of
-// 32 features, a lane two samples, whose 32 values it reads along the samples (coalesced) and keeps in registers.
-// The codes pass through shared memory so that a sample's 128 bytes leave together.
+// 32 features, a lane two samples, whose 32 values it reads along the samples (a warp instruction takes 128 bytes of a
+// feature) and keeps in registers, so that a block's magnitude and codes need no exchange.  The codes pass through
+// shared memory, so that a sample's 128 bytes leave together.
+// PAIR: rows start on boundaries of two elements and a lane takes two neighbouring samples; otherwise samples lane, lane + 32.
 constexpr int TUR = 64;
-template <typename T, int ACT>
+template <typename T, bool PAIR>
+struct alignas(2 * sizeof(T)) Two {  // an element of each of a lane's two samples
+  T v[2];
+};
+template <typename T, bool PAIR>
+__device__ __forceinline__ Two<T, PAIR> load_two(const T* row, int lane, bool in0, bool in1) {
+  Two<T, PAIR> t;
+  if constexpr (PAIR) {
+    if constexpr (sizeof(T) == 2) {
+      uint32_t w = 0;
+      if (in0) w = __ldg(reinterpret_cast<const uint32_t*>(row + 2 * lane));  // R is even: both or none
+      *reinterpret_cast<uint32_t*>(t.v) = w;
+    } else {
+      uint2 w = make_uint2(0, 0);
+      if (in0) w = __ldg(reinterpret_cast<const uint2*>(row + 2 * lane));
+      *reinterpret_cast<uint2*>(t.v) = w;
+    }
+  } else {
+    t.v[0] = in0 ? row[lane] : St<T>::st(0.f);
+    t.v[1] = in1 ? row[lane + 32] : St<T>::st(0.f);
+  }
+  return t;
+}
+template <typename T, int ACT, bool PAIR>
 __global__ void __launch_bounds__(THREADS) mx4_turned_kernel(const T* __restrict__ x, unsigned char* __restrict__ codes,
                                                              unsigned char* __restrict__ scales, int R, int K, int kp) {
   __shared__ __align__(16) unsigned char s_code[TUR][144];  // 128 bytes of codes per sample, rows 16 bytes apart mod 128
@@ -245,18 +286,27 @@ __global__ void __launch_bounds__(THREADS) mx4_turned_kernel(const T* __restrict
   const int r0 = blockIdx.x * TUR, k0 = blockIdx.y * TCOL;  // neighbouring CTAs read neighbouring samples
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int kb = k0 + MX_BLOCK * warp;
+  const int rl[2] = {PAIR ? 2 * lane : lane, PAIR ? 2 * lane + 1 : lane + 32};
+  const bool in[2] = {r0 + rl[0] < R, r0 + rl[1] < R};
+  const T* src = x + (long long)kb * R + r0;
+  Two<T, PAIR> v[MX_BLOCK];
+  if (kb + MX_BLOCK <= K) {
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int r = r0 + 32 * h + lane;
-    float v[MX_BLOCK];
+    for (int i = 0; i < MX_BLOCK; ++i) v[i] = load_two<T, PAIR>(src + (long long)i * R, lane, in[0], in[1]);
+  } else {
 #pragma unroll
     for (int i = 0; i < MX_BLOCK; ++i)
-      v[i] = (r < R && kb + i < K) ? St<T>::ld(x[(long long)(kb + i) * R + r]) : 0.f;
+      v[i] = load_two<T, PAIR>(src + (long long)i * R, lane, in[0] && kb + i < K, in[1] && kb + i < K);
+  }
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    float f[MX_BLOCK];
     uint32_t m = 0;
 #pragma unroll
     for (int i = 0; i < MX_BLOCK; ++i) {
-      v[i] = (r < R && kb + i < K) ? act_full<ACT>(v[i]) : 0.f;
-      m = max(m, abs_bits(v[i]));
+      f[i] = act_full<ACT>(St<T>::ld(v[i].v[h]));
+      if (ACT == IPC_ACT_SIGMOID && !(in[h] && kb + i < K)) f[i] = 0.f;  // (the other f are 0 at 0)
+      m = max(m, abs_bits(f[i]));
     }
     const uint32_t byte = mx4_scale_byte(m);
     const float inv = mx_inv_scale(byte);
@@ -266,11 +316,11 @@ __global__ void __launch_bounds__(THREADS) mx4_turned_kernel(const T* __restrict
     for (int q = 0; q < 4; ++q) {
       float a[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) a[j] = byte == MX_NAN_BYTE ? 0.f : v[8 * q + j] * inv;
+      for (int j = 0; j < 8; ++j) a[j] = byte == MX_NAN_BYTE ? 0.f : f[8 * q + j] * inv;
       w[q] = mx4_pack8(a);
     }
-    *reinterpret_cast<uint4*>(&s_code[32 * h + lane][16 * warp]) = o;
-    s_scale[32 * h + lane][warp] = (unsigned char)byte;
+    *reinterpret_cast<uint4*>(&s_code[rl[h]][16 * warp]) = o;
+    s_scale[rl[h]][warp] = (unsigned char)byte;
   }
   __syncthreads();
 #pragma unroll
@@ -294,32 +344,57 @@ __global__ void __launch_bounds__(THREADS) mx4_restore_kernel(const unsigned cha
                                                               const unsigned char* __restrict__ scales,
                                                               T* __restrict__ out, int R, int K, int kp) {
   const int r0 = blockIdx.y * TR, c0 = blockIdx.x * TCOL;
-  const int tid = threadIdx.x;
-  const int cj = tid & 15, rr = tid >> 4;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if constexpr (VEC) {
+    constexpr int N = 8, TPR = TCOL / N, RPI = THREADS / TPR;
+    const int c = c0 + N * (tid % TPR);
 #pragma unroll
-  for (int it = 0; it < TR / 16; ++it) {
-    const int r = r0 + rr + 16 * it, c = c0 + 16 * cj;
-    if (r >= R || c >= K) continue;
-    const uint2 q = __ldg(reinterpret_cast<const uint2*>(codes + (long long)r * (kp / 2) + c / 2));
-    const float sc = mx_scale(scales[mx4_scale_at(r, c / MX_BLOCK, kp / 128)]);
-    uint32_t h[8];
-    mx4_unpack8(q.x, reinterpret_cast<uint32_t(&)[4]>(h[0]));
-    mx4_unpack8(q.y, reinterpret_cast<uint32_t(&)[4]>(h[4]));
-    float v[16];
+    for (int it = 0; it < TR / RPI; ++it) {
+      const int r = r0 + tid / TPR + RPI * it;
+      if (r >= R || c >= K) continue;
+      const uint32_t q = __ldg(reinterpret_cast<const uint32_t*>(codes + (long long)r * (kp / 2) + c / 2));
+      const float sc = mx_scale(scales[mx4_scale_at(r, c / MX_BLOCK, kp / 128)]);
+      uint32_t h[4];
+      mx4_unpack8(q, h);
+      float v[N];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[j]));
-      v[2 * j] = f.x * sc;
-      v[2 * j + 1] = f.y * sc;
+      for (int j = 0; j < 4; ++j) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[j]));
+        v[2 * j] = f.x * sc;
+        v[2 * j + 1] = f.y * sc;
+      }
+#pragma unroll
+      for (int g = 0; g < N; g += Vec<T>::N)  // (K is a multiple of a vector)
+        if (c + g < K) Vec<T>::store(out + (long long)r * K + c + g, *reinterpret_cast<float(*)[Vec<T>::N]>(v + g));
     }
-    T* o = out + (long long)r * K + c;
-    if (VEC && c + 16 <= K) {
-      Vec16<T>::store(o, v);
-    } else {
+  } else {
+    for (int r = r0 + warp; r < r0 + TR && r < R; r += THREADS / 32) {
 #pragma unroll
-      for (int j = 0; j < 16; ++j)
-        if (c + j < K) o[j] = St<T>::st(v[j]);
+      for (int j = 0; j < TB; ++j) {
+        const int c = c0 + MX_BLOCK * j + lane;
+        if (c >= K) continue;
+        const uint32_t q = codes[(long long)r * (kp / 2) + c / 2] >> (4 * (lane & 1));
+        const float sc = mx_scale(scales[mx4_scale_at(r, c / MX_BLOCK, kp / 128)]);
+        uint32_t h[4];
+        mx4_unpack8(q & 15u, h);
+        out[(long long)r * K + c] = St<T>::st(__half2float(__ushort_as_half((unsigned short)(h[0] & 0xffffu))) * sc);
+      }
     }
+  }
+}
+
+// Rows copied to a stride that TMA takes: a thread stores 8 elements as one vector.
+__global__ void __launch_bounds__(THREADS) mx8_pack_kernel(const uint16_t* __restrict__ src, uint4* __restrict__ dst,
+                                                           int rows, int n, int ld8) {
+  const long long total = (long long)rows * ld8;
+  for (long long i = blockIdx.x * (long long)THREADS + threadIdx.x; i < total; i += (long long)gridDim.x * THREADS) {
+    const int r = (int)(i / ld8), c = (int)(i % ld8) * 8;
+    const uint16_t* p = src + (long long)r * n + c;
+    uint4 v;
+    uint16_t* h = reinterpret_cast<uint16_t*>(&v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) h[j] = c + j < n ? __ldg(p + j) : (uint16_t)0;
+    dst[i] = v;
   }
 }
 
@@ -354,23 +429,31 @@ int launch_mx8_store(const void* x, signed char* codes, unsigned char* scales, i
 }
 
 int launch_mx8_restore(const signed char* codes, const unsigned char* scales, void* out, int D, int B, long long ld_out,
-                       int pad_cols, int act, int dtype, cudaStream_t s) {
+                       int act, int dtype, cudaStream_t s) {
   const int nb = (int)(mx8_ld(B) / MX_BLOCK);
   dim3 grid;
-  int rc = grid_of("8-bit restore", D, TR, pad_cols, &grid);
+  int rc = grid_of("8-bit restore", D, TR, B, &grid);
   if (rc) return rc;
   IPC_DISPATCH_DT(dtype, TT, {
     TT* ot = static_cast<TT*>(out);
     const bool vec = rows_aligned<TT>(out, ld_out);
     IPC_DISPATCH_ACT(act, AC, {
       if (vec)
-        mx8_restore_kernel<TT, AC, true><<<grid, THREADS, 0, s>>>(codes, scales, ot, D, B, nb, ld_out, pad_cols);
+        mx8_restore_kernel<TT, AC, true><<<grid, THREADS, 0, s>>>(codes, scales, ot, D, B, nb, ld_out);
       else
-        mx8_restore_kernel<TT, AC, false><<<grid, THREADS, 0, s>>>(codes, scales, ot, D, B, nb, ld_out, pad_cols);
+        mx8_restore_kernel<TT, AC, false><<<grid, THREADS, 0, s>>>(codes, scales, ot, D, B, nb, ld_out);
     });
   });
   count_launch();
   return check_launch("8-bit restore");
+}
+
+int launch_mx8_pack(const void* src, void* dst, int rows, int n, long long ld, cudaStream_t s) {
+  const long long blocks = ((long long)rows * (ld / 8) + THREADS - 1) / THREADS;
+  mx8_pack_kernel<<<(int)(blocks < 148 * 8 ? blocks : 148 * 8), THREADS, 0, s>>>(
+      static_cast<const uint16_t*>(src), static_cast<uint4*>(dst), rows, n, (int)(ld / 8));
+  count_launch();
+  return check_launch("row copy");
 }
 
 int launch_mx4_quantize(const void* x, unsigned char* codes, unsigned char* scales, int R, int K, int turned, int act,
@@ -389,8 +472,10 @@ int launch_mx4_quantize(const void* x, unsigned char* codes, unsigned char* scal
     const TT* xt = static_cast<const TT*>(x);
     const bool vec = rows_aligned<TT>(x, K);
     IPC_DISPATCH_ACT(act, AC, {
-      if (turned)
-        mx4_turned_kernel<TT, AC><<<grid, THREADS, 0, s>>>(xt, codes, scales, R, K, kp);
+      if (turned && R % 2 == 0 && (reinterpret_cast<uintptr_t>(x) % (2 * sizeof(TT))) == 0)
+        mx4_turned_kernel<TT, AC, true><<<grid, THREADS, 0, s>>>(xt, codes, scales, R, K, kp);
+      else if (turned)
+        mx4_turned_kernel<TT, AC, false><<<grid, THREADS, 0, s>>>(xt, codes, scales, R, K, kp);
       else if (vec)
         mx4_rows_kernel<TT, AC, true><<<grid, THREADS, 0, s>>>(xt, codes, scales, R, K, kp);
       else

@@ -10,6 +10,7 @@
 // NaN is stored as codes 0 with the scale byte 255 and reads back as 32 NaNs.
 #pragma once
 #include "ipc_common.cuh"
+#include "ipc_generic.cuh"
 
 namespace ipc {
 
@@ -50,6 +51,13 @@ __device__ __forceinline__ uint32_t mx4_pack8(const float (&v)[8]) {
       : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
   return r;
 }
+__device__ __forceinline__ uint32_t mx4_pack2(float lo, float hi) {
+  uint32_t r;
+  asm("{\n\t.reg .b8 b;\n\tcvt.rn.satfinite.e2m1x2.f32 b, %2, %1;\n\tmov.b32 %0, {b, b, b, b};\n\t}"
+      : "=r"(r)
+      : "f"(lo), "f"(hi));
+  return r & 0xffu;
+}
 // The inverse: eight 4-bit codes as four half2.
 __device__ __forceinline__ void mx4_unpack8(uint32_t codes, uint32_t (&h)[4]) {
   asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
@@ -73,9 +81,13 @@ __device__ __forceinline__ long long mx4_scale_at(int r, int j, int atoms_k) {
 }
 
 int launch_mx8_store(const void* x, signed char* codes, unsigned char* scales, int D, int B, int dtype, cudaStream_t s);
-// out[d][b] = cast(f(codes * 2^s)), rows ld_out apart; columns B .. pad_cols - 1 of out are zeroed (pad_cols >= B)
+// out[d][b] = cast(f(codes * 2^s)), rows ld_out >= B apart
 int launch_mx8_restore(const signed char* codes, const unsigned char* scales, void* out, int D, int B, long long ld_out,
-                       int pad_cols, int act, int dtype, cudaStream_t s);
+                       int act, int dtype, cudaStream_t s);
+// dst [rows][ld] = src [rows][n], 16-bit elements (ld a multiple of 8, dst 16-byte aligned; columns n .. ld - 1 undefined)
+int launch_mx8_pack(const void* src, void* dst, int rows, int n, long long ld, cudaStream_t s);
+// one-launch product with a checkpoint (p.ck, p.cks), any shape, 16-bit storage: MODE_W, _WD, _G, _BK
+int launch_mx8_small(const GemmArgs& p, int mode, int act, int dtype, cudaStream_t s);
 int launch_mx4_quantize(const void* x, unsigned char* codes, unsigned char* scales, int R, int K, int turned, int act,
                         int dtype, cudaStream_t s);
 int launch_mx4_restore(const unsigned char* codes, const unsigned char* scales, void* out, int R, int K, int dtype,

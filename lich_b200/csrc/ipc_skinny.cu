@@ -77,7 +77,7 @@ template <typename T, int MODE>
 __device__ __forceinline__ uint32_t sk_load_a(const GemmArgs& p, const T* A, int m, int k, bool vec) {
   if (m >= p.Mg || k >= p.Kg) return 0u;
   const uint16_t* a16 = reinterpret_cast<const uint16_t*>(A);
-  if constexpr (MODE == MODE_I || MODE == MODE_BK) {  // A(m,k) = W_low[k][m]
+  if constexpr (MODE == MODE_I) {  // A(m,k) = W_low[k][m]
     const uint16_t lo = __ldg(a16 + (long long)k * p.lda + m);
     const uint16_t hi = (k + 1 < p.Kg) ? __ldg(a16 + (long long)(k + 1) * p.lda + m) : (uint16_t)0;
     return sk_pack(lo, hi);
@@ -127,7 +127,7 @@ __global__ void __launch_bounds__(SK_THREADS) skinny_kernel(const __grid_constan
   for (int j = 0; j < NB; ++j)
 #pragma unroll
     for (int r = 0; r < 4; ++r) acc[j][r] = 0.f;
-  const bool vec = (MODE != MODE_I && MODE != MODE_BK) && (p.lda % 2 == 0) && ((reinterpret_cast<uintptr_t>(A) & 3) == 0);
+  const bool vec = (MODE != MODE_I) && (p.lda % 2 == 0) && ((reinterpret_cast<uintptr_t>(A) & 3) == 0);
   const int kw0 = k_base + warp * kw;
   const int kw1 = min(min(kw0 + kw, k_base + ks), p.Kg);
   const int r0 = m0 + gq, r1 = m0 + gq + 8;
@@ -234,14 +234,14 @@ int launch_skinny_nb(const GemmArgs& p, cudaStream_t s) {
 bool skinny_eligible(int mode, int M, int K, int B, int dtype, int algo) {
   if (algo != IPC_ALGO_AUTO) return false;
   if (dtype != IPC_DT_F16 && dtype != IPC_DT_BF16) return false;
-  if (mode != MODE_P && mode != MODE_I && mode != MODE_F && mode != MODE_BK) return false;
+  if (mode != MODE_P && mode != MODE_I && mode != MODE_F) return false;
   return M >= 1 && B >= 1 && B <= SK_MAX_B && K >= 1 && K <= SK_MAX_CLUSTER * SK_MAX_SLICE;
 }
 
 int launch_skinny(const GemmArgs& p, int mode, bool bact, int act, int dtype, cudaStream_t s) {
   if (p.Mg <= 0 || p.Ng <= 0 || p.groups <= 0) return IPC_OK;
   IPC_DISPATCH_DT16(dtype, TT, {
-    if (!bact && mode != MODE_I && mode != MODE_BK && !(mode == MODE_F && p.aux2 != nullptr)) {
+    if (!bact && mode != MODE_I && !(mode == MODE_F && p.aux2 != nullptr)) {
       if (mode == MODE_P) return launch_skinny_nb<TT, IPC_ACT_IDENTITY, MODE_P, false>(p, s);
       return launch_skinny_nb<TT, IPC_ACT_IDENTITY, MODE_F, false>(p, s);
     }
@@ -249,7 +249,6 @@ int launch_skinny(const GemmArgs& p, int mode, bool bact, int act, int dtype, cu
       switch (mode) {
         case MODE_P: return launch_skinny_nb<TT, AC, MODE_P, true>(p, s);
         case MODE_I: return launch_skinny_nb<TT, AC, MODE_I, false>(p, s);
-        case MODE_BK: return launch_skinny_nb<TT, AC, MODE_BK, false>(p, s);
         case MODE_F:
           return bact ? launch_skinny_nb<TT, AC, MODE_F, true>(p, s) : launch_skinny_nb<TT, AC, MODE_F, false>(p, s);
         default: return set_error(IPC_ERR_ARG, "small-batch GEMM: bad mode %d", mode);

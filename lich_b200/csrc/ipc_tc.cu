@@ -116,6 +116,8 @@ struct TcParams {
   const signed char* ck;  // BK: the 8-bit states' codes, their row stride, and their scale bytes [block][row]
   const unsigned char* cks;
   long long ld_ck;
+  int ragged;     // WD, G, BK: rows of out start on any element: stored a lane per column, not in 16-byte vectors
+  int ws_ld;      // row stride of the split-K partials (Ng rounded up to 8)
 };
 
 // Bounded wait: false (and the device status set) if the phase never completes.
@@ -567,6 +569,22 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
               release_acc(tempty0 + 8 * acc);
             }
             __syncwarp();
+            if ((MODE == MODE_G || MODE == MODE_BK) && p.ragged) {
+              const int nc = nw + 64 * cc + lane;
+#pragma unroll 4
+              for (int r = 0; r < 32; ++r) {
+                if (r0 + r >= p.Mg) break;
+                T* orow = dst + g * p.gs_out + (long long)(r0 + r) * p.ld_out;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                  const int col = 32 * h + lane;
+                  const uint16_t v = lds16(xb + r * 128 + (((col >> 3) ^ (r & 7)) << 4) + 2 * (col & 7));
+                  if (nc + 32 * h < p.Ng) *reinterpret_cast<uint16_t*>(orow + nc + 32 * h) = v;
+                }
+              }
+              __syncwarp();
+              continue;
+            }
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
               const int r = 4 * i + cr, n = nw + 64 * cc + 8 * cj;
@@ -716,6 +734,18 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
                                 __float_as_uint(p.scale * __uint_as_float(raw[4 * j + 2])),
                                 __float_as_uint(p.scale * __uint_as_float(raw[4 * j + 3]))));
             __syncwarp();
+            if (p.ragged) {  // a lane per column; adds into dw when asked to
+              const int n = nw + 32 * c + lane;
+#pragma unroll 4
+              for (int r = 0; r < 32; ++r) {
+                if (r0 + r >= p.Mg) break;
+                const float v = __uint_as_float(lds32(xb + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + 4 * (lane & 3)));
+                float* o = dst + g * p.gs_out + (long long)(r0 + r) * p.ld_out + n;
+                if (n < p.Ng) *o = p.accumulate ? *o + v : v;
+              }
+              __syncwarp();
+              continue;
+            }
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
               const int r = 4 * i + cr, n = nw + 32 * c + 4 * cj;
@@ -763,7 +793,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
               if (n >= p.Ng) continue;
               if (p.splits > 1) {  // fp32 partial of this K range; the reduce pass applies the epilogue
                 float4* dst = reinterpret_cast<float4*>(
-                    p.ws + (((long long)sp * p.groups + g) * p.Mg + m) * (long long)p.Ng + n);
+                    p.ws + (((long long)sp * p.groups + g) * p.Mg + m) * (long long)p.ws_ld + n);
                 dst[0] = make_float4(__uint_as_float(raw[8 * v]), __uint_as_float(raw[8 * v + 1]),
                                      __uint_as_float(raw[8 * v + 2]), __uint_as_float(raw[8 * v + 3]));
                 dst[1] = make_float4(__uint_as_float(raw[8 * v + 4]), __uint_as_float(raw[8 * v + 5]),
@@ -885,6 +915,24 @@ __global__ void ws_reduce_kernel(const float* __restrict__ ws, int splits, long 
   }
 }
 
+// The same for rows that start anywhere: an element a thread, partials with rows ws_ld apart (one group).
+template <typename T, int MODE>
+__global__ void ws_reduce_ragged_kernel(const float* __restrict__ ws, int splits, int M, int N, int ws_ld, void* out,
+                                        float scale, int accumulate) {
+  const long long n = (long long)M * N;
+  for (long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x; i < n; i += (long long)gridDim.x * blockDim.x) {
+    const long long at = (i / N) * ws_ld + i % N;
+    float acc = ws[at];
+    for (int sp = 1; sp < splits; ++sp) acc += ws[(long long)sp * M * ws_ld + at];
+    if constexpr (MODE == MODE_WD) {
+      float* dw = reinterpret_cast<float*>(out) + i;
+      *dw = (accumulate ? *dw : 0.f) + scale * acc;
+    } else {
+      reinterpret_cast<T*>(out)[i] = St<T>::st(scale * acc);
+    }
+  }
+}
+
 template <typename T, int ACT, int MODE, int BN, int PAIR>
 int launch_tc_t(const GemmArgs& a, int dtype, cudaStream_t s, float* ws, size_t ws_bytes, const TcTune* tune) {
   constexpr bool A_MN = (MODE == MODE_I || MODE == MODE_BK);
@@ -918,6 +966,8 @@ int launch_tc_t(const GemmArgs& a, int dtype, cudaStream_t s, float* ws, size_t 
   // a roughly square block of output tiles and re-reads each operand block about as often as the other
   p.raster = (tune != nullptr && tune->raster > 0) ? tune->raster : (PAIR ? TC_RASTER / 2 : TC_RASTER);
   p.opt = a.opt;
+  p.ragged = a.ragged;
+  p.ws_ld = (a.Ng + 7) / 8 * 8;
   p.ck = a.ck; p.cks = a.cks; p.ld_ck = a.ld_ck;
   // split-K: a weight update with fewer output tiles than half the SMs and a long batch reduction
   const int nk = (a.Kg + TC_BK - 1) / TC_BK;
@@ -931,7 +981,7 @@ int launch_tc_t(const GemmArgs& a, int dtype, cudaStream_t s, float* ws, size_t 
   if ((MODE == MODE_W || MODE == MODE_WD || MODE == MODE_WO || MODE == MODE_G) && ws != nullptr && want != 1 &&
       (want >= 2 || (p.tiles < units / 2 && nk >= 8)) &&
       a.gsOut == (long long)a.Mg * a.Ng) {  // the reduce pass walks out as one dense [groups][M][N] array
-    const long long tile_bytes = (long long)a.groups * a.Mg * a.Ng * 4;
+    const long long tile_bytes = (long long)a.groups * a.Mg * p.ws_ld * 4;
     int splits = want >= 2 ? min(want, nk) : min(units / p.tiles, nk / 4);  // heuristic: one wave of units
     const long long fit = (long long)(ws_bytes / (size_t)tile_bytes);
     if (fit < splits) splits = (int)fit;
@@ -946,7 +996,7 @@ int launch_tc_t(const GemmArgs& a, int dtype, cudaStream_t s, float* ws, size_t 
   // 3.5 with halves); taken for a saving of >= 5 % of the tile time (or on request, tc_splits >= 2)
   p.atomic = 0;
   p.mcast = a.mcast;
-  if (MODE == MODE_WD && PAIR && p.splits == 1 && !a.accumulate && want != 1 && nk >= 16 &&
+  if (MODE == MODE_WD && PAIR && p.splits == 1 && !a.accumulate && !a.ragged && want != 1 && nk >= 16 &&
       a.gsOut == (long long)a.Mg * a.Ng) {
     const long long units = cap / 2 > 0 ? cap / 2 : 1;
     const long long w1 = (p.tiles + units - 1) / units, w2 = (2LL * p.tiles + units - 1) / units;
@@ -965,7 +1015,7 @@ int launch_tc_t(const GemmArgs& a, int dtype, cudaStream_t s, float* ws, size_t 
   CUtensorMap te[3];
   memset(te, 0, sizeof(te));
   // WD accumulating into dw reads dw back per element: the row-per-thread path
-  p.staged = EPI_STAGED && (p.splits == 1 || p.atomic) && !(MODE == MODE_WD && a.accumulate);
+  p.staged = EPI_STAGED && (p.splits == 1 || p.atomic) && !(MODE == MODE_WD && a.accumulate && !a.ragged);
   if (MODE == MODE_I && p.staged) {
     const void* src[3] = {a.aux, a.out, a.aux2};
     const long long gs[3] = {a.gsAux, a.gsOut, a.gsAux2};
@@ -1012,6 +1062,16 @@ int launch_tc_t(const GemmArgs& a, int dtype, cudaStream_t s, float* ws, size_t 
   count_launch();
   int rc2 = check_launch("tcgen05 GEMM");
   if (rc2 || p.splits == 1 || p.atomic) return rc2;
+  if constexpr (MODE == MODE_WD || MODE == MODE_G) {
+    if (a.ragged) {
+      const long long n = (long long)a.Mg * a.Ng;
+      const int blocks = (int)std::min<long long>((n + 255) / 256, 148LL * 16);
+      ws_reduce_ragged_kernel<T, MODE><<<blocks, 256, 0, s>>>(ws, p.splits, a.Mg, a.Ng, p.ws_ld, a.out, a.scale,
+                                                              a.accumulate);
+      count_launch();
+      return check_launch("split-K reduce");
+    }
+  }
   if constexpr (MODE == MODE_W || MODE == MODE_WD || MODE == MODE_WO || MODE == MODE_G) {
     const long long n4 = (long long)a.groups * a.Mg * a.Ng / 4;
     long long blocks = (n4 + 255) / 256;
@@ -1079,7 +1139,7 @@ int launch_tc(const GemmArgs& a, int mode, int act, int dtype, cudaStream_t s, f
   // TMA maps and 16-byte epilogue vectors need 16-byte aligned operands; a view that starts mid-vector
   // takes the generic kernel
   const uintptr_t mis = reinterpret_cast<uintptr_t>(a.A) | reinterpret_cast<uintptr_t>(a.Bm) |
-                        reinterpret_cast<uintptr_t>(a.out) | reinterpret_cast<uintptr_t>(a.aux) |
+                        (a.ragged ? 0 : reinterpret_cast<uintptr_t>(a.out)) | reinterpret_cast<uintptr_t>(a.aux) |
                         reinterpret_cast<uintptr_t>(a.aux2) | reinterpret_cast<uintptr_t>(a.ck);
   if (mis & 15) {
     if (a.mcast) return set_error(IPC_ERR_ARG, "IPC_FLAG_MULTIMEM_RED: operands must be 16-byte aligned");
@@ -1096,7 +1156,7 @@ int launch_tc(const GemmArgs& a, int mode, int act, int dtype, cudaStream_t s, f
   const long long cap = grid_cap();
   const bool splitk = (mode == MODE_W || mode == MODE_WD || mode == MODE_WO || mode == MODE_G) && ws != nullptr && t256 < cap / 2 &&
                       (a.Kg + TC_BK - 1) / TC_BK >= 8 && a.gsOut == (long long)a.Mg * a.Ng &&
-                      ws_bytes >= (size_t)(2LL * a.groups * a.Mg * a.Ng * 4);
+                      ws_bytes >= (size_t)(2LL * a.groups * a.Mg * ((a.Ng + 7) / 8 * 8) * 4);
   const long long cost256 = ((t256 + cap - 1) / cap) * (256 + 416), cost128 = ((t128 + cap - 1) / cap) * (128 + 416);
   bool wide = a.Ng >= 256 && (cost256 <= cost128 || splitk);
   if (tune != nullptr && (tune->bn == 128 || tune->bn == 256)) wide = tune->bn == 256;

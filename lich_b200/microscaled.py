@@ -97,6 +97,17 @@ class _MxOp:
                 return f"{self.kind}: argument {i} is not contiguous"
         return f"{self.kind}: tensors on different devices"
 
+    def _workspace(self, dev: int, stream: int):
+        """(address, bytes) of this operator's workspace for one stream of a device: calls on two streams may overlap."""
+        ws = self._ws.get((dev, stream))
+        if ws is None:
+            n = c_size_t(0)
+            with torch.cuda.device(dev):
+                N.check(self._ws_bytes(byref(n)))
+                buf = torch.empty(int(n.value), device=f"cuda:{dev}", dtype=torch.uint8) if n.value else None
+            ws = self._ws[dev, stream] = (None if buf is None else buf.data_ptr(), int(n.value), buf)
+        return ws[:2]
+
     def _launch(self, tensors, *args) -> None:
         """The C entry on the tensors' device and its current stream; its error as an exception."""
         dev = tensors[0].get_device()
@@ -150,23 +161,15 @@ class CheckpointWeightKernel(_MxOp):
         self.mode, self.M, self.K, self.B = mode, int(M), int(K), int(B)
         self.act, self.dt, self.alpha, self.algo = N.act_code(activation), N.dtype_code(dtype), float(alpha), _algo(cfg)
 
-    def _workspace(self, dev: int, stream: int):
-        """This operator's workspace for one stream of a device: calls on two streams may overlap."""
-        ws = self._ws.get((dev, stream))
-        if ws is None:
-            n = c_size_t(0)
-            with torch.cuda.device(dev):
-                N.check(N.load().ipc_mx8_weight_ws_bytes(self.mode, self.M, self.K, self.B, self.dt, self.algo, byref(n)))
-                buf = torch.empty(max(int(n.value), 16), device=f"cuda:{dev}", dtype=torch.uint8)
-            ws = self._ws[dev, stream] = (buf, buf.data_ptr(), int(n.value))
-        return ws
+    def _ws_bytes(self, n) -> int:
+        return N.load().ipc_mx8_weight_ws_bytes(self.mode, self.M, self.K, self.B, self.dt, self.algo, n)
 
     def __call__(self, out, e, codes, scales, *, accumulate: bool = False):
         t = (out, e, codes, scales)
         s = self._stream(t)
         if accumulate and self.mode != N.MODE_WDELTA:
             raise ValueError(f"{self.kind}: only a weight delta in float32 accumulates")
-        _, ws, n = self._workspace(out.get_device(), s)
+        ws, n = self._workspace(out.get_device(), s)
         self._launch(t, self.mode, out.data_ptr(), e.data_ptr(), codes.data_ptr(), scales.data_ptr(), self.M, self.K,
                      self.B, self.alpha, N.FLAG_ACCUMULATE if accumulate else 0, self.act, self.dt, self.algo, ws, n, s)
 
@@ -182,11 +185,15 @@ class CheckpointBackwardKernel(_MxOp):
         self.M, self.K, self.B = int(M), int(K), int(B)
         self.act, self.dt, self.algo = N.act_code(activation), N.dtype_code(dtype), _algo(cfg)
 
+    def _ws_bytes(self, n) -> int:
+        return N.load().ipc_mx8_backward_ws_bytes(self.M, self.K, self.B, self.dt, self.algo, n)
+
     def __call__(self, w, e, codes, scales, e_up):
         t = (w, e, codes, scales, e_up)
         s = self._stream(t)
+        ws, n = self._workspace(w.get_device(), s)
         self._launch(t, e_up.data_ptr(), w.data_ptr(), e.data_ptr(), codes.data_ptr(), scales.data_ptr(), self.M, self.K,
-                     self.B, self.act, self.dt, self.algo, s)
+                     self.B, self.act, self.dt, self.algo, ws, n, s)
 
 
 class Mxfp4QuantizeKernel(_MxOp):

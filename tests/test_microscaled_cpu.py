@@ -87,7 +87,7 @@ def test_abi_refuses_bad_arguments():
     assert lib.ipc_mx8_store(None, None, None, 4, 4, 9, None) == A
     assert lib.ipc_mx8_restore(None, None, None, 4, 4, 77, 1, None) == A
     assert lib.ipc_mx8_weight(3, None, None, None, None, 4, 4, 4, 1.0, 0, 99, 1, 0, None, 0, None) == A
-    assert lib.ipc_mx8_backward(None, None, None, None, None, 4, 4, -4, 0, 1, 0, None) == A
+    assert lib.ipc_mx8_backward(None, None, None, None, None, 4, 4, -4, 0, 1, 0, None, 0, None) == A
     assert lib.ipc_mxfp4_quantize(None, None, None, 4, -4, 0, 0, 1, None) == A
     assert lib.ipc_mxfp4_restore(None, None, None, 4, 4, 5, None) == A
     assert lib.ipc_mxfp4_forward(None, None, None, None, None, 4, 4, -1, 1, None) == A

@@ -370,3 +370,77 @@ def test_forward_marks_what_was_not_finite(M, K, B):
     mx.build_mxfp4_forward(M, K, B, "float32")(wq.to(DEV), wsc.to(DEV), aq.to(DEV), asc.to(DEV), out)
     bad = out.isnan().cpu()
     assert bad[3].all() and bad.sum() == B
+
+
+@pytest.mark.parametrize("backend", ["simt", "tcgen05"])
+@pytest.mark.parametrize("dt", HALF)
+@pytest.mark.parametrize("M,K,B", SIZES + [(33, 31, 95), (130, 259, 1029), (200, 136, 4099), (257, 513, 130)])
+def test_products_of_any_size_on_either_kernel(M, K, B, dt, backend):
+    """Both kernels take every shape: odd strides go through copied operands and a lane-per-column epilogue on one, tails
+    of tiles, splits of the reduction on the other."""
+    from lich_b200 import _native as N
+    from lich_b200.tilelang_kernels import KernelConfig
+    mx = _mx()
+    cfg = KernelConfig(backend=backend)
+    act = ACTS[(M + K + 2 * B) % 6]
+    e, c, s, ref, err = _delta_case(M, K, B, dt, act, 20)
+    alpha = 1.0 / B
+    ed = e.to(DEV)
+    g = torch.full((M, K), 7.0, device=DEV, dtype=dt)
+    mx.build_weight_delta_checkpoint(M, K, B, act, NAME[dt], alpha, NAME[dt], cfg)(g, ed, c, s)
+    _within(g, alpha * ref, (alpha * err) * (1 + U[dt]) + U[dt] * alpha * ref.abs() + TINY[dt])
+    dw = torch.full((M, K), 7.0, device=DEV)
+    k = mx.build_weight_delta_checkpoint(M, K, B, act, NAME[dt], alpha, "float32", cfg)
+    k(dw, ed, c, s)
+    k(dw, ed, c, s, accumulate=True)
+    _within(dw, 2 * alpha * ref, 2 * alpha * err + 2.0 ** -22 * 2 * alpha * ref.abs())
+    w0 = _rand((M, K), 22, 0.05, dt)
+    w = w0.to(DEV)
+    mx.build_weight_update_checkpoint(M, K, B, act, NAME[dt], 0.01, cfg)(w, ed, c, s)
+    want = w0.double() + 0.01 * ref
+    _within(w, want, (0.01 * err) * (1 + U[dt]) + (U[dt] + 2.0 ** -22) * (want.abs() + 0.01 * ref.abs()) + TINY[dt])
+    xhat = X.load8(c.cpu(), s.cpu(), B)
+    up = torch.full((K, B), 7.0, device=DEV, dtype=dt)
+    mx.build_error_backward_checkpoint(M, K, B, act, NAME[dt], cfg)(w0.to(DEV), ed, c, s, up)
+    acc = w0.double().t() @ e.double()
+    S = w0.double().abs().t() @ e.double().abs()
+    rb = X.backward(w0, e, xhat, act)
+    tol = _slope_err(act, xhat, dt) * (acc.abs() + S * M * 2.0 ** -23) + X.slope(act, xhat).abs() * S * M * 2.0 ** -23
+    _within(up, rb, tol * (1 + U[dt]) + (U[dt] + 2.0 ** -23) * rb.abs() + TINY[dt])
+    assert N.device_status() == 0
+
+
+def test_products_on_views_that_start_between_vectors():
+    """Contiguous tensors two bytes past a 16-byte boundary, at sizes that take the tensor-core kernel otherwise."""
+    mx = _mx()
+    M, K, B, dt = 512, 1024, 2048, torch.bfloat16
+    e, c, s, ref, err = _delta_case(M, K, B, dt, "tanh", 30)
+
+    def off(t):
+        flat = torch.zeros(t.numel() + 1, device=DEV, dtype=t.dtype)
+        flat[1:] = t.reshape(-1).to(DEV)
+        return flat[1:].view(t.shape)
+
+    alpha = 1.0 / B
+    for name in ("bfloat16", "float32"):
+        out = off(torch.full((M, K), 7.0, dtype=getattr(torch, name)))
+        mx.build_weight_delta_checkpoint(M, K, B, "tanh", "bfloat16", alpha, name)(out, e.to(DEV), c, s)
+        u = U[out.dtype] + 2.0 ** -23
+        _within(out, alpha * ref, (alpha * err) * (1 + u) + u * alpha * ref.abs() + TINY[out.dtype])
+        out = torch.full((M, K), 7.0, dtype=getattr(torch, name), device=DEV)
+        mx.build_weight_delta_checkpoint(M, K, B, "tanh", "bfloat16", alpha, name)(out, off(e), c, s)
+        _within(out, alpha * ref, (alpha * err) * (1 + u) + u * alpha * ref.abs() + TINY[out.dtype])
+    w0 = _rand((M, K), 32, 0.05, dt)
+    want = w0.double() + 0.01 * ref
+    w = off(w0)
+    mx.build_weight_update_checkpoint(M, K, B, "tanh", "bfloat16", 0.01)(w, e.to(DEV), c, s)
+    _within(w, want, (0.01 * err) * (1 + U[dt]) + (U[dt] + 2.0 ** -22) * (want.abs() + 0.01 * ref.abs()) + TINY[dt])
+    xhat = X.load8(c.cpu(), s.cpu(), B)
+    acc, S = w0.double().t() @ e.double(), w0.double().abs().t() @ e.double().abs()
+    rb = X.backward(w0, e, xhat, "tanh")
+    tol = _slope_err("tanh", xhat, dt) * (acc.abs() + S * M * 2.0 ** -23) + X.slope("tanh", xhat).abs() * S * M * 2.0 ** -23
+    for ww, ee, shift in ((off(w0), e.to(DEV), False), (w0.to(DEV), off(e), False), (w0.to(DEV), e.to(DEV), True)):
+        up = torch.full((K, B), 7.0, dtype=dt, device=DEV)
+        up = off(up) if shift else up
+        mx.build_error_backward_checkpoint(M, K, B, "tanh", "bfloat16")(ww, ee, c, s, up)
+        _within(up, rb, tol * (1 + U[dt]) + (U[dt] + 2.0 ** -23) * rb.abs() + TINY[dt])
