@@ -453,7 +453,7 @@ static bool mx8_large(int mode, int M, int K, int B, int dtype, int algo) {
   if (dtype == IPC_DT_F32 || (algo != IPC_ALGO_AUTO && algo != IPC_ALGO_TCGEN05)) return false;
   if (M < 1 || K < 1 || B < 1) return false;
   if (algo == IPC_ALGO_TCGEN05) return true;
-  return (double)M * K * B >= (mode == MODE_BK ? MX8_LARGE_BACKWARD : MX8_LARGE_WEIGHT);
+  return (double)M * K * (B < 64 ? 64 : B) >= (mode == MODE_BK ? MX8_LARGE_BACKWARD : MX8_LARGE_WEIGHT);
 }
 static long long up8(long long n) { return (n + 7) / 8 * 8; }
 static size_t up256(size_t n) { return (n + 255) / 256 * 256; }
@@ -475,7 +475,9 @@ static Mx8WeightWs mx8_weight_ws(int mode, int M, int K, int B, int dtype, int a
     w.values = up256((size_t)K * w.ld * 2);
     w.e = B % 8 ? up256((size_t)M * w.ld * 2) : 0;
     w.delta = (mode == MODE_W && K % 8) ? up256((size_t)M * K * 4) : 0;
-    w.partial = IPC_SPLITK_WS_BYTES;
+    // split-K: its partial sums and second pass cost about 10 us, which a batch below 2048 does not win back
+    // (1000 x 1021 x 777: 26 us split in three, 11 us in one)
+    w.partial = B >= 2048 ? IPC_SPLITK_WS_BYTES : 0;
   }
   w.total = w.values + w.e + w.delta + w.partial;
   return w;
@@ -536,7 +538,7 @@ int ipc_mx8_weight(int mode, void* out, const void* e, const signed char* codes,
   p.lda = w.ld; p.gsA = (long long)M * w.ld;
   p.Bm = ws; p.ldb = w.ld; p.gsB = (long long)K * w.ld;
   p.ck = nullptr;
-  float* part = reinterpret_cast<float*>(ws + w.values + w.e + w.delta);
+  float* part = w.partial ? reinterpret_cast<float*>(ws + w.values + w.e + w.delta) : nullptr;
   if (aligned16(out) && K % 8 == 0) return launch_tc(p, mode, act, dtype, s, part, w.partial);
   p.ragged = 1;
   if (mode != MODE_W) return launch_tc(p, mode, act, dtype, s, part, w.partial);

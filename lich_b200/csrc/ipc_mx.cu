@@ -24,6 +24,19 @@ struct Vec {  // one 16-byte vector
 #pragma unroll
     for (int j = 0; j < N; ++j) v[j] = St<T>::ld(h[j]);
   }
+  // bits (of a float) of the largest magnitude.  16-bit types: compared as they are, two at a time; the bits of a
+  // magnitude grow with it in either type, and a NaN's lie above infinity's.
+  static __device__ __forceinline__ uint32_t max_bits(const uint4& raw) {
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+    if constexpr (sizeof(T) == 4) {
+      return max(max(w[0] & 0x7fffffffu, w[1] & 0x7fffffffu), max(w[2] & 0x7fffffffu, w[3] & 0x7fffffffu));
+    } else {
+      const uint32_t m = __vmaxu2(__vmaxu2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu),
+                                  __vmaxu2(w[2] & 0x7fff7fffu, w[3] & 0x7fff7fffu));
+      const uint16_t b = (uint16_t)max(m & 0xffffu, m >> 16);
+      return __float_as_uint(St<T>::ld(*reinterpret_cast<const T*>(&b)));
+    }
+  }
   static __device__ __forceinline__ void store(T* p, const float (&v)[N]) {
     uint4 raw;
     T* h = reinterpret_cast<T*>(&raw);
@@ -83,27 +96,30 @@ __global__ void __launch_bounds__(THREADS) mx8_store_kernel(const T* __restrict_
   if constexpr (VEC) {
     constexpr int N = Vec<T>::N, TPR = TCOL / N, RPI = THREADS / TPR;  // threads a row, rows at a time
     const int c = c0 + N * (tid % TPR);
+    uint4 raw[TR / RPI];
+#pragma unroll
+    for (int it = 0; it < TR / RPI; ++it) {  // all loads first
+      const int d = d0 + tid / TPR + RPI * it;
+      raw[it] = make_uint4(0, 0, 0, 0);
+      if (d < D && c < B) raw[it] = __ldg(reinterpret_cast<const uint4*>(x + (long long)d * B + c));
+    }
 #pragma unroll
     for (int it = 0; it < TR / RPI; ++it) {
       const int r = tid / TPR + RPI * it, d = d0 + r;
-      float v[N];
-#pragma unroll
-      for (int j = 0; j < N; ++j) v[j] = 0.f;
-      if (d < D && c < B) Vec<T>::load(x + (long long)d * B + c, v);
-      uint32_t m = 0;
-#pragma unroll
-      for (int j = 0; j < N; ++j) m = max(m, abs_bits(v[j]));
-      const uint32_t byte = mx8_scale_byte(group_max<MX_BLOCK / N>(m));
+      const uint32_t byte = mx8_scale_byte(group_max<MX_BLOCK / N>(Vec<T>::max_bits(raw[it])));
       const float inv = mx_inv_scale(byte);
       if (c % MX_BLOCK == 0) s_scale[(c - c0) / MX_BLOCK][r] = (unsigned char)byte;
       if (d < D && c < ldc) {
+        const T* h = reinterpret_cast<const T*>(&raw[it]);
         uint32_t w[N / 4];
 #pragma unroll
         for (int q = 0; q < N / 4; ++q) {
-          uint32_t t = 0;
+          // v * 2^-s + 1.5 * 2^23: the integer nearest to v * 2^-s (ties to even) in the sum's low byte
+          uint32_t t[4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) t |= ((uint32_t)mx8_code(v[4 * q + j], inv) & 0xffu) << (8 * j);
-          w[q] = t;
+          for (int j = 0; j < 4; ++j) t[j] = __float_as_uint(fmaf(St<T>::ld(h[4 * q + j]), inv, 12582912.f));
+          w[q] = __byte_perm(__byte_perm(t[0], t[1], 0x0040), __byte_perm(t[2], t[3], 0x0040), 0x5410);
+          if (byte == MX_NAN_BYTE) w[q] = 0;
         }
         st_codes(codes + (long long)d * ldc + c, w);
       }
@@ -139,19 +155,30 @@ __global__ void __launch_bounds__(THREADS)
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const long long ldc = (long long)nb * MX_BLOCK;
   if constexpr (VEC) {
-    constexpr int N = Vec<T>::N, TPR = TCOL / N, RPI = THREADS / TPR;
+    constexpr int N = Vec<T>::N, TPR = TCOL / N, RPI = THREADS / TPR, IT = TR / RPI;
     const int c = c0 + N * (tid % TPR);
+    if (c >= cols) return;
+    uint32_t w[IT][N / 4], byte[IT];
 #pragma unroll
-    for (int it = 0; it < TR / RPI; ++it) {
+    for (int it = 0; it < IT; ++it) {  // all loads first
       const int d = d0 + tid / TPR + RPI * it;
-      if (d >= D || c >= cols) continue;
-      uint32_t w[N / 4];
-      ld_codes(codes + (long long)d * ldc + c, w);
-      const float sc = mx_scale(scales[(long long)(c / MX_BLOCK) * D + d]);
-      const signed char* q = reinterpret_cast<const signed char*>(w);
+      byte[it] = 0;
+#pragma unroll
+      for (int q = 0; q < N / 4; ++q) w[it][q] = 0;
+      if (d < D) {
+        ld_codes(codes + (long long)d * ldc + c, w[it]);
+        byte[it] = __ldg(scales + (long long)(c / MX_BLOCK) * D + d);
+      }
+    }
+#pragma unroll
+    for (int it = 0; it < IT; ++it) {
+      const int d = d0 + tid / TPR + RPI * it;
+      if (d >= D) continue;
+      const float sc = mx_scale(byte[it]);
       float v[N];
 #pragma unroll
-      for (int j = 0; j < N; ++j) v[j] = act_for<T, ACT>((float)q[j] * sc);
+      for (int j = 0; j < N; ++j)
+        v[j] = act_for<T, ACT>((float)(signed char)(w[it][j / 4] >> (8 * (j % 4))) * sc);
       T* o = out + (long long)d * ld_out + c;
       if (c + N <= cols) {
         Vec<T>::store(o, v);
@@ -165,12 +192,18 @@ __global__ void __launch_bounds__(THREADS)
     for (int r = warp; r < TR; r += THREADS / 32) {
       const int d = d0 + r;
       if (d >= D) break;
+      int q[TB];
+      uint32_t byte[TB];
 #pragma unroll
       for (int j = 0; j < TB; ++j) {
         const int c = c0 + MX_BLOCK * j + lane;
-        if (c >= cols) continue;
-        out[(long long)d * ld_out + c] = St<T>::st(act_for<T, ACT>(
-            (float)codes[(long long)d * ldc + c] * mx_scale(scales[(long long)(c / MX_BLOCK) * D + d])));
+        q[j] = c < cols ? __ldg(codes + (long long)d * ldc + c) : 0;
+        byte[j] = c < cols ? __ldg(scales + (long long)(c / MX_BLOCK) * D + d) : 0u;
+      }
+#pragma unroll
+      for (int j = 0; j < TB; ++j) {
+        const int c = c0 + MX_BLOCK * j + lane;
+        if (c < cols) out[(long long)d * ld_out + c] = St<T>::st(act_for<T, ACT>((float)q[j] * mx_scale(byte[j])));
       }
     }
   }
@@ -187,21 +220,25 @@ __global__ void __launch_bounds__(THREADS) mx4_rows_kernel(const T* __restrict__
   if constexpr (VEC) {
     constexpr int N = 8, TPR = TCOL / N, RPI = THREADS / TPR;  // 8 codes: 4 bytes a thread
     const int c = c0 + N * (tid % TPR);
+    constexpr int NV = N / Vec<T>::N;
+    uint4 raw[TR / RPI][NV];
+#pragma unroll
+    for (int it = 0; it < TR / RPI; ++it)  // all loads first (K is a multiple of a vector)
+#pragma unroll
+      for (int h = 0; h < NV; ++h) {
+        const int r = r0 + tid / TPR + RPI * it, ch = c + h * Vec<T>::N;
+        raw[it][h] = make_uint4(0, 0, 0, 0);
+        if (r < R && ch < K) raw[it][h] = __ldg(reinterpret_cast<const uint4*>(x + (long long)r * K + ch));
+      }
 #pragma unroll
     for (int it = 0; it < TR / RPI; ++it) {
       const int rr = tid / TPR + RPI * it, r = r0 + rr;
       float v[N];
 #pragma unroll
-      for (int j = 0; j < N; ++j) v[j] = 0.f;
-      if (r < R) {  // (K is a multiple of a vector)
-#pragma unroll
-        for (int h = 0; h < N; h += Vec<T>::N)
-          if (c + h < K) {
-            float u[Vec<T>::N];
-            Vec<T>::load(x + (long long)r * K + c + h, u);
-#pragma unroll
-            for (int j = 0; j < Vec<T>::N; ++j) v[h + j] = act_full<ACT>(u[j]);
-          }
+      for (int j = 0; j < N; ++j) {
+        const T* h = reinterpret_cast<const T*>(raw[it]);
+        v[j] = act_full<ACT>(St<T>::ld(h[j]));
+        if (ACT == IPC_ACT_SIGMOID && !(r < R && c + j < K)) v[j] = 0.f;  // (the other f are 0 at 0)
       }
       uint32_t m = 0;
 #pragma unroll
@@ -216,14 +253,19 @@ __global__ void __launch_bounds__(THREADS) mx4_rows_kernel(const T* __restrict__
       }
     }
   } else {
-    for (int rr = warp; rr < TR; rr += THREADS / 32) {
-      const int r = r0 + rr;
-      float v[TB];
+    constexpr int RW = TR / (THREADS / 32);  // rows of a warp, all loads first
+    float in[RW][TB];
+#pragma unroll
+    for (int i = 0; i < RW; ++i)
 #pragma unroll
       for (int j = 0; j < TB; ++j) {
-        const int c = c0 + MX_BLOCK * j + lane;
-        v[j] = (r < R && c < K) ? St<T>::ld(x[(long long)r * K + c]) : 0.f;
+        const int r = r0 + warp + THREADS / 32 * i, c = c0 + MX_BLOCK * j + lane;
+        in[i][j] = (r < R && c < K) ? St<T>::ld(x[(long long)r * K + c]) : 0.f;
       }
+#pragma unroll
+    for (int i = 0; i < RW; ++i) {
+      const int rr = warp + THREADS / 32 * i, r = r0 + rr;
+      float (&v)[TB] = in[i];
 #pragma unroll
       for (int j = 0; j < TB; ++j) {
         const int c = c0 + MX_BLOCK * j + lane;
@@ -348,14 +390,24 @@ __global__ void __launch_bounds__(THREADS) mx4_restore_kernel(const unsigned cha
   if constexpr (VEC) {
     constexpr int N = 8, TPR = TCOL / N, RPI = THREADS / TPR;
     const int c = c0 + N * (tid % TPR);
+    if (c >= K) return;
+    uint32_t q[TR / RPI], byte[TR / RPI];
+#pragma unroll
+    for (int it = 0; it < TR / RPI; ++it) {  // all loads first
+      const int r = r0 + tid / TPR + RPI * it;
+      q[it] = byte[it] = 0;
+      if (r < R) {
+        q[it] = __ldg(reinterpret_cast<const uint32_t*>(codes + (long long)r * (kp / 2) + c / 2));
+        byte[it] = __ldg(scales + mx4_scale_at(r, c / MX_BLOCK, kp / 128));
+      }
+    }
 #pragma unroll
     for (int it = 0; it < TR / RPI; ++it) {
       const int r = r0 + tid / TPR + RPI * it;
-      if (r >= R || c >= K) continue;
-      const uint32_t q = __ldg(reinterpret_cast<const uint32_t*>(codes + (long long)r * (kp / 2) + c / 2));
-      const float sc = mx_scale(scales[mx4_scale_at(r, c / MX_BLOCK, kp / 128)]);
+      if (r >= R) continue;
+      const float sc = mx_scale(byte[it]);
       uint32_t h[4];
-      mx4_unpack8(q, h);
+      mx4_unpack8(q[it], h);
       float v[N];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -368,18 +420,28 @@ __global__ void __launch_bounds__(THREADS) mx4_restore_kernel(const unsigned cha
         if (c + g < K) Vec<T>::store(out + (long long)r * K + c + g, *reinterpret_cast<float(*)[Vec<T>::N]>(v + g));
     }
   } else {
-    for (int r = r0 + warp; r < r0 + TR && r < R; r += THREADS / 32) {
+    constexpr int RW = TR / (THREADS / 32);
+    uint32_t q[RW][TB], byte[RW][TB];
+#pragma unroll
+    for (int i = 0; i < RW; ++i)  // all loads first
 #pragma unroll
       for (int j = 0; j < TB; ++j) {
-        const int c = c0 + MX_BLOCK * j + lane;
-        if (c >= K) continue;
-        const uint32_t q = codes[(long long)r * (kp / 2) + c / 2] >> (4 * (lane & 1));
-        const float sc = mx_scale(scales[mx4_scale_at(r, c / MX_BLOCK, kp / 128)]);
-        uint32_t h[4];
-        mx4_unpack8(q & 15u, h);
-        out[(long long)r * K + c] = St<T>::st(__half2float(__ushort_as_half((unsigned short)(h[0] & 0xffffu))) * sc);
+        const int r = r0 + warp + THREADS / 32 * i, c = c0 + MX_BLOCK * j + lane;
+        const bool in = r < R && c < K;
+        q[i][j] = in ? __ldg(codes + (long long)r * (kp / 2) + c / 2) : 0u;
+        byte[i][j] = in ? __ldg(scales + mx4_scale_at(r, c / MX_BLOCK, kp / 128)) : 0u;
       }
-    }
+#pragma unroll
+    for (int i = 0; i < RW; ++i)
+#pragma unroll
+      for (int j = 0; j < TB; ++j) {
+        const int r = r0 + warp + THREADS / 32 * i, c = c0 + MX_BLOCK * j + lane;
+        uint32_t h[4];
+        mx4_unpack8((q[i][j] >> (4 * (lane & 1))) & 15u, h);
+        if (r < R && c < K)
+          out[(long long)r * K + c] =
+              St<T>::st(__half2float(__ushort_as_half((unsigned short)(h[0] & 0xffffu))) * mx_scale(byte[i][j]));
+      }
   }
 }
 

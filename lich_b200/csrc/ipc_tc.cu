@@ -915,15 +915,18 @@ __global__ void ws_reduce_kernel(const float* __restrict__ ws, int splits, long 
   }
 }
 
-// The same for rows that start anywhere: an element a thread, partials with rows ws_ld apart (one group).
+// The same for rows that start anywhere: a row of `out` a block row, an element a thread, partials with rows ws_ld apart
+// (one group).
 template <typename T, int MODE>
 __global__ void ws_reduce_ragged_kernel(const float* __restrict__ ws, int splits, int M, int N, int ws_ld, void* out,
                                         float scale, int accumulate) {
-  const long long n = (long long)M * N;
-  for (long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x; i < n; i += (long long)gridDim.x * blockDim.x) {
-    const long long at = (i / N) * ws_ld + i % N;
-    float acc = ws[at];
-    for (int sp = 1; sp < splits; ++sp) acc += ws[(long long)sp * M * ws_ld + at];
+  const int n = blockIdx.x * blockDim.x + threadIdx.x;
+  if (n >= N) return;
+  for (int m = blockIdx.y; m < M; m += gridDim.y) {
+    const float* p = ws + (long long)m * ws_ld + n;
+    float acc = *p;
+    for (int sp = 1; sp < splits; ++sp) acc += p[(long long)sp * M * ws_ld];
+    const long long i = (long long)m * N + n;
     if constexpr (MODE == MODE_WD) {
       float* dw = reinterpret_cast<float*>(out) + i;
       *dw = (accumulate ? *dw : 0.f) + scale * acc;
@@ -1064,10 +1067,9 @@ int launch_tc_t(const GemmArgs& a, int dtype, cudaStream_t s, float* ws, size_t 
   if (rc2 || p.splits == 1 || p.atomic) return rc2;
   if constexpr (MODE == MODE_WD || MODE == MODE_G) {
     if (a.ragged) {
-      const long long n = (long long)a.Mg * a.Ng;
-      const int blocks = (int)std::min<long long>((n + 255) / 256, 148LL * 16);
-      ws_reduce_ragged_kernel<T, MODE><<<blocks, 256, 0, s>>>(ws, p.splits, a.Mg, a.Ng, p.ws_ld, a.out, a.scale,
-                                                              a.accumulate);
+      const dim3 grid((a.Ng + 255) / 256, a.Mg < 65535 ? a.Mg : 65535);
+      ws_reduce_ragged_kernel<T, MODE><<<grid, 256, 0, s>>>(ws, p.splits, a.Mg, a.Ng, p.ws_ld, a.out, a.scale,
+                                                            a.accumulate);
       count_launch();
       return check_launch("split-K reduce");
     }
