@@ -448,12 +448,15 @@ int ipc_mx8_restore(const signed char* codes, const unsigned char* scales, void*
 // Products with a checkpoint.  Large ones run on the tcgen05 GEMMs, whose operands TMA loads: rows on 16-byte
 // boundaries.  So f(x^) is restored, and an operand with a row stride that is no multiple of 8 copied, into rows of the
 // workspace that are.  The rest (16-bit storage) is one launch of mx8_small_kernel, which needs none.
-constexpr double MX8_LARGE_WEIGHT = 3e8, MX8_LARGE_BACKWARD = 3e8;
 static bool mx8_large(int mode, int M, int K, int B, int dtype, int algo) {
   if (dtype == IPC_DT_F32 || (algo != IPC_ALGO_AUTO && algo != IPC_ALGO_TCGEN05)) return false;
   if (M < 1 || K < 1 || B < 1) return false;
   if (algo == IPC_ALGO_TCGEN05) return true;
-  return (double)M * K * (B < 64 ? 64 : B) >= (mode == MODE_BK ? MX8_LARGE_BACKWARD : MX8_LARGE_WEIGHT);
+  // Measured (GPU time, us, one launch against tcgen05): delta 512^3 7.9 / 8.7, 512 x 512 x 1024 11.4 / 11.0, 1000 x 1021 x 333
+  // 15.8 / 11.3, 4096 x 4096 x 16 42 / 17 (outputs, not the sum, fill that one); backward 256 x 512 x 512 7.4 / 6.3, and with
+  // both operands copied 1000 x 1021 x 333 27 / 15.
+  if (mode == MODE_BK) return (double)M * K * B >= (K % 8 || B % 8 ? 1.5e8 : 5e7);
+  return (double)M * K * (B < 64 ? 64 : B) >= 2.5e8;
 }
 static long long up8(long long n) { return (n + 7) / 8 * 8; }
 static size_t up256(size_t n) { return (n + 255) / 256 * 256; }
@@ -528,13 +531,13 @@ int ipc_mx8_weight(int mode, void* out, const void* e, const signed char* codes,
   if (w.values == 0 || (direct && !aligned16(e)) || (mode == MODE_W && K % 8 == 0 && !aligned16(out)))
     return launch_mx8_small(p, mode, act, dtype, s);
   char* ws = static_cast<char*>(workspace);
-  rc = launch_mx8_restore(codes, scales, ws, K, B, w.ld, act, dtype, s);
-  if (rc) return rc;
-  if (!direct) {
-    rc = launch_mx8_pack(e, ws + w.values, M, B, w.ld, s);
-    if (rc) return rc;
+  if (direct) {
+    rc = launch_mx8_restore(codes, scales, ws, K, B, w.ld, act, dtype, s);
+  } else {
+    rc = launch_mx8_restore_pack(codes, scales, ws, K, B, w.ld, e, ws + w.values, M, act, dtype, s);
     p.A = ws + w.values;
   }
+  if (rc) return rc;
   p.lda = w.ld; p.gsA = (long long)M * w.ld;
   p.Bm = ws; p.ldb = w.ld; p.gsB = (long long)K * w.ld;
   p.ck = nullptr;
@@ -593,16 +596,10 @@ int ipc_mx8_backward(void* e_up, const void* w, const void* e, const signed char
   const bool wide = mx8_large(MODE_BK, M, K, B, dtype, algo) && (K % 8 || aligned16(w)) && (B % 8 || aligned16(e));
   if (!wide) return launch_mx8_small(p, MODE_BK, act, dtype, s);
   char* ws = static_cast<char*>(workspace);
-  if (K % 8) {
-    rc = launch_mx8_pack(w, ws, M, K, up8(K), s);
-    if (rc) return rc;
-    p.A = ws; p.lda = up8(K); p.gsA = M * p.lda;
-  }
-  if (B % 8) {
-    rc = launch_mx8_pack(e, ws + w_bytes, M, B, up8(B), s);
-    if (rc) return rc;
-    p.Bm = ws + w_bytes; p.ldb = up8(B); p.gsB = M * p.ldb;
-  }
+  rc = launch_mx8_pack(K % 8 ? w : nullptr, ws, M, K, up8(K), B % 8 ? e : nullptr, ws + w_bytes, M, B, up8(B), s);
+  if (rc) return rc;
+  if (K % 8) { p.A = ws; p.lda = up8(K); p.gsA = M * p.lda; }
+  if (B % 8) { p.Bm = ws + w_bytes; p.ldb = up8(B); p.gsB = M * p.ldb; }
   p.ragged = B % 8 != 0 || !aligned16(e_up);
   return launch_tc(p, MODE_BK, act, dtype, s);
 }

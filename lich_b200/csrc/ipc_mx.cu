@@ -148,9 +148,9 @@ __global__ void __launch_bounds__(THREADS) mx8_store_kernel(const T* __restrict_
 }
 
 template <typename T, int ACT, bool VEC>
-__global__ void __launch_bounds__(THREADS)
-    mx8_restore_kernel(const signed char* __restrict__ codes, const unsigned char* __restrict__ scales,
-                       T* __restrict__ out, int D, int cols, int nb, long long ld_out) {
+__device__ __forceinline__ void restore_tile(const signed char* __restrict__ codes,
+                                             const unsigned char* __restrict__ scales, T* __restrict__ out, int D,
+                                             int cols, int nb, long long ld_out) {
   const int d0 = blockIdx.y * TR, c0 = blockIdx.x * TCOL;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const long long ldc = (long long)nb * MX_BLOCK;
@@ -207,6 +207,13 @@ __global__ void __launch_bounds__(THREADS)
       }
     }
   }
+}
+
+template <typename T, int ACT, bool VEC>
+__global__ void __launch_bounds__(THREADS)
+    mx8_restore_kernel(const signed char* __restrict__ codes, const unsigned char* __restrict__ scales,
+                       T* __restrict__ out, int D, int cols, int nb, long long ld_out) {
+  restore_tile<T, ACT, VEC>(codes, scales, out, D, cols, nb, ld_out);
 }
 
 // ---------------------------------------------------------------------------- 4 bits
@@ -445,19 +452,43 @@ __global__ void __launch_bounds__(THREADS) mx4_restore_kernel(const unsigned cha
   }
 }
 
-// Rows copied to a stride that TMA takes: a thread stores 8 elements as one vector.
-__global__ void __launch_bounds__(THREADS) mx8_pack_kernel(const uint16_t* __restrict__ src, uint4* __restrict__ dst,
-                                                           int rows, int n, int ld8) {
-  const long long total = (long long)rows * ld8;
-  for (long long i = blockIdx.x * (long long)THREADS + threadIdx.x; i < total; i += (long long)gridDim.x * THREADS) {
-    const int r = (int)(i / ld8), c = (int)(i % ld8) * 8;
-    const uint16_t* p = src + (long long)r * n + c;
+// Rows of 16-bit elements copied to a stride that TMA takes: a thread stores 8 elements as one vector.
+struct PackJob {
+  const uint16_t* src;
+  uint4* dst;
+  int rows, n, ld8;
+};
+__device__ __forceinline__ void pack_rows(const PackJob& j, int block, int blocks) {
+  const long long total = (long long)j.rows * j.ld8;
+  for (long long i = block * (long long)THREADS + threadIdx.x; i < total; i += (long long)blocks * THREADS) {
+    const int r = (int)(i / j.ld8), c = (int)(i % j.ld8) * 8;
+    const uint16_t* p = j.src + (long long)r * j.n + c;
     uint4 v;
     uint16_t* h = reinterpret_cast<uint16_t*>(&v);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) h[j] = c + j < n ? __ldg(p + j) : (uint16_t)0;
-    dst[i] = v;
+    for (int k = 0; k < 8; ++k) h[k] = c + k < j.n ? __ldg(p + k) : (uint16_t)0;
+    j.dst[i] = v;
   }
+}
+int pack_blocks(const PackJob& j) {
+  const long long n = ((long long)j.rows * j.ld8 + THREADS - 1) / THREADS;
+  return (int)(n < 148 * 8 ? n : 148 * 8);
+}
+__global__ void __launch_bounds__(THREADS) mx8_pack_kernel(const PackJob a, const PackJob b, int blocks_a) {
+  if ((int)blockIdx.x < blocks_a)
+    pack_rows(a, blockIdx.x, blocks_a);
+  else
+    pack_rows(b, blockIdx.x - blocks_a, gridDim.x - blocks_a);
+}
+// f(x^) of a checkpoint and the copy of another operand in one launch: the last `blocks_b` rows of blocks copy
+template <typename T, int ACT>
+__global__ void __launch_bounds__(THREADS)
+    mx8_restore_pack_kernel(const signed char* __restrict__ codes, const unsigned char* __restrict__ scales,
+                            T* __restrict__ out, int D, int cols, int nb, long long ld_out, const PackJob j, int rows_r) {
+  if ((int)blockIdx.y < rows_r)
+    restore_tile<T, ACT, true>(codes, scales, out, D, cols, nb, ld_out);
+  else
+    pack_rows(j, (blockIdx.y - rows_r) * gridDim.x + blockIdx.x, (gridDim.y - rows_r) * gridDim.x);
 }
 
 template <typename T>
@@ -510,12 +541,37 @@ int launch_mx8_restore(const signed char* codes, const unsigned char* scales, vo
   return check_launch("8-bit restore");
 }
 
-int launch_mx8_pack(const void* src, void* dst, int rows, int n, long long ld, cudaStream_t s) {
-  const long long blocks = ((long long)rows * (ld / 8) + THREADS - 1) / THREADS;
-  mx8_pack_kernel<<<(int)(blocks < 148 * 8 ? blocks : 148 * 8), THREADS, 0, s>>>(
-      static_cast<const uint16_t*>(src), static_cast<uint4*>(dst), rows, n, (int)(ld / 8));
+int launch_mx8_pack(const void* src_a, void* dst_a, int rows_a, int n_a, long long ld_a, const void* src_b, void* dst_b,
+                    int rows_b, int n_b, long long ld_b, cudaStream_t s) {
+  const PackJob a{static_cast<const uint16_t*>(src_a), static_cast<uint4*>(dst_a), src_a ? rows_a : 0, n_a, (int)(ld_a / 8)};
+  const PackJob b{static_cast<const uint16_t*>(src_b), static_cast<uint4*>(dst_b), src_b ? rows_b : 0, n_b, (int)(ld_b / 8)};
+  const int blocks_a = src_a ? pack_blocks(a) : 0, blocks_b = src_b ? pack_blocks(b) : 0;
+  if (blocks_a + blocks_b == 0) return IPC_OK;
+  mx8_pack_kernel<<<blocks_a + blocks_b, THREADS, 0, s>>>(a, b, blocks_a);
   count_launch();
   return check_launch("row copy");
+}
+
+int launch_mx8_restore_pack(const signed char* codes, const unsigned char* scales, void* out, int D, int B,
+                            long long ld_out, const void* src, void* dst, int rows, int act, int dtype, cudaStream_t s) {
+  const int nb = (int)(mx8_ld(B) / MX_BLOCK);
+  dim3 grid;
+  const int rc = grid_of("8-bit restore", D, TR, B, &grid);
+  if (rc) return rc;
+  const PackJob j{static_cast<const uint16_t*>(src), static_cast<uint4*>(dst), rows, B, (int)(ld_out / 8)};
+  const int rows_r = grid.y;
+  long long extra = (pack_blocks(j) + grid.x - 1) / grid.x;
+  if (rows_r + extra > 65535) extra = 65535 - rows_r;
+  if (extra < 1) return set_error(IPC_ERR_ARG, "8-bit restore: %d rows are too many", D);
+  grid.y += (unsigned)extra;
+  IPC_DISPATCH_DT16(dtype, TT, {
+    TT* ot = static_cast<TT*>(out);
+    IPC_DISPATCH_ACT(act, AC, {
+      mx8_restore_pack_kernel<TT, AC><<<grid, THREADS, 0, s>>>(codes, scales, ot, D, B, nb, ld_out, j, rows_r);
+    });
+  });
+  count_launch();
+  return check_launch("8-bit restore");
 }
 
 int launch_mx4_quantize(const void* x, unsigned char* codes, unsigned char* scales, int R, int K, int turned, int act,

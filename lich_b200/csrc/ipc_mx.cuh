@@ -84,8 +84,13 @@ int launch_mx8_store(const void* x, signed char* codes, unsigned char* scales, i
 // out[d][b] = cast(f(codes * 2^s)), rows ld_out >= B apart
 int launch_mx8_restore(const signed char* codes, const unsigned char* scales, void* out, int D, int B, long long ld_out,
                        int act, int dtype, cudaStream_t s);
-// dst [rows][ld] = src [rows][n], 16-bit elements (ld a multiple of 8, dst 16-byte aligned; columns n .. ld - 1 undefined)
-int launch_mx8_pack(const void* src, void* dst, int rows, int n, long long ld, cudaStream_t s);
+// Up to two copies dst [rows][ld] = src [rows][n] of 16-bit elements in one launch (a null src: none; ld a multiple of 8,
+// dst 16-byte aligned, columns n .. ld - 1 zeroed)
+int launch_mx8_pack(const void* src_a, void* dst_a, int rows_a, int n_a, long long ld_a, const void* src_b, void* dst_b,
+                    int rows_b, int n_b, long long ld_b, cudaStream_t s);
+// launch_mx8_restore and such a copy of src [rows][B] to the same stride, in one launch (16-bit storage)
+int launch_mx8_restore_pack(const signed char* codes, const unsigned char* scales, void* out, int D, int B,
+                            long long ld_out, const void* src, void* dst, int rows, int act, int dtype, cudaStream_t s);
 // one-launch product with a checkpoint (p.ck, p.cks), any shape, 16-bit storage: MODE_W, _WD, _G, _BK
 int launch_mx8_small(const GemmArgs& p, int mode, int act, int dtype, cudaStream_t s);
 int launch_mx4_quantize(const void* x, unsigned char* codes, unsigned char* scales, int R, int K, int turned, int act,

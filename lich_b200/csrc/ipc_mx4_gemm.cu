@@ -353,6 +353,130 @@ __global__ void __launch_bounds__(F_THREADS, 1)
   }
 }
 
+// ----------------------------------------------------------------------------------- few samples
+// A whole tile of the kernel above costs its set-up (8 us for a single sample) whatever it holds.  Here a warp owns 16
+// rows x 8 NB samples and a part of K; codes go from global memory to registers, are widened to fp16 (exact) and multiplied by
+// mma.sync a block of 32 columns at a time (two MMAs into zeros), and the block's sum is scaled into the fp32
+// accumulator: (c * 2^sw) * 2^sa.  Which of a block's columns an MMA's k stands for is free as long as both operands
+// agree, so lane t of a quad takes 8 neighbouring columns: 4 bytes of each row.  The KW warps of a row block add up in
+// shared memory in warp order.  One read of W: 4096 x 4096 x 1 is 8.9 MB.
+constexpr int G_WARPS = 8;
+
+__device__ __forceinline__ void g_mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                      uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// the four scale bytes of an atom's row (0 for a row past the operand: its codes are not read either)
+__device__ __forceinline__ uint32_t g_scales(const unsigned char* sc, int r, int rows, int atom, int atoms) {
+  return r < rows ? __ldg(reinterpret_cast<const uint32_t*>(sc + mx4_scale_at(r, 4 * atom, atoms))) : 0u;
+}
+
+template <typename T, int NB>
+__global__ void __launch_bounds__(32 * G_WARPS)
+    mx4_small_kernel(const unsigned char* __restrict__ w, const unsigned char* __restrict__ wsc,
+                     const unsigned char* __restrict__ a, const unsigned char* __restrict__ asc, T* __restrict__ out,
+                     int M, int B, int kp, int kw) {
+  __shared__ float red[G_WARPS][16][8 * NB + 1];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const int part = warp % kw;  // this warp's share of K
+  const int m0 = (blockIdx.x * (G_WARPS / kw) + warp / kw) * 16, n0 = blockIdx.y * 8 * NB;
+  const int atoms = kp / 128, ldc = kp / 2;
+  float acc[NB][4] = {};
+  const unsigned char* w0 = w + (long long)(m0 + g) * ldc + 4 * t;
+  const unsigned char* w1 = w0 + 8LL * ldc;
+  const bool in0 = m0 + g < M, in1 = m0 + g + 8 < M;
+  struct Atom {
+    uint32_t cw[4][2], ca[4][NB], sw[2], sa[NB][2];
+  };
+  auto fetch = [&](Atom& f, int at) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int o = 64 * at + 16 * j;
+      f.cw[j][0] = in0 ? __ldg(reinterpret_cast<const uint32_t*>(w0 + o)) : 0u;
+      f.cw[j][1] = in1 ? __ldg(reinterpret_cast<const uint32_t*>(w1 + o)) : 0u;
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        const int n = n0 + 8 * b + g;
+        f.ca[j][b] = n < B ? __ldg(reinterpret_cast<const uint32_t*>(a + (long long)n * ldc + 4 * t + o)) : 0u;
+      }
+    }
+    f.sw[0] = g_scales(wsc, m0 + g, M, at, atoms);
+    f.sw[1] = g_scales(wsc, m0 + g + 8, M, at, atoms);
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      f.sa[b][0] = g_scales(asc, n0 + 8 * b + 2 * t, B, at, atoms);
+      f.sa[b][1] = g_scales(asc, n0 + 8 * b + 2 * t + 1, B, at, atoms);
+    }
+  };
+  Atom cur, next;
+  if (part < atoms) fetch(cur, part);
+  for (int at = part; at < atoms; at += kw) {
+    if (at + kw < atoms) fetch(next, at + kw);  // the next atom's loads under this one's MMAs
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      uint32_t x0[4], x1[4];
+      mx4_unpack8(cur.cw[j][0], x0);
+      mx4_unpack8(cur.cw[j][1], x1);
+      const float f0 = mx_scale((cur.sw[0] >> (8 * j)) & 255u), f1 = mx_scale((cur.sw[1] >> (8 * j)) & 255u);
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        uint32_t y[4];
+        mx4_unpack8(cur.ca[j][b], y);
+        float c[4] = {};
+        g_mma(c, x0[0], x1[0], x0[1], x1[1], y[0], y[1]);
+        g_mma(c, x0[2], x1[2], x0[3], x1[3], y[2], y[3]);
+        const float h0 = mx_scale((cur.sa[b][0] >> (8 * j)) & 255u), h1 = mx_scale((cur.sa[b][1] >> (8 * j)) & 255u);
+        acc[b][0] = fmaf(c[0] * f0, h0, acc[b][0]);
+        acc[b][1] = fmaf(c[1] * f0, h1, acc[b][1]);
+        acc[b][2] = fmaf(c[2] * f1, h0, acc[b][2]);
+        acc[b][3] = fmaf(c[3] * f1, h1, acc[b][3]);
+      }
+    }
+    cur = next;
+  }
+  if (kw > 1) {
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) red[warp][g + (r >= 2 ? 8 : 0)][8 * b + 2 * t + (r & 1)] = acc[b][r];
+    __syncthreads();
+    for (int i = threadIdx.x; i < G_WARPS / kw * 16 * 8 * NB; i += 32 * G_WARPS) {
+      const int n = i % (8 * NB), r = i / (8 * NB) % 16, rb = i / (16 * 8 * NB);
+      const int m = (blockIdx.x * (G_WARPS / kw) + rb) * 16 + r;
+      float sum = 0.f;
+      for (int k = 0; k < kw; ++k) sum += red[rb * kw + k][r][n];
+      if (m < M && n0 + n < B) out[(long long)m * B + n0 + n] = St<T>::st(sum);
+    }
+  } else {
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int m = m0 + g + (r >= 2 ? 8 : 0), n = n0 + 8 * b + 2 * t + (r & 1);
+        if (m < M && n < B) out[(long long)m * B + n] = St<T>::st(acc[b][r]);
+      }
+  }
+}
+
+template <typename T>
+int launch_few(const unsigned char* w, const unsigned char* wsc, const unsigned char* a, const unsigned char* asc,
+               void* out, int M, int K, int B, cudaStream_t s) {
+  const int kp = (int)mx4_kp(K), atoms = kp / 128;
+  const int kw = atoms >= 8 ? 8 : atoms >= 4 ? 4 : atoms >= 2 ? 2 : 1;
+  const int rows = 16 * (G_WARPS / kw);
+  const int nb = B <= 8 ? 1 : 2;
+  const dim3 grid((unsigned)((M + rows - 1) / rows), (unsigned)((B + 8 * nb - 1) / (8 * nb)));
+  T* o = static_cast<T*>(out);
+  if (nb == 1)
+    mx4_small_kernel<T, 1><<<grid, 32 * G_WARPS, 0, s>>>(w, wsc, a, asc, o, M, B, kp, kw);
+  else
+    mx4_small_kernel<T, 2><<<grid, 32 * G_WARPS, 0, s>>>(w, wsc, a, asc, o, M, B, kp, kw);
+  count_launch();
+  return check_launch("4-bit product of few samples");
+}
+
 // ------------------------------------------------------------------------------------------ host
 PFN_cuTensorMapEncodeTiled_v12000 f_encode() {
   static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
@@ -453,6 +577,7 @@ int launch_mx4_gemm(const unsigned char* w, const unsigned char* wsc, const unsi
       count_launch();
       return check_launch("4-bit product of no columns");
     }
+    if (B <= 16) return launch_few<TT>(w, wsc, a, asc, out, M, K, B, s);
     return wide ? launch_tiles<TT, 256>(w, wsc, a, asc, out, M, K, B, s)
                 : launch_tiles<TT, 128>(w, wsc, a, asc, out, M, K, B, s);
   });
