@@ -478,9 +478,7 @@ static Mx8WeightWs mx8_weight_ws(int mode, int M, int K, int B, int dtype, int a
     w.values = up256((size_t)K * w.ld * 2);
     w.e = B % 8 ? up256((size_t)M * w.ld * 2) : 0;
     w.delta = (mode == MODE_W && K % 8) ? up256((size_t)M * K * 4) : 0;
-    // split-K: its partial sums and second pass cost about 10 us, which a batch below 2048 does not win back
-    // (1000 x 1021 x 777: 26 us split in three, 11 us in one)
-    w.partial = B >= 2048 ? IPC_SPLITK_WS_BYTES : 0;
+    w.partial = B > 4032 ? TAIL_FLAG_BYTES + IPC_SPLITK_WS_BYTES : 0;  // a last round of tiles halved along the batch
   }
   w.total = w.values + w.e + w.delta + w.partial;
   return w;
@@ -531,22 +529,28 @@ int ipc_mx8_weight(int mode, void* out, const void* e, const signed char* codes,
   if (w.values == 0 || (direct && !aligned16(e)) || (mode == MODE_W && K % 8 == 0 && !aligned16(out)))
     return launch_mx8_small(p, mode, act, dtype, s);
   char* ws = static_cast<char*>(workspace);
+  p.tail_ws = w.partial ? ws + w.values + w.e + w.delta : nullptr;
+  p.tail_bytes = w.partial;
+  // with fewer tiles than half the SMs: split-K over the same space, behind the flags
+  float* part = w.partial ? reinterpret_cast<float*>(static_cast<char*>(p.tail_ws) + TAIL_FLAG_BYTES) : nullptr;
+  const size_t part_bytes = w.partial ? w.partial - TAIL_FLAG_BYTES : 0;
+  int* tail_flags = static_cast<int*>(p.tail_ws);
+  const int n_flags = w.partial ? (int)(TAIL_FLAG_BYTES / 4) : 0;
   if (direct) {
-    rc = launch_mx8_restore(codes, scales, ws, K, B, w.ld, act, dtype, s);
+    rc = launch_mx8_restore(codes, scales, ws, K, B, w.ld, act, dtype, s, tail_flags, n_flags);
   } else {
-    rc = launch_mx8_restore_pack(codes, scales, ws, K, B, w.ld, e, ws + w.values, M, act, dtype, s);
+    rc = launch_mx8_restore_pack(codes, scales, ws, K, B, w.ld, e, ws + w.values, M, act, dtype, s, tail_flags, n_flags);
     p.A = ws + w.values;
   }
   if (rc) return rc;
   p.lda = w.ld; p.gsA = (long long)M * w.ld;
   p.Bm = ws; p.ldb = w.ld; p.gsB = (long long)K * w.ld;
   p.ck = nullptr;
-  float* part = w.partial ? reinterpret_cast<float*>(ws + w.values + w.e + w.delta) : nullptr;
-  if (aligned16(out) && K % 8 == 0) return launch_tc(p, mode, act, dtype, s, part, w.partial);
+  if (aligned16(out) && K % 8 == 0) return launch_tc(p, mode, act, dtype, s, part, part_bytes);
   p.ragged = 1;
-  if (mode != MODE_W) return launch_tc(p, mode, act, dtype, s, part, w.partial);
+  if (mode != MODE_W) return launch_tc(p, mode, act, dtype, s, part, part_bytes);
   p.out = ws + w.values + w.e;  // W with ragged rows: the fp32 delta, then W += delta
-  rc = launch_tc(p, MODE_WD, act, dtype, s, part, w.partial);
+  rc = launch_tc(p, MODE_WD, act, dtype, s, part, part_bytes);
   if (rc) return rc;
   return launch_apply(out, static_cast<const float*>(p.out), (long long)M * K, dtype, s);
 }

@@ -43,6 +43,8 @@ __device__ __forceinline__ float opt_step(const OptParams& o, float w, float g, 
   return w - o.lr * g;
 }
 
+constexpr size_t TAIL_FLAG_BYTES = 8192;  // a flag per epilogue warp of every CTA: 148 x 8
+
 // C[m,n] = sum_k A(m,k) B(k,n) per group, then a MODE epilogue on the
 // row-major [Mg, Ng] output.  Orientation (fixed by MODE):
 //   P, F : A(m,k) = A[m*lda + k]   B(k,n) = B[k*ldb + n]   (Mg,Ng,Kg) = (M,B,K)
@@ -68,6 +70,10 @@ struct GemmArgs {
   const signed char* ck;     // BK: 8-bit checkpoint of the [Mg, Ng] states, codes ld_ck apart, 16-byte aligned ...
   const unsigned char* cks;  // ... and its scale bytes [ceil(Ng / 32)][Mg]  (ipc_mx.cuh)
   long long ld_ck;
+  // W, WD, G: workspace that lets the tiles of the last, partly filled round be halved along the reduction (its flags, the
+  // first TAIL_FLAG_BYTES, zeroed by an earlier kernel of the stream); null: no such split
+  void* tail_ws;
+  size_t tail_bytes;
   int ragged;       // WD, G, BK: rows of out start anywhere (odd Ng, or a view); lda and ldb still suit TMA
 };
 

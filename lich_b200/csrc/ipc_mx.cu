@@ -84,6 +84,12 @@ __device__ __forceinline__ float act_for(float v) {
   return act_full<ACT>(v);
 }
 
+// words of a later kernel's workspace, cleared by the first CTA
+__device__ __forceinline__ void zero_words(int* zero, int n) {
+  if (blockIdx.x == 0 && blockIdx.y == 0)
+    for (int i = threadIdx.x; i < n; i += THREADS) zero[i] = 0;
+}
+
 // ---------------------------------------------------------------------------- 8 bits
 // VEC: rows start on 16-byte boundaries (so B is a multiple of a vector); 4 threads a block (8 in fp32).
 template <typename T, bool VEC>
@@ -177,8 +183,9 @@ __device__ __forceinline__ void restore_tile(const signed char* __restrict__ cod
       const float sc = mx_scale(byte[it]);
       float v[N];
 #pragma unroll
-      for (int j = 0; j < N; ++j)
-        v[j] = act_for<T, ACT>((float)(signed char)(w[it][j / 4] >> (8 * (j % 4))) * sc);
+      for (int q = 0; q < N / 4; ++q) mx8_floats(w[it][q], v + 4 * q);
+#pragma unroll
+      for (int j = 0; j < N; ++j) v[j] = act_for<T, ACT>(v[j] * sc);
       T* o = out + (long long)d * ld_out + c;
       if (c + N <= cols) {
         Vec<T>::store(o, v);
@@ -212,7 +219,8 @@ __device__ __forceinline__ void restore_tile(const signed char* __restrict__ cod
 template <typename T, int ACT, bool VEC>
 __global__ void __launch_bounds__(THREADS)
     mx8_restore_kernel(const signed char* __restrict__ codes, const unsigned char* __restrict__ scales,
-                       T* __restrict__ out, int D, int cols, int nb, long long ld_out) {
+                       T* __restrict__ out, int D, int cols, int nb, long long ld_out, int* zero, int n_zero) {
+  zero_words(zero, n_zero);
   restore_tile<T, ACT, VEC>(codes, scales, out, D, cols, nb, ld_out);
 }
 
@@ -484,7 +492,9 @@ __global__ void __launch_bounds__(THREADS) mx8_pack_kernel(const PackJob a, cons
 template <typename T, int ACT>
 __global__ void __launch_bounds__(THREADS)
     mx8_restore_pack_kernel(const signed char* __restrict__ codes, const unsigned char* __restrict__ scales,
-                            T* __restrict__ out, int D, int cols, int nb, long long ld_out, const PackJob j, int rows_r) {
+                            T* __restrict__ out, int D, int cols, int nb, long long ld_out, const PackJob j, int rows_r, int* zero,
+                            int n_zero) {
+  zero_words(zero, n_zero);
   if ((int)blockIdx.y < rows_r)
     restore_tile<T, ACT, true>(codes, scales, out, D, cols, nb, ld_out);
   else
@@ -522,7 +532,7 @@ int launch_mx8_store(const void* x, signed char* codes, unsigned char* scales, i
 }
 
 int launch_mx8_restore(const signed char* codes, const unsigned char* scales, void* out, int D, int B, long long ld_out,
-                       int act, int dtype, cudaStream_t s) {
+                       int act, int dtype, cudaStream_t s, int* zero, int n_zero) {
   const int nb = (int)(mx8_ld(B) / MX_BLOCK);
   dim3 grid;
   int rc = grid_of("8-bit restore", D, TR, B, &grid);
@@ -532,9 +542,9 @@ int launch_mx8_restore(const signed char* codes, const unsigned char* scales, vo
     const bool vec = rows_aligned<TT>(out, ld_out);
     IPC_DISPATCH_ACT(act, AC, {
       if (vec)
-        mx8_restore_kernel<TT, AC, true><<<grid, THREADS, 0, s>>>(codes, scales, ot, D, B, nb, ld_out);
+        mx8_restore_kernel<TT, AC, true><<<grid, THREADS, 0, s>>>(codes, scales, ot, D, B, nb, ld_out, zero, n_zero);
       else
-        mx8_restore_kernel<TT, AC, false><<<grid, THREADS, 0, s>>>(codes, scales, ot, D, B, nb, ld_out);
+        mx8_restore_kernel<TT, AC, false><<<grid, THREADS, 0, s>>>(codes, scales, ot, D, B, nb, ld_out, zero, n_zero);
     });
   });
   count_launch();
@@ -553,7 +563,8 @@ int launch_mx8_pack(const void* src_a, void* dst_a, int rows_a, int n_a, long lo
 }
 
 int launch_mx8_restore_pack(const signed char* codes, const unsigned char* scales, void* out, int D, int B,
-                            long long ld_out, const void* src, void* dst, int rows, int act, int dtype, cudaStream_t s) {
+                            long long ld_out, const void* src, void* dst, int rows, int act, int dtype, cudaStream_t s,
+                            int* zero, int n_zero) {
   const int nb = (int)(mx8_ld(B) / MX_BLOCK);
   dim3 grid;
   const int rc = grid_of("8-bit restore", D, TR, B, &grid);
@@ -567,7 +578,8 @@ int launch_mx8_restore_pack(const signed char* codes, const unsigned char* scale
   IPC_DISPATCH_DT16(dtype, TT, {
     TT* ot = static_cast<TT*>(out);
     IPC_DISPATCH_ACT(act, AC, {
-      mx8_restore_pack_kernel<TT, AC><<<grid, THREADS, 0, s>>>(codes, scales, ot, D, B, nb, ld_out, j, rows_r);
+      mx8_restore_pack_kernel<TT, AC><<<grid, THREADS, 0, s>>>(codes, scales, ot, D, B, nb, ld_out, j, rows_r, zero,
+                                                                 n_zero);
     });
   });
   count_launch();

@@ -38,6 +38,14 @@ __device__ __forceinline__ float mx_inv_scale(uint32_t byte) {
 // One 8-bit code.  A block marked NaN multiplies by 0: v * 0 is 0 or NaN, and NaN converts to 0.
 __device__ __forceinline__ int mx8_code(float v, float inv) { return __float2int_rn(v * inv); }
 
+// The four codes of a word as floats: a code + 128 in the low byte of 2^23's mantissa, less 2^23 + 128 (exact; two ALU
+// operations each, where a conversion would take the slower pipe that f's MUFU forms need).
+__device__ __forceinline__ void mx8_floats(uint32_t codes, float* v) {
+  const uint32_t u = codes ^ 0x80808080u;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7540u + i)) - 8388736.f;
+}
+
 // Eight numbers (already scaled, |v| <= 6) as 4-bit codes, the first in the lowest bits.
 __device__ __forceinline__ uint32_t mx4_pack8(const float (&v)[8]) {
   uint32_t r;
@@ -81,16 +89,17 @@ __device__ __forceinline__ long long mx4_scale_at(int r, int j, int atoms_k) {
 }
 
 int launch_mx8_store(const void* x, signed char* codes, unsigned char* scales, int D, int B, int dtype, cudaStream_t s);
-// out[d][b] = cast(f(codes * 2^s)), rows ld_out >= B apart
+// out[d][b] = cast(f(codes * 2^s)), rows ld_out >= B apart; n_zero words at `zero` are cleared beside it
 int launch_mx8_restore(const signed char* codes, const unsigned char* scales, void* out, int D, int B, long long ld_out,
-                       int act, int dtype, cudaStream_t s);
+                       int act, int dtype, cudaStream_t s, int* zero = nullptr, int n_zero = 0);
 // Up to two copies dst [rows][ld] = src [rows][n] of 16-bit elements in one launch (a null src: none; ld a multiple of 8,
 // dst 16-byte aligned, columns n .. ld - 1 zeroed)
 int launch_mx8_pack(const void* src_a, void* dst_a, int rows_a, int n_a, long long ld_a, const void* src_b, void* dst_b,
                     int rows_b, int n_b, long long ld_b, cudaStream_t s);
 // launch_mx8_restore and such a copy of src [rows][B] to the same stride, in one launch (16-bit storage)
 int launch_mx8_restore_pack(const signed char* codes, const unsigned char* scales, void* out, int D, int B,
-                            long long ld_out, const void* src, void* dst, int rows, int act, int dtype, cudaStream_t s);
+                            long long ld_out, const void* src, void* dst, int rows, int act, int dtype, cudaStream_t s,
+                            int* zero = nullptr, int n_zero = 0);
 // one-launch product with a checkpoint (p.ck, p.cks), any shape, 16-bit storage: MODE_W, _WD, _G, _BK
 int launch_mx8_small(const GemmArgs& p, int mode, int act, int dtype, cudaStream_t s);
 int launch_mx4_quantize(const void* x, unsigned char* codes, unsigned char* scales, int R, int K, int turned, int act,

@@ -96,7 +96,8 @@ __device__ __forceinline__ uint4 shifted(const Row8<VEC>& r, int left) {
   return make_uint4(o[0], o[1], o[2], o[3]);
 }
 
-template <typename T, int ACT, int MODE, bool VEC>
+// VA, VB: the A operand (E; W for BK) and the E of BK load in whole vectors.
+template <typename T, int ACT, int MODE, bool VA, bool VB>
 __global__ void __launch_bounds__(STHREADS) mx8_small_kernel(const __grid_constant__ GemmArgs p, int k_per_split) {
   constexpr bool BKM = MODE == MODE_BK;
   constexpr int LDA = BKM ? SM + 8 : SK + 8, LDB = BKM ? SN + 8 : SK + 8;  // shared rows, 16 bytes apart mod 128
@@ -115,7 +116,8 @@ __global__ void __launch_bounds__(STHREADS) mx8_small_kernel(const __grid_consta
 
   constexpr int NA = SM * SK / 8 / STHREADS;                       // 16-byte vectors of A a thread moves a step: 2
   constexpr int NB = BKM ? SN * SK / 8 / STHREADS : SN * SK / 16 / STHREADS;  // of E: 4; of codes: 2
-  Row8<VEC> ra[NA], rbe[BKM ? NB : 1];
+  Row8<VA> ra[NA];
+  Row8<VB> rbe[BKM ? NB : 1];
   uint4 rb[NB];
   uint32_t rs[NB];
   auto fetch = [&](int k0) {
@@ -124,10 +126,10 @@ __global__ void __launch_bounds__(STHREADS) mx8_small_kernel(const __grid_consta
       const int i = tid + STHREADS * j;
       if constexpr (BKM) {  // W rows k0.., columns m0..
         const int r = i / (SM / 8), c = i % (SM / 8) * 8;
-        ra[j] = row8<T, VEC>(A + (long long)(k0 + r) * p.lda, m0 + c, p.Mg, k0 + r < k_hi, A, A + (long long)p.Kg * p.lda);
+        ra[j] = row8<T, VA>(A + (long long)(k0 + r) * p.lda, m0 + c, p.Mg, k0 + r < k_hi, A, A + (long long)p.Kg * p.lda);
       } else {
         const int r = i / (SK / 8), c = i % (SK / 8) * 8;
-        ra[j] = row8<T, VEC>(A + (long long)(m0 + r) * p.lda, k0 + c, p.Kg, m0 + r < p.Mg, A, A + (long long)p.Mg * p.lda);
+        ra[j] = row8<T, VA>(A + (long long)(m0 + r) * p.lda, k0 + c, p.Kg, m0 + r < p.Mg, A, A + (long long)p.Mg * p.lda);
       }
     }
 #pragma unroll
@@ -135,7 +137,7 @@ __global__ void __launch_bounds__(STHREADS) mx8_small_kernel(const __grid_consta
       const int i = tid + STHREADS * j;
       if constexpr (BKM) {
         const int r = i / (SN / 8), c = i % (SN / 8) * 8;
-        rbe[j] = row8<T, VEC>(E + (long long)(k0 + r) * p.ldb, n0 + c, p.Ng, k0 + r < k_hi, E, E + (long long)p.Kg * p.ldb);
+        rbe[j] = row8<T, VB>(E + (long long)(k0 + r) * p.ldb, n0 + c, p.Ng, k0 + r < k_hi, E, E + (long long)p.Kg * p.ldb);
       } else {  // 16 codes and their scale byte
         const int r = i / (SK / 16), c = i % (SK / 16) * 16;
         rb[j] = make_uint4(0, 0, 0, 0);
@@ -155,22 +157,26 @@ __global__ void __launch_bounds__(STHREADS) mx8_small_kernel(const __grid_consta
       const int i = tid + STHREADS * j;
       const int w = BKM ? SM / 8 : SK / 8;
       // (past a row's end lie the next row's numbers: of no effect in columns that are not stored, zeros for the sum)
-      *reinterpret_cast<uint4*>(a + (i / w) * LDA + i % w * 8) = shifted<VEC>(ra[j], BKM ? 8 : p.Kg - k0 - i % w * 8);
+      *reinterpret_cast<uint4*>(a + (i / w) * LDA + i % w * 8) = shifted<VA>(ra[j], BKM ? 8 : p.Kg - k0 - i % w * 8);
     }
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
       const int i = tid + STHREADS * j;
       if constexpr (BKM) {
-        *reinterpret_cast<uint4*>(b + (i / (SN / 8)) * LDB + i % (SN / 8) * 8) = shifted<VEC>(rbe[j], 8);
+        *reinterpret_cast<uint4*>(b + (i / (SN / 8)) * LDB + i % (SN / 8) * 8) = shifted<VB>(rbe[j], 8);
       } else {
         const int r = i / (SK / 16), c = i % (SK / 16) * 16;
-        const signed char* q = reinterpret_cast<const signed char*>(&rb[j]);
+        float q[16];
+        mx8_floats(rb[j].x, q);
+        mx8_floats(rb[j].y, q + 4);
+        mx8_floats(rb[j].z, q + 8);
+        mx8_floats(rb[j].w, q + 12);
         const float sc = mx_scale(rs[j]);
         const bool in = n0 + r < p.Ng;
         uint4 o[2];
         T* h = reinterpret_cast<T*>(o);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) h[e] = St<T>::st(in && k0 + c + e < k_hi ? act_f_hw<ACT>((float)q[e] * sc) : 0.f);
+        for (int e = 0; e < 16; ++e) h[e] = St<T>::st(in && k0 + c + e < k_hi ? act_f_hw<ACT>(q[e] * sc) : 0.f);
         uint4* dst = reinterpret_cast<uint4*>(b + r * LDB + c);
         dst[0] = o[0];
         dst[1] = o[1];
@@ -248,7 +254,7 @@ __global__ void __launch_bounds__(STHREADS) mx8_small_kernel(const __grid_consta
     }
 }
 
-template <typename T, int ACT, int MODE, bool VEC>
+template <typename T, int ACT, int MODE, bool VA, bool VB>
 int launch_small_t(const GemmArgs& p, cudaStream_t s) {
   constexpr bool BKM = MODE == MODE_BK;
   const long long gx = (p.Ng + SN - 1) / SN, gy = (p.Mg + SM - 1) / SM;
@@ -263,7 +269,7 @@ int launch_small_t(const GemmArgs& p, cudaStream_t s) {
   C = steps > 0 ? (int)((steps + per - 1) / per) : 1;
   constexpr int TILES = 2 * (BKM ? SK * (SM + 8) + SK * (SN + 8) : (SM + SN) * (SK + 8)) * 2;
   const int smem = TILES + (C - 1) * SM * SN * 4;
-  cudaError_t err = ensure_kernel_smem<mx8_small_kernel<T, ACT, MODE, VEC>>(TILES + (S_MAX_SPLIT - 1) * SM * SN * 4);
+  cudaError_t err = ensure_kernel_smem<mx8_small_kernel<T, ACT, MODE, VA, VB>>(TILES + (S_MAX_SPLIT - 1) * SM * SN * 4);
   if (err != cudaSuccess) return set_error(IPC_ERR_CUDA, "checkpoint product smem attribute: %s", cudaGetErrorString(err));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)gx, (unsigned)gy, C);
@@ -277,7 +283,7 @@ int launch_small_t(const GemmArgs& p, cudaStream_t s) {
   attr[0].val.clusterDim.z = C;
   cfg.attrs = attr;
   cfg.numAttrs = C > 1 ? 1 : 0;
-  err = cudaLaunchKernelEx(&cfg, mx8_small_kernel<T, ACT, MODE, VEC>, p, (int)(per * SK));
+  err = cudaLaunchKernelEx(&cfg, mx8_small_kernel<T, ACT, MODE, VA, VB>, p, (int)(per * SK));
   if (err != cudaSuccess) return set_error(IPC_ERR_CUDA, "checkpoint product launch: %s", cudaGetErrorString(err));
   count_launch();
   return check_launch("checkpoint product");
@@ -287,16 +293,17 @@ int launch_small_t(const GemmArgs& p, cudaStream_t s) {
 
 int launch_mx8_small(const GemmArgs& p, int mode, int act, int dtype, cudaStream_t s) {
   const bool bk = mode == MODE_BK;
-  const uintptr_t bits = reinterpret_cast<uintptr_t>(p.A) | (uintptr_t)(p.lda * 2) |
-                         (bk ? reinterpret_cast<uintptr_t>(p.Bm) | (uintptr_t)(p.ldb * 2) : 0);
-  const bool vec = (bits & 15) == 0 && (bk ? p.Mg % 8 == 0 && p.Ng % 8 == 0 : p.Kg % 8 == 0);
+  const bool va = ((reinterpret_cast<uintptr_t>(p.A) | (uintptr_t)(p.lda * 2)) & 15) == 0 && (bk ? p.Mg : p.Kg) % 8 == 0;
+  const bool vb = ((reinterpret_cast<uintptr_t>(p.Bm) | (uintptr_t)(p.ldb * 2)) & 15) == 0 && p.Ng % 8 == 0;
   IPC_DISPATCH_DT16(dtype, TT, {
     IPC_DISPATCH_ACT(act, AC, {
       switch (mode) {
-        case MODE_W: return vec ? launch_small_t<TT, AC, MODE_W, true>(p, s) : launch_small_t<TT, AC, MODE_W, false>(p, s);
-        case MODE_WD: return vec ? launch_small_t<TT, AC, MODE_WD, true>(p, s) : launch_small_t<TT, AC, MODE_WD, false>(p, s);
-        case MODE_G: return vec ? launch_small_t<TT, AC, MODE_G, true>(p, s) : launch_small_t<TT, AC, MODE_G, false>(p, s);
-        case MODE_BK: return vec ? launch_small_t<TT, AC, MODE_BK, true>(p, s) : launch_small_t<TT, AC, MODE_BK, false>(p, s);
+        case MODE_W: return va ? launch_small_t<TT, AC, MODE_W, true, true>(p, s) : launch_small_t<TT, AC, MODE_W, false, true>(p, s);
+        case MODE_WD: return va ? launch_small_t<TT, AC, MODE_WD, true, true>(p, s) : launch_small_t<TT, AC, MODE_WD, false, true>(p, s);
+        case MODE_G: return va ? launch_small_t<TT, AC, MODE_G, true, true>(p, s) : launch_small_t<TT, AC, MODE_G, false, true>(p, s);
+        case MODE_BK:
+          if (va && vb) return launch_small_t<TT, AC, MODE_BK, true, true>(p, s);
+          return va ? launch_small_t<TT, AC, MODE_BK, true, false>(p, s) : launch_small_t<TT, AC, MODE_BK, false, false>(p, s);
         default: return set_error(IPC_ERR_ARG, "checkpoint product: bad mode %d", mode);
       }
     });

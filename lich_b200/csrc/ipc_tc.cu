@@ -43,6 +43,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <climits>
 #include <cstdio>
 #include <cstring>
 #include <mutex>
@@ -117,6 +118,13 @@ struct TcParams {
   const unsigned char* cks;
   long long ld_ck;
   int ragged;     // WD, G, BK: rows of out start on any element: stored a lane per column, not in 16-byte vectors
+  // The last round of tiles (W, WD, G; one group, splits == 1): units from tail_from on are the halves of the remaining
+  // tiles, tail_kps K blocks the first.  The first half owns the tile; the second leaves its fp32 accumulators in
+  // tail_ws, [tile][CTA of the pair][warp][32-column chunk][4 registers][lane], and raises a flag per warp; the owner's
+  // warps wait for theirs and add them.
+  int tail_from, tail_kps;
+  int* tail_flags;
+  float* tail_ws;
   int ws_ld;      // row stride of the split-K partials (Ng rounded up to 8)
 };
 
@@ -133,6 +141,7 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
 // first row it owns: tile row + 128 rank).
 __device__ __forceinline__ void tile_coords(const TcParams& p, int t, int bn, int& g, int& m0, int& n0, int& s,
                                             int tm = TC_BM, int rank = 0) {
+  if (t >= p.tail_from) t = p.tail_from + (t - p.tail_from) / 2;
   s = t % p.splits;
   t /= p.splits;
   const int tiles_mn = p.tiles_m * p.tiles_n;
@@ -144,6 +153,64 @@ __device__ __forceinline__ void tile_coords(const TcParams& p, int t, int bn, in
   const int within = r - band * p.raster * p.tiles_n;
   m0 = (first_m + within % band_m) * tm + TC_BM * rank;
   n0 = (within / band_m) * bn;
+}
+
+// K blocks of unit t (split index sp)
+__device__ __forceinline__ void k_range(const TcParams& p, int t, int sp, int nk, int& k0, int& k1) {
+  if (t >= p.tail_from) {
+    const bool second = (t - p.tail_from) & 1;
+    k0 = second ? p.tail_kps : 0;
+    k1 = second ? nk : p.tail_kps;
+  } else {
+    k0 = sp * p.kps;
+    k1 = min(nk, k0 + p.kps);
+  }
+}
+// Epilogue side of a halved tile: the slot of warp w of the CTA at `rank`, and the 32 accumulators of a lane's row in a chunk
+// (8 vectors: a warp instruction moves 512 bytes)
+__device__ __forceinline__ long long tail_slot(const TcParams& p, int t, int ncta, int rank, int w) {
+  return ((long long)((t - p.tail_from) / 2) * ncta + rank) * TC_EPI_WARPS + w;
+}
+template <int CHUNKS>
+__device__ __forceinline__ void tail_put(const TcParams& p, long long slot, int c, int lane, const uint32_t (&r)[32]) {
+  uint4* d = reinterpret_cast<uint4*>(p.tail_ws) + (slot * CHUNKS + c) * 256 + lane;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) __stcg(d + 32 * j, make_uint4(r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]));
+}
+template <int CHUNKS>
+__device__ __forceinline__ void tail_get(const TcParams& p, long long slot, int c, int lane, float4 (&v)[8]) {
+  const float4* d = reinterpret_cast<const float4*>(p.tail_ws) + (slot * CHUNKS + c) * 256 + lane;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = __ldcg(d + 32 * j);
+}
+__device__ __forceinline__ void tail_add(uint32_t (&r)[32], const float4 (&v)[8]) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    r[4 * j] = __float_as_uint(__uint_as_float(r[4 * j]) + v[j].x);
+    r[4 * j + 1] = __float_as_uint(__uint_as_float(r[4 * j + 1]) + v[j].y);
+    r[4 * j + 2] = __float_as_uint(__uint_as_float(r[4 * j + 2]) + v[j].z);
+    r[4 * j + 3] = __float_as_uint(__uint_as_float(r[4 * j + 3]) + v[j].w);
+  }
+}
+__device__ __forceinline__ void tail_signal(const TcParams& p, long long slot, int lane) {
+  __threadfence();
+  __syncwarp();
+  if (lane == 0) asm volatile("st.release.gpu.global.s32 [%0], 1;" ::"l"(p.tail_flags + slot) : "memory");
+}
+// bounded like an mbarrier wait
+__device__ __forceinline__ bool tail_wait(const TcParams& p, long long slot, volatile int* abort_flag) {
+  const long long t0 = now_ns();
+  while (true) {
+    int v;
+    asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(p.tail_flags + slot) : "memory");
+    if (v != 0) return true;
+    if (*abort_flag) return false;
+    if (now_ns() - t0 > MBAR_WAIT_NS) {
+      atomicCAS(&g_device_status, 0, IPC_ERR_TIMEOUT);
+      *abort_flag = 1;
+      return false;
+    }
+  }
 }
 
 template <typename T>
@@ -237,12 +304,13 @@ __device__ __forceinline__ uint4 pack_scaled(const uint32_t* acc8, float scale) 
 // BK: cast(f'(x) acc) for 8 columns whose states are the lower or upper 8 codes of `codes`, f' in its MUFU form
 template <typename T, int ACT>
 __device__ __forceinline__ uint4 epi_vec_bk(const uint4& codes, int half, float step, const uint32_t* acc8) {
-  const uint32_t c2[2] = {half ? codes.z : codes.x, half ? codes.w : codes.y};
-  const signed char* c = reinterpret_cast<const signed char*>(c2);
+  float c[8];
+  mx8_floats(half ? codes.z : codes.x, c);
+  mx8_floats(half ? codes.w : codes.y, c + 4);
   uint4 o;
   T* oh = reinterpret_cast<T*>(&o);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) oh[j] = St<T>::st(act_df_hw<ACT>((float)c[j] * step) * __uint_as_float(acc8[j]));
+  for (int j = 0; j < 8; ++j) oh[j] = St<T>::st(act_df_hw<ACT>(c[j] * step) * __uint_as_float(acc8[j]));
   return o;
 }
 // ... and the coalesced pass stores it and cast(f(x)) of the stored x (the A_out of the forward sweep)
@@ -297,6 +365,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
   constexpr uint32_t B_BYTES = BNL * TC_BK * 2;
   constexpr uint32_t STAGE_BYTES = A_BYTES + B_BYTES;
   constexpr uint32_t TMEM_COLS = 2 * BN;  // two accumulators
+  constexpr bool TAIL = MODE == MODE_W || MODE == MODE_G;  // (and WD, in its own epilogue)
   // instruction descriptor: fp32 accumulate, A/B fp16 or bf16, majors, N, M = 128 (256 for a pair)
   constexpr uint32_t FMT = std::is_same<T, __half>::value ? 0u : 1u;
   constexpr uint32_t IDESC = (1u << 4) | (FMT << 7) | (FMT << 10) | ((A_MN ? 1u : 0u) << 15) |
@@ -374,8 +443,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
       int g, m0, n0, sp;
       tile_coords(p, t, BN, g, m0, n0, sp, TM, rank);  // m0: this CTA's first row
       const int nb = n0 + BNL * rank;                  // this CTA's first B column
-      const int kb_end = min(nk, (sp + 1) * p.kps);
-      for (int kb = sp * p.kps; kb < kb_end; ++kb) {
+      int kb_begin, kb_end;
+      k_range(p, t, sp, nk, kb_begin, kb_end);
+      for (int kb = kb_begin; kb < kb_end; ++kb) {
         ok = mbar_wait(empty0 + 8 * s, phase ^ 1, abort_flag);
         __syncwarp();
         if (!ok) break;
@@ -433,8 +503,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
       if (!ok) break;
       tc_fence_after();
       const uint32_t d_tmem = tmem_base + acc * BN;
-      const int sp = t % p.splits;
-      const int kb_begin = sp * p.kps, kb_end = min(nk, (sp + 1) * p.kps);
+      int kb_begin, kb_end;
+      k_range(p, t, t % p.splits, nk, kb_begin, kb_end);
       for (int kb = kb_begin; kb < kb_end; ++kb) {
         ok = mbar_wait(full0 + 8 * s, phase, abort_flag);
         __syncwarp();
@@ -487,8 +557,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         // with coalesced 16-byte stores (a warp instruction covers 4 rows x 128 bytes).
         // F has no input block: the row threads write cast(acc) into the buffer, and the coalesced
         // pass stores it and, when A_out is given, cast(f(x)) beside it.  G: the same with scale acc.
-        // BK: a row thread reads the 8-bit states of its own row (HC bytes, whole sectors) into registers
-        // before the accumulator is ready and writes cast(f'(x) acc).
+        // BK: the 8-bit states are read with coalesced loads a tile ahead and passed through the buffer to the
+        // row threads, which write cast(f'(x) acc).
         constexpr bool HAS_IN = (MODE == MODE_P || MODE == MODE_W);
         constexpr int NCH = HC / 64;        // 64-column chunks per warp and tile
         constexpr int NPRE = 8 * NCH;       // prefetched 16-byte vectors per thread
@@ -513,28 +583,71 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
           }
         };
         if (HAS_IN && unit0 < p.tiles) prefetch(unit0);
+        constexpr int VPR = HC / 16;                          // BK: 16-byte vectors of codes in a row of the warp's block
+        uint4 ckv[MODE == MODE_BK ? VPR : 1];                 // a tile ahead: rows of the block across lanes; then the
+        uint32_t ckb[MODE == MODE_BK ? HC / 32 : 1];          // thread's own row, and its scale bytes
+        auto cswz = [&](int row) { return VPR == 8 ? (row & 7) : ((row >> 1) & 3); };
+        auto fetch_states = [&](int t) {
+          int g, m0, n0, sp;
+          tile_coords(p, t, BN, g, m0, n0, sp, TM, rank);
+          const int r0 = m0 + 32 * q, nw = n0 + c_lo;
+#pragma unroll
+          for (int i = 0; i < (MODE == MODE_BK ? VPR : 0); ++i) {
+            const int r = r0 + (32 * i + lane) / VPR, n = nw + 16 * (lane % VPR);
+            ckv[i] = (r < p.Mg && n < p.Ng) ? __ldg(reinterpret_cast<const uint4*>(p.ck + (long long)r * p.ld_ck + n))
+                                            : make_uint4(0, 0, 0, 0);
+          }
+#pragma unroll
+          for (int i = 0; i < (MODE == MODE_BK ? HC / 32 : 0); ++i)
+            ckb[i] = (r0 + lane < p.Mg && nw + 32 * i < p.Ng)
+                         ? p.cks[(long long)((nw + 32 * i) / 32) * p.Mg + r0 + lane] : 0u;
+        };
+        if (MODE == MODE_BK && unit0 < p.tiles) fetch_states(unit0);
         for (int t = unit0; t < p.tiles; t += units) {
           int g, m0, n0, sp;
           tile_coords(p, t, BN, g, m0, n0, sp, TM, rank);
           const int r0 = m0 + 32 * q, nw = n0 + c_lo;
-          uint4 ckv[MODE == MODE_BK ? HC / 16 : 1];
-          uint32_t ckb[MODE == MODE_BK ? HC / 32 : 1];
-          if constexpr (MODE == MODE_BK) {
-            const bool in = r0 + lane < p.Mg;
-            const signed char* row = p.ck + (long long)(r0 + lane) * p.ld_ck;
+          bool ok = mbar_wait(tfull0 + 8 * acc, aphase, abort_flag);
+          uint4 st[MODE == MODE_BK ? VPR : 1];
+          uint32_t sb[MODE == MODE_BK ? HC / 32 : 1];
+          if constexpr (MODE == MODE_BK) {  // the states of this thread's row through the buffer; then the next tile's
 #pragma unroll
-            for (int i = 0; i < HC / 16; ++i)
-              ckv[i] = (in && nw + 16 * i < p.Ng) ? __ldg(reinterpret_cast<const uint4*>(row + nw + 16 * i))
-                                                  : make_uint4(0, 0, 0, 0);
+            for (int i = 0; i < VPR; ++i) {
+              const int r = (32 * i + lane) / VPR;
+              sts128(xb + r * HC + (((lane % VPR) ^ cswz(r)) << 4), ckv[i]);
+            }
+            __syncwarp();
 #pragma unroll
-            for (int i = 0; i < HC / 32; ++i)
-              ckb[i] = (in && nw + 32 * i < p.Ng) ? p.cks[(long long)((nw + 32 * i) / 32) * p.Mg + r0 + lane] : 0u;
+            for (int i = 0; i < VPR; ++i) st[i] = lds128(xb + lane * HC + ((i ^ cswz(lane)) << 4));
+#pragma unroll
+            for (int i = 0; i < HC / 32; ++i) sb[i] = ckb[i];
+            __syncwarp();
+            if (t + units < p.tiles) fetch_states(t + units);
           }
-          const bool ok = mbar_wait(tfull0 + 8 * acc, aphase, abort_flag);
-          __syncwarp();
+          const bool halved = TAIL && t >= p.tail_from, owner = halved && ((t - p.tail_from) & 1) == 0;
+          const long long slot = halved ? tail_slot(p, t, NCTA, rank, warp - 2) : 0;
+          if (owner && ok) ok = tail_wait(p, slot, abort_flag);
+          ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           tc_fence_after();
           const uint32_t trow = tmem_base + ((uint32_t)(32 * q) << 16) + acc * BN;
+          float4 other[TAIL ? 8 : 1];  // the second half's accumulators, a chunk ahead
+          if constexpr (TAIL)
+            if (owner) tail_get<HC / 32>(p, slot, 0, lane, other);
+          if (halved && !owner) {  // the second half: to the workspace
+#pragma unroll 1
+            for (int c = 0; c < HC / 32; ++c) {
+              uint32_t raw[32];
+              tmem_ld32(trow + c_lo + 32 * c, raw);
+              tail_put<HC / 32>(p, slot, c, lane, raw);
+            }
+            tc_fence_before();
+            release_acc(tempty0 + 8 * acc);
+            tail_signal(p, slot, lane);
+            if (HAS_IN && t + units < p.tiles) prefetch(t + units);
+            if (++acc == 2) { acc = 0; aphase ^= 1; }
+            continue;
+          }
 #pragma unroll
           for (int cc = 0; cc < NCH; ++cc) {
             if constexpr (HAS_IN) {
@@ -551,13 +664,19 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
             for (int hf = 0; hf < 2; ++hf) {
               uint32_t raw[32];
               tmem_ld32(trow + c_lo + 64 * cc + 32 * hf, raw);
+              if constexpr (TAIL) {
+                if (owner) {
+                  tail_add(raw, other);
+                  if (2 * cc + hf + 1 < HC / 32) tail_get<HC / 32>(p, slot, 2 * cc + hf + 1, lane, other);
+                }
+              }
 #pragma unroll
               for (int j = 0; j < 4; ++j) {
                 const uint32_t a = xb + lane * 128 + (((4 * hf + j) ^ (lane & 7)) << 4);
                 if constexpr (HAS_IN)
                   sts128(a, epi_vec_pw<T, MODE>(lds128(a), raw + 8 * j, p.scale));
                 else if constexpr (MODE == MODE_BK)
-                  sts128(a, epi_vec_bk<T, ACT>(ckv[4 * cc + 2 * hf + j / 2], j & 1, mx_scale(ckb[2 * cc + hf]), raw + 8 * j));
+                  sts128(a, epi_vec_bk<T, ACT>(st[4 * cc + 2 * hf + j / 2], j & 1, mx_scale(sb[2 * cc + hf]), raw + 8 * j));
                 else if constexpr (MODE == MODE_G)
                   sts128(a, pack_scaled<T>(raw + 8 * j, p.scale));
                 else
@@ -713,15 +832,37 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
           int g, m0, n0, sp;
           tile_coords(p, t, BN, g, m0, n0, sp, TM, rank);
           const int r0 = m0 + 32 * q, nw = n0 + c_lo;
-          const bool ok = mbar_wait(tfull0 + 8 * acc, aphase, abort_flag);
-          __syncwarp();
+          bool ok = mbar_wait(tfull0 + 8 * acc, aphase, abort_flag);
+          const bool halved = t >= p.tail_from, owner = halved && ((t - p.tail_from) & 1) == 0;
+          const long long slot = halved ? tail_slot(p, t, NCTA, rank, warp - 2) : 0;
+          if (owner && ok) ok = tail_wait(p, slot, abort_flag);
+          ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           tc_fence_after();
           const uint32_t trow = tmem_base + ((uint32_t)(32 * q) << 16) + acc * BN;
+          float4 other[8];
+          if (owner) tail_get<HC / 32>(p, slot, 0, lane, other);
+          if (halved && !owner) {
+#pragma unroll 1
+            for (int c = 0; c < HC / 32; ++c) {
+              uint32_t raw[32];
+              tmem_ld32(trow + c_lo + 32 * c, raw);
+              tail_put<HC / 32>(p, slot, c, lane, raw);
+            }
+            tc_fence_before();
+            release_acc(tempty0 + 8 * acc);
+            tail_signal(p, slot, lane);
+            if (++acc == 2) { acc = 0; aphase ^= 1; }
+            continue;
+          }
 #pragma unroll 1
           for (int c = 0; c < HC / 32; ++c) {
             uint32_t raw[32];
             tmem_ld32(trow + c_lo + 32 * c, raw);
+            if (owner) {
+              tail_add(raw, other);
+              if (c + 1 < HC / 32) tail_get<HC / 32>(p, slot, c + 1, lane, other);
+            }
             if (c == HC / 32 - 1) {  // every accumulator column read: release it to the MMA warp
               tc_fence_before();
               release_acc(tempty0 + 8 * acc);
@@ -936,6 +1077,14 @@ __global__ void ws_reduce_ragged_kernel(const float* __restrict__ ws, int splits
   }
 }
 
+// Whether the tiles of the last round are halved along the reduction: where the halves fit into the idle CTAs (pairs) and
+// half a tile is at least 32 K blocks (about 11 us; the exchange costs 3).
+bool tail_halves(long long tiles, long long units, int nk, long long tile_bytes, size_t ws_bytes) {
+  const long long rest = tiles % units;
+  return rest > 0 && 2 * rest <= units && nk >= 64 && ws_bytes >= TAIL_FLAG_BYTES &&
+         rest * tile_bytes <= (long long)(ws_bytes - TAIL_FLAG_BYTES);
+}
+
 template <typename T, int ACT, int MODE, int BN, int PAIR>
 int launch_tc_t(const GemmArgs& a, int dtype, cudaStream_t s, float* ws, size_t ws_bytes, const TcTune* tune) {
   constexpr bool A_MN = (MODE == MODE_I || MODE == MODE_BK);
@@ -1010,6 +1159,16 @@ int launch_tc_t(const GemmArgs& a, int dtype, cudaStream_t s, float* ws, size_t 
     }
   }
   p.tiles *= p.splits;
+  p.tail_from = INT_MAX;
+  if ((MODE == MODE_W || MODE == MODE_WD || MODE == MODE_G) && a.tail_ws != nullptr && p.splits == 1 && a.groups == 1 &&
+      !(MODE == MODE_WD && a.accumulate && !a.ragged) && tail_halves(p.tiles, units, nk, (long long)TM * BN * 4, a.tail_bytes)) {
+    const int rest = p.tiles % units;
+    p.tail_from = p.tiles - rest;
+    p.tail_kps = (nk + 1) / 2;
+    p.tail_flags = static_cast<int*>(a.tail_ws);
+    p.tail_ws = reinterpret_cast<float*>(static_cast<char*>(a.tail_ws) + TAIL_FLAG_BYTES);
+    p.tiles += rest;
+  }
   // staged epilogue (no split-K): P / W through the transpose buffer, I through TMA with three maps
   // (E, X, A_out) of 32-row x 16-column boxes, 32-byte swizzle
   constexpr bool EPI_STAGED =
@@ -1184,6 +1343,18 @@ int launch_tc(const GemmArgs& a, int mode, int act, int dtype, cudaStream_t s, f
       const long long c2 = ((tp * s2 + u2 - 1) / u2) * (256 + 416) * 9 / s2;
       pair = c2 < c1;
     }
+  }
+  if (a.tail_ws != nullptr && !splitk) {
+    // the same estimate with the last round halved where that pays
+    const int nk = (a.Kg + TC_BK - 1) / TC_BK;
+    auto half_rounds = [&](long long tiles, long long units, long long tile_bytes) {
+      return tiles / units * 2 + (tiles % units ? (tail_halves(tiles, units, nk, tile_bytes, a.tail_bytes) ? 1 : 2) : 0);
+    };
+    const long long c256 = half_rounds(t256, cap, 128 * 256 * 4) * (256 + 416) * 10;
+    const long long c128 = half_rounds(t128, cap, 128 * 128 * 4) * (128 + 416) * 10;
+    const long long cp = half_rounds(tp, std::max(1LL, cap / 2), 256 * 256 * 4) * (256 + 416) * 9;
+    wide = a.Ng >= 256 && c256 <= c128;
+    pair = a.Ng >= 256 && cap >= 2 && cp < std::min(c256, c128);
   }
   if (tune != nullptr && tune->pair == 1) pair = false;
   if (tune != nullptr && tune->pair == 2) pair = a.Ng >= 256;

@@ -444,3 +444,37 @@ def test_products_on_views_that_start_between_vectors():
         up = off(up) if shift else up
         mx.build_error_backward_checkpoint(M, K, B, "tanh", "bfloat16")(ww, ee, c, s, up)
         _within(up, rb, tol * (1 + U[dt]) + (U[dt] + 2.0 ** -23) * rb.abs() + TINY[dt])
+
+
+@pytest.mark.parametrize("M,K,B", [(1024, 1024, 2048), (2304, 2304, 4096), (1000, 1021, 4500), (512, 640, 4096),
+                                   (2048, 4096, 4160)])
+def test_delta_with_a_halved_last_round(M, K, B):
+    """Shapes whose last round of tiles fills half the GPU or less: its tiles are halved along the batch.  Checked on samples of the rows against 64 bits, and bit for bit against another run."""
+    from lich_b200 import _native as N
+    mx = _mx()
+    dt = torch.bfloat16
+    e, x = _rand((M, B), 1, 0.3, dt), _rand((K, B), 2, 1.5, dt)
+    c, s = mx.empty_checkpoint(K, B, device=DEV)
+    mx.build_checkpoint(K, B, "bfloat16")(x.to(DEV), c, s)
+    xhat = X.load8(c.cpu(), s.cpu(), B)
+    a = torch.tanh(xhat)
+    rows = torch.arange(0, M, max(1, M // 61))
+    er, ed = e[rows].double(), e.to(DEV)
+    ref, S = er @ a.t(), er.abs() @ a.abs().t()
+    err = (er.abs() @ (MUFU * a.abs() + U[dt] * a.abs() + TINY[dt]).t()) * (1 + 2.0 ** -8) + S * B * 2.0 ** -23
+    for name in ("float32", "bfloat16"):
+        k = mx.build_weight_delta_checkpoint(M, K, B, "tanh", "bfloat16", 1.0, name)
+        outs = []
+        for _ in range(3):
+            out = torch.full((M, K), 7.0, device=DEV, dtype=getattr(torch, name))
+            k(out, ed, c, s)
+            outs.append(out)
+        u = U[out.dtype] + 2.0 ** -23
+        _within(outs[0][rows.to(DEV)], ref, err * (1 + u) + u * ref.abs())
+        assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
+    w0 = _rand((M, K), 3, 0.05, dt)
+    w = w0.to(DEV)
+    mx.build_weight_update_checkpoint(M, K, B, "tanh", "bfloat16", 0.01)(w, ed, c, s)
+    want = w0[rows].double() + 0.01 * ref
+    _within(w[rows.to(DEV)], want, (0.01 * err) * (1 + U[dt]) + (U[dt] + 2.0 ** -22) * (want.abs() + 0.01 * ref.abs()))
+    assert N.device_status() == 0
