@@ -312,6 +312,18 @@ __global__ void __launch_bounds__(THREADS) mx4_rows_kernel(const T* __restrict__
 // shared memory, so that a sample's 128 bytes leave together.
 // PAIR: rows start on boundaries of two elements and a lane takes two neighbouring samples; otherwise samples lane, lane + 32.
 constexpr int TUR = 64;
+// relu of two 16-bit numbers (like act_f, 0 for a NaN)
+template <typename T>
+__device__ __forceinline__ uint32_t relu2(uint32_t w) {
+  if constexpr (std::is_same<T, __half>::value) {
+    const __half2 r = __hmax2(*reinterpret_cast<__half2*>(&w), __float2half2_rn(0.f));
+    return *reinterpret_cast<const uint32_t*>(&r);
+  } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    const __nv_bfloat162 r = __hmax2(*reinterpret_cast<__nv_bfloat162*>(&w), __float2bfloat162_rn(0.f));
+    return *reinterpret_cast<const uint32_t*>(&r);
+  }
+  return w;
+}
 template <typename T, bool PAIR>
 struct alignas(2 * sizeof(T)) Two {  // an element of each of a lane's two samples
   T v[2];
@@ -355,17 +367,36 @@ __global__ void __launch_bounds__(THREADS) mx4_turned_kernel(const T* __restrict
     for (int i = 0; i < MX_BLOCK; ++i)
       v[i] = load_two<T, PAIR>(src + (long long)i * R, lane, in[0] && kb + i < K, in[1] && kb + i < K);
   }
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    float f[MX_BLOCK];
+  // 16-bit types under an f that only clears: both samples' largest magnitudes at once, as stored
+  constexpr bool PACKED = sizeof(T) == 2 && (ACT == IPC_ACT_RELU || ACT == IPC_ACT_IDENTITY);
+  uint32_t top[2] = {0, 0};
+  if constexpr (PACKED) {
     uint32_t m = 0;
 #pragma unroll
     for (int i = 0; i < MX_BLOCK; ++i) {
-      f[i] = act_full<ACT>(St<T>::ld(v[i].v[h]));
-      if (ACT == IPC_ACT_SIGMOID && !(in[h] && kb + i < K)) f[i] = 0.f;  // (the other f are 0 at 0)
-      m = max(m, abs_bits(f[i]));
+      uint32_t& w = *reinterpret_cast<uint32_t*>(v[i].v);
+      if constexpr (ACT == IPC_ACT_RELU) w = relu2<T>(w);
+      m = __vmaxu2(m, w & 0x7fff7fffu);
     }
-    const uint32_t byte = mx4_scale_byte(m);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint16_t b = (uint16_t)(h ? m >> 16 : m & 0xffffu);
+      top[h] = __float_as_uint(St<T>::ld(*reinterpret_cast<const T*>(&b)));
+    }
+  }
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    float f[MX_BLOCK];
+#pragma unroll
+    for (int i = 0; i < MX_BLOCK; ++i) {
+      f[i] = St<T>::ld(v[i].v[h]);
+      if constexpr (!PACKED) {
+        f[i] = act_full<ACT>(f[i]);
+        if (ACT == IPC_ACT_SIGMOID && !(in[h] && kb + i < K)) f[i] = 0.f;  // (the other f are 0 at 0)
+        top[h] = max(top[h], abs_bits(f[i]));
+      }
+    }
+    const uint32_t byte = mx4_scale_byte(top[h]);
     const float inv = mx_inv_scale(byte);
     uint4 o;
     uint32_t* w = reinterpret_cast<uint32_t*>(&o);
@@ -373,8 +404,8 @@ __global__ void __launch_bounds__(THREADS) mx4_turned_kernel(const T* __restrict
     for (int q = 0; q < 4; ++q) {
       float a[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) a[j] = byte == MX_NAN_BYTE ? 0.f : f[8 * q + j] * inv;
-      w[q] = mx4_pack8(a);
+      for (int j = 0; j < 8; ++j) a[j] = f[8 * q + j] * inv;
+      w[q] = byte == MX_NAN_BYTE ? 0u : mx4_pack8(a);
     }
     *reinterpret_cast<uint4*>(&s_code[rl[h]][16 * warp]) = o;
     s_scale[rl[h]][warp] = (unsigned char)byte;

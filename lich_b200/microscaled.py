@@ -35,6 +35,8 @@ from .tilelang_kernels import KernelConfig, _algo
 N.load()
 
 BLOCK = 32
+# what torch.cuda.current_device() and current_stream().cuda_stream come down to, at a tenth of their cost
+_current_device, _current_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
 
 def checkpoint_shapes(D: int, B: int) -> tuple[tuple[int, int], tuple[int, int]]:
@@ -69,8 +71,9 @@ class _MxOp:
         self._fn = getattr(N.load(), entry)
         self._ws: dict = {}
 
-    def _stream(self, tensors) -> int:
-        """The current stream of the tensors' device, after checking the tensors against ``spec``."""
+    def _stream(self, tensors):
+        """The current stream of the tensors' device, after checking the tensors against ``spec``; None when that device is
+        not the current one (``_elsewhere``)."""
         try:
             dev = tensors[0].get_device()
             for t, (shape, dtype) in zip(tensors, self.spec):
@@ -78,10 +81,14 @@ class _MxOp:
                     break
             else:
                 if dev >= 0:
-                    return torch._C._cuda_getCurrentRawStream(dev)
+                    return _current_stream(dev) if dev == _current_device() else None
         except AttributeError:
             pass
         raise ValueError(self._refusal(tensors))
+
+    def _elsewhere(self, *tensors, **kw) -> None:
+        with torch.cuda.device(tensors[0].device):
+            self(*tensors, **kw)
 
     def _refusal(self, tensors) -> str:
         for i, (t, (shape, dtype)) in enumerate(zip(tensors, self.spec)):
@@ -108,17 +115,6 @@ class _MxOp:
             ws = self._ws[dev, stream] = (None if buf is None else buf.data_ptr(), int(n.value), buf)
         return ws[:2]
 
-    def _launch(self, tensors, *args) -> None:
-        """The C entry on the tensors' device and its current stream; its error as an exception."""
-        dev = tensors[0].get_device()
-        if dev == torch._C._cuda_getDevice():
-            rc = self._fn(*args)
-        else:
-            with torch.cuda.device(dev):
-                rc = self._fn(*args)
-        if rc:
-            N.check(rc)
-
     def get_kernel_source(self) -> str:
         return f"lich_b200 {self.kind} {self.spec} (prebuilt sm_100a kernel, include/ipc_b200.h)"
 
@@ -132,9 +128,12 @@ class CheckpointKernel(_MxOp):
         self.D, self.B, self.dt = int(D), int(B), N.dtype_code(dtype)
 
     def __call__(self, x, codes, scales):
-        t = (x, codes, scales)
-        s = self._stream(t)
-        self._launch(t, x.data_ptr(), codes.data_ptr(), scales.data_ptr(), self.D, self.B, self.dt, s)
+        s = self._stream((x, codes, scales))
+        if s is None:
+            return self._elsewhere(x, codes, scales)
+        rc = self._fn(x.data_ptr(), codes.data_ptr(), scales.data_ptr(), self.D, self.B, self.dt, s)
+        if rc:
+            N.check(rc)
 
 
 class CheckpointRestoreKernel(_MxOp):
@@ -146,9 +145,12 @@ class CheckpointRestoreKernel(_MxOp):
         self.D, self.B, self.act, self.dt = int(D), int(B), N.act_code(activation), N.dtype_code(dtype)
 
     def __call__(self, codes, scales, out):
-        t = (codes, scales, out)
-        s = self._stream(t)
-        self._launch(t, codes.data_ptr(), scales.data_ptr(), out.data_ptr(), self.D, self.B, self.act, self.dt, s)
+        s = self._stream((codes, scales, out))
+        if s is None:
+            return self._elsewhere(codes, scales, out)
+        rc = self._fn(codes.data_ptr(), scales.data_ptr(), out.data_ptr(), self.D, self.B, self.act, self.dt, s)
+        if rc:
+            N.check(rc)
 
 
 class CheckpointWeightKernel(_MxOp):
@@ -165,13 +167,16 @@ class CheckpointWeightKernel(_MxOp):
         return N.load().ipc_mx8_weight_ws_bytes(self.mode, self.M, self.K, self.B, self.dt, self.algo, n)
 
     def __call__(self, out, e, codes, scales, *, accumulate: bool = False):
-        t = (out, e, codes, scales)
-        s = self._stream(t)
+        s = self._stream((out, e, codes, scales))
         if accumulate and self.mode != N.MODE_WDELTA:
             raise ValueError(f"{self.kind}: only a weight delta in float32 accumulates")
+        if s is None:
+            return self._elsewhere(out, e, codes, scales, accumulate=accumulate)
         ws, n = self._workspace(out.get_device(), s)
-        self._launch(t, self.mode, out.data_ptr(), e.data_ptr(), codes.data_ptr(), scales.data_ptr(), self.M, self.K,
-                     self.B, self.alpha, N.FLAG_ACCUMULATE if accumulate else 0, self.act, self.dt, self.algo, ws, n, s)
+        rc = self._fn(self.mode, out.data_ptr(), e.data_ptr(), codes.data_ptr(), scales.data_ptr(), self.M, self.K, self.B,
+                      self.alpha, N.FLAG_ACCUMULATE if accumulate else 0, self.act, self.dt, self.algo, ws, n, s)
+        if rc:
+            N.check(rc)
 
 
 class CheckpointBackwardKernel(_MxOp):
@@ -189,11 +194,14 @@ class CheckpointBackwardKernel(_MxOp):
         return N.load().ipc_mx8_backward_ws_bytes(self.M, self.K, self.B, self.dt, self.algo, n)
 
     def __call__(self, w, e, codes, scales, e_up):
-        t = (w, e, codes, scales, e_up)
-        s = self._stream(t)
+        s = self._stream((w, e, codes, scales, e_up))
+        if s is None:
+            return self._elsewhere(w, e, codes, scales, e_up)
         ws, n = self._workspace(w.get_device(), s)
-        self._launch(t, e_up.data_ptr(), w.data_ptr(), e.data_ptr(), codes.data_ptr(), scales.data_ptr(), self.M, self.K,
-                     self.B, self.act, self.dt, self.algo, ws, n, s)
+        rc = self._fn(e_up.data_ptr(), w.data_ptr(), e.data_ptr(), codes.data_ptr(), scales.data_ptr(), self.M, self.K,
+                      self.B, self.act, self.dt, self.algo, ws, n, s)
+        if rc:
+            N.check(rc)
 
 
 class Mxfp4QuantizeKernel(_MxOp):
@@ -207,10 +215,12 @@ class Mxfp4QuantizeKernel(_MxOp):
         self.act, self.dt = N.act_code(activation), N.dtype_code(dtype)
 
     def __call__(self, x, codes, scales):
-        t = (x, codes, scales)
-        s = self._stream(t)
-        self._launch(t, x.data_ptr(), codes.data_ptr(), scales.data_ptr(), self.R, self.K, self.turned, self.act, self.dt,
-                     s)
+        s = self._stream((x, codes, scales))
+        if s is None:
+            return self._elsewhere(x, codes, scales)
+        rc = self._fn(x.data_ptr(), codes.data_ptr(), scales.data_ptr(), self.R, self.K, self.turned, self.act, self.dt, s)
+        if rc:
+            N.check(rc)
 
 
 class Mxfp4RestoreKernel(_MxOp):
@@ -222,9 +232,12 @@ class Mxfp4RestoreKernel(_MxOp):
         self.R, self.K, self.dt = int(R), int(K), N.dtype_code(dtype)
 
     def __call__(self, codes, scales, out):
-        t = (codes, scales, out)
-        s = self._stream(t)
-        self._launch(t, codes.data_ptr(), scales.data_ptr(), out.data_ptr(), self.R, self.K, self.dt, s)
+        s = self._stream((codes, scales, out))
+        if s is None:
+            return self._elsewhere(codes, scales, out)
+        rc = self._fn(codes.data_ptr(), scales.data_ptr(), out.data_ptr(), self.R, self.K, self.dt, s)
+        if rc:
+            N.check(rc)
 
 
 class Mxfp4ForwardKernel(_MxOp):
@@ -238,10 +251,13 @@ class Mxfp4ForwardKernel(_MxOp):
         self.M, self.K, self.B, self.dt = int(M), int(K), int(B), N.dtype_code(dtype)
 
     def __call__(self, w, w_scales, a, a_scales, out):
-        t = (w, w_scales, a, a_scales, out)
-        s = self._stream(t)
-        self._launch(t, w.data_ptr(), w_scales.data_ptr(), a.data_ptr(), a_scales.data_ptr(), out.data_ptr(), self.M,
-                     self.K, self.B, self.dt, s)
+        s = self._stream((w, w_scales, a, a_scales, out))
+        if s is None:
+            return self._elsewhere(w, w_scales, a, a_scales, out)
+        rc = self._fn(w.data_ptr(), w_scales.data_ptr(), a.data_ptr(), a_scales.data_ptr(), out.data_ptr(), self.M, self.K,
+                      self.B, self.dt, s)
+        if rc:
+            N.check(rc)
 
 
 def _validate(*sizes, activation="identity", dtype):
