@@ -447,16 +447,25 @@ int ipc_mx8_restore(const signed char* codes, const unsigned char* scales, void*
 
 // Products with a checkpoint.  Large ones run on the tcgen05 GEMMs, whose operands TMA loads: rows on 16-byte
 // boundaries.  So f(x^) is restored, and an operand with a row stride that is no multiple of 8 copied, into rows of the
-// workspace that are.  The rest (16-bit storage) is one launch of mx8_small_kernel, which needs none.
+// workspace that are.  The rest (16-bit storage) is one launch of mx8_small_kernel, and a few samples are one of
+// ipc_mx8_few.cu: they need none.
+// Few samples.  Measured (GPU time, us, fp32 FMAs against the kernels above): delta 4096 x 4096 x 1 11 / 19, x 8 17 / 18,
+// 1024 x 1024 x 1 3.5 / 6.3, 2816 x 3035 x 15 15 / 26, 300 x 301 x 5 4.4 / 3.8; backward 4096 x 4096 x 4 19 / 44, 3643 x 639 x 4 8.4 / 17, x 8 39 / 24.
+// fp32 storage has no other kernel for them than the generic one.
+static bool mx8_few(int mode, int M, int K, int B, int dtype, int algo) {
+  if (algo != IPC_ALGO_AUTO || B < 1) return false;
+  if (mode == MODE_BK) return B <= 4;
+  return dtype == IPC_DT_F32 ? B <= 16 : (B <= 8 || (B <= 16 && K % 8)) && (double)M * K >= 4e5;
+}
 static bool mx8_large(int mode, int M, int K, int B, int dtype, int algo) {
   if (dtype == IPC_DT_F32 || (algo != IPC_ALGO_AUTO && algo != IPC_ALGO_TCGEN05)) return false;
   if (M < 1 || K < 1 || B < 1) return false;
   if (algo == IPC_ALGO_TCGEN05) return true;
-  // Measured (GPU time, us, one launch against tcgen05): delta 512^3 7.9 / 8.7, 512 x 512 x 1024 11.4 / 11.0, 1000 x 1021 x 333
-  // 15.8 / 11.3, 4096 x 4096 x 16 42 / 17 (outputs, not the sum, fill that one); backward 256 x 512 x 512 7.4 / 6.3, and with
+  // Measured (GPU time, us, one launch against tcgen05): delta 256 x 512 x 512 7.4 / 8.9, 512^3 9.8 / 8.8, 1000 x 1021 x 333
+  // 19.5 / 9.8, 4096 x 4096 x 64 56 / 17 (outputs, not the sum, fill that one); backward 256 x 512 x 512 7.4 / 6.3, and with
   // both operands copied 1000 x 1021 x 333 27 / 15.
   if (mode == MODE_BK) return (double)M * K * B >= (K % 8 || B % 8 ? 1.5e8 : 5e7);
-  return (double)M * K * (B < 64 ? 64 : B) >= 2.5e8;
+  return (double)M * K * (B < 64 ? 64 : B) >= 1.2e8;
 }
 static long long up8(long long n) { return (n + 7) / 8 * 8; }
 static size_t up256(size_t n) { return (n + 255) / 256 * 256; }
@@ -469,7 +478,7 @@ struct Mx8WeightWs {
 };
 static Mx8WeightWs mx8_weight_ws(int mode, int M, int K, int B, int dtype, int algo) {
   Mx8WeightWs w{};
-  if (M == 0 || K == 0 || B == 0) return w;
+  if (M == 0 || K == 0 || B == 0 || mx8_few(mode, M, K, B, dtype, algo)) return w;
   if (dtype == IPC_DT_F32) {
     w.ld = B;
     w.values = up256((size_t)K * B * 4);
@@ -478,7 +487,7 @@ static Mx8WeightWs mx8_weight_ws(int mode, int M, int K, int B, int dtype, int a
     w.values = up256((size_t)K * w.ld * 2);
     w.e = B % 8 ? up256((size_t)M * w.ld * 2) : 0;
     w.delta = (mode == MODE_W && K % 8) ? up256((size_t)M * K * 4) : 0;
-    w.partial = B > 4032 ? TAIL_FLAG_BYTES + IPC_SPLITK_WS_BYTES : 0;  // a last round of tiles halved along the batch
+    w.partial = B > 2496 ? TAIL_FLAG_BYTES + IPC_SPLITK_WS_BYTES : 0;  // a last round of tiles halved along the batch
   }
   w.total = w.values + w.e + w.delta + w.partial;
   return w;
@@ -517,6 +526,7 @@ int ipc_mx8_weight(int mode, void* out, const void* e, const signed char* codes,
   p.scale = scale;
   p.accumulate = (flags & IPC_FLAG_ACCUMULATE) != 0;
   p.ck = codes; p.cks = scales; p.ld_ck = mx8_ld(B);
+  if (mx8_few(mode, M, K, B, dtype, algo)) return launch_mx8_few(p, mode, act, dtype, s);
   if (dtype == IPC_DT_F32) {
     if (algo == IPC_ALGO_TCGEN05) return set_error(IPC_ERR_UNSUPPORTED, "tcgen05 path: 16-bit storage only");
     if (B > 0) rc = launch_mx8_restore(codes, scales, workspace, K, B, B, act, dtype, s);
@@ -558,7 +568,7 @@ int ipc_mx8_weight(int mode, void* out, const void* e, const signed char* codes,
 // workspace of the error product: W [M][lw] when K is no multiple of 8, E [M][le] when B is none
 static size_t mx8_backward_ws(int M, int K, int B, int dtype, int algo, size_t* w_bytes) {
   *w_bytes = 0;
-  if (!mx8_large(MODE_BK, M, K, B, dtype, algo)) return 0;
+  if (mx8_few(MODE_BK, M, K, B, dtype, algo) || !mx8_large(MODE_BK, M, K, B, dtype, algo)) return 0;
   *w_bytes = K % 8 ? up256((size_t)M * up8(K) * 2) : 0;
   return *w_bytes + (B % 8 ? up256((size_t)M * up8(B) * 2) : 0);
 }
@@ -593,6 +603,7 @@ int ipc_mx8_backward(void* e_up, const void* w, const void* e, const signed char
   p.out = e_up; p.gsOut = (long long)K * B;
   p.ck = codes; p.cks = scales; p.ld_ck = mx8_ld(B);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (mx8_few(MODE_BK, M, K, B, dtype, algo)) return launch_mx8_few(p, MODE_BK, act, dtype, s);
   if (dtype == IPC_DT_F32) {
     if (algo == IPC_ALGO_TCGEN05) return set_error(IPC_ERR_UNSUPPORTED, "tcgen05 path: 16-bit storage only");
     return launch_generic(p, MODE_BK, false, act, dtype, s);

@@ -102,6 +102,8 @@ int launch_mx8_restore_pack(const signed char* codes, const unsigned char* scale
                             int* zero = nullptr, int n_zero = 0);
 // one-launch product with a checkpoint (p.ck, p.cks), any shape, 16-bit storage: MODE_W, _WD, _G, _BK
 int launch_mx8_small(const GemmArgs& p, int mode, int act, int dtype, cudaStream_t s);
+// the same for a few samples (1 to 16; MODE_BK 1 to 4), any storage type, in fp32
+int launch_mx8_few(const GemmArgs& p, int mode, int act, int dtype, cudaStream_t s);
 int launch_mx4_quantize(const void* x, unsigned char* codes, unsigned char* scales, int R, int K, int turned, int act,
                         int dtype, cudaStream_t s);
 int launch_mx4_restore(const unsigned char* codes, const unsigned char* scales, void* out, int R, int K, int dtype,

@@ -329,13 +329,10 @@ __global__ void __launch_bounds__(F_THREADS, 1)
               const uint32_t a = xb + r * 64 + ((j ^ ((r >> 1) & 3)) << 4) + in;
               T v;
               if constexpr (sizeof(T) == 4) {
-                uint32_t w;
-                asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(a));
-                v = __uint_as_float(w);
+                v = __uint_as_float(lds32(a));
               } else {
-                uint16_t w;
-                asm volatile("ld.shared.u16 %0, [%1];" : "=h"(w) : "r"(a));
-                v = *reinterpret_cast<T*>(&w);
+                const uint16_t h = lds16(a);
+                v = *reinterpret_cast<const T*>(&h);
               }
               if (r0 + r < p.M && ne + col < p.N) out[(long long)(r0 + r) * p.ld_out + ne + col] = v;
             }

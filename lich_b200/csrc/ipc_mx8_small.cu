@@ -5,7 +5,9 @@
 //
 // These are bound by latency, so the aim is one launch, many CTAs and few dependent steps.  A CTA owns a 32 x 64 tile and
 // walks the reduction in steps of 64, the next step's operands in registers while mma.sync works on this one's in shared
-// memory.  The states are read as codes and f is applied on the way to shared memory: no restored copy, no second launch.
+// memory.  The states are read as codes and f is applied on the way to shared memory: no restored copy, no second launch,
+// and where f(x^) does not fit 16 bits, a second operand holds what the first rounds off: the MMAs are idle anyway, and
+// the sum then has fp32's accuracy (the rounding of f would be as large as the result's own).
 // A long reduction with few tiles is split over the CTAs of a cluster, whose partial sums meet in the first CTA's
 // shared memory and are added in rank order (deterministic).
 #include "ipc_epilogue.cuh"
@@ -96,16 +98,23 @@ __device__ __forceinline__ uint4 shifted(const Row8<VEC>& r, int left) {
   return make_uint4(o[0], o[1], o[2], o[3]);
 }
 
+// Whether f(x^) is kept in two parts: relu and identity give c * 2^s, which 16 bits hold.
+__host__ __device__ constexpr bool s_low(int act, int mode) {
+  return mode != MODE_BK && act != IPC_ACT_RELU && act != IPC_ACT_IDENTITY;
+}
+
 // VA, VB: the A operand (E; W for BK) and the E of BK load in whole vectors.
 template <typename T, int ACT, int MODE, bool VA, bool VB>
 __global__ void __launch_bounds__(STHREADS) mx8_small_kernel(const __grid_constant__ GemmArgs p, int k_per_split) {
   constexpr bool BKM = MODE == MODE_BK;
+  constexpr bool LOW = s_low(ACT, MODE);
   constexpr int LDA = BKM ? SM + 8 : SK + 8, LDB = BKM ? SN + 8 : SK + 8;  // shared rows, 16 bytes apart mod 128
   constexpr int ROWS_A = BKM ? SK : SM, ROWS_B = BKM ? SK : SN;
   extern __shared__ __align__(16) uint8_t s_smem[];
   T* sA = reinterpret_cast<T*>(s_smem);
   T* sB = sA + 2 * ROWS_A * LDA;
-  float* red = reinterpret_cast<float*>(sB + 2 * ROWS_B * LDB);
+  T* sL = sB + 2 * ROWS_B * LDB;  // what sB rounds off
+  float* red = reinterpret_cast<float*>(sL + (LOW ? 2 * ROWS_B * LDB : 0));
   const int m0 = blockIdx.y * SM, n0 = blockIdx.x * SN;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, wm = warp >> 1, wn = warp & 1;
   const int C = gridDim.z, rank = blockIdx.z;
@@ -173,13 +182,23 @@ __global__ void __launch_bounds__(STHREADS) mx8_small_kernel(const __grid_consta
         mx8_floats(rb[j].w, q + 12);
         const float sc = mx_scale(rs[j]);
         const bool in = n0 + r < p.Ng;
-        uint4 o[2];
+        uint4 o[2], l[2];
         T* h = reinterpret_cast<T*>(o);
+        T* lo = reinterpret_cast<T*>(l);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) h[e] = St<T>::st(in && k0 + c + e < k_hi ? act_f_hw<ACT>(q[e] * sc) : 0.f);
+        for (int e = 0; e < 16; ++e) {
+          const float f = in && k0 + c + e < k_hi ? act_f_hw<ACT>(q[e] * sc) : 0.f;
+          h[e] = St<T>::st(f);
+          if constexpr (LOW) lo[e] = St<T>::st(f - St<T>::ld(h[e]));
+        }
         uint4* dst = reinterpret_cast<uint4*>(b + r * LDB + c);
         dst[0] = o[0];
         dst[1] = o[1];
+        if constexpr (LOW) {
+          dst = reinterpret_cast<uint4*>(sL + buf * ROWS_B * LDB + r * LDB + c);
+          dst[0] = l[0];
+          dst[1] = l[1];
+        }
       }
     }
   };
@@ -192,6 +211,7 @@ __global__ void __launch_bounds__(STHREADS) mx8_small_kernel(const __grid_consta
     __syncthreads();  // (the other buffer's readers passed the barrier before this one)
     if (k0 + SK < k_hi) fetch(k0 + SK);
     const uint32_t a = saddr(sA + buf * ROWS_A * LDA), b = saddr(sB + buf * ROWS_B * LDB);
+    const uint32_t low = saddr(sL + (LOW ? buf * ROWS_B * LDB : 0));
 #pragma unroll
     for (int kk = 0; kk < SK; kk += 16) {
       uint32_t fa[4], fb[2][4];
@@ -215,6 +235,13 @@ __global__ void __launch_bounds__(STHREADS) mx8_small_kernel(const __grid_consta
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j) s_mma<T>(acc[j], fa, fb[j >> 1][2 * (j & 1)], fb[j >> 1][2 * (j & 1) + 1]);
+      if constexpr (LOW) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          ldsm4(fb[h], low + ((wn * 32 + 16 * h + (lane & 7) + ((lane & 16) >> 1)) * LDB + kk + (lane & 8)) * 2);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s_mma<T>(acc[j], fa, fb[j >> 1][2 * (j & 1)], fb[j >> 1][2 * (j & 1) + 1]);
+      }
     }
   }
 
@@ -267,7 +294,8 @@ int launch_small_t(const GemmArgs& p, cudaStream_t s) {
   if (C < 1) C = 1;
   const long long per = (steps + C - 1) / C;
   C = steps > 0 ? (int)((steps + per - 1) / per) : 1;
-  constexpr int TILES = 2 * (BKM ? SK * (SM + 8) + SK * (SN + 8) : (SM + SN) * (SK + 8)) * 2;
+  constexpr int TILES =
+      2 * (BKM ? SK * (SM + 8) + SK * (SN + 8) : (SM + SN + (s_low(ACT, MODE) ? SN : 0)) * (SK + 8)) * 2;
   const int smem = TILES + (C - 1) * SM * SN * 4;
   cudaError_t err = ensure_kernel_smem<mx8_small_kernel<T, ACT, MODE, VA, VB>>(TILES + (S_MAX_SPLIT - 1) * SM * SN * 4);
   if (err != cudaSuccess) return set_error(IPC_ERR_CUDA, "checkpoint product smem attribute: %s", cudaGetErrorString(err));

@@ -1078,10 +1078,10 @@ __global__ void ws_reduce_ragged_kernel(const float* __restrict__ ws, int splits
 }
 
 // Whether the tiles of the last round are halved along the reduction: where the halves fit into the idle CTAs (pairs) and
-// half a tile is at least 32 K blocks (about 11 us; the exchange costs 3).
+// half a tile is at least 20 K blocks (about 7 us; the exchange costs 3).
 bool tail_halves(long long tiles, long long units, int nk, long long tile_bytes, size_t ws_bytes) {
   const long long rest = tiles % units;
-  return rest > 0 && 2 * rest <= units && nk >= 64 && ws_bytes >= TAIL_FLAG_BYTES &&
+  return rest > 0 && 2 * rest <= units && nk >= 40 && ws_bytes >= TAIL_FLAG_BYTES &&
          rest * tile_bytes <= (long long)(ws_bytes - TAIL_FLAG_BYTES);
 }
 
