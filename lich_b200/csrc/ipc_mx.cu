@@ -2,9 +2,9 @@
 //
 // These kernels are bound by memory: every input element is read once, every code and scale byte written once.  A CTA
 // owns a tile of 32 rows x 256 columns, so that the scale bytes of a tile, which lie across the rows in both layouts,
-// leave as whole sectors.  A thread moves one 16-byte vector of the 16- or 32-bit side, so that a warp instruction covers
-// whole sectors (with two vectors a thread the stores of a restore reach L2 as half sectors: 22 us against 17 us for 8-bit
-// codes at 4096 x 8192 in bf16).  Rows that do not start on 16-byte boundaries take a lane per element.
+// leave as whole sectors.  A thread that restores writes one 16-byte vector at a time, so that a warp instruction covers
+// whole sectors (with two vectors a thread the stores reach L2 as half sectors: 22 us against 17 us for 8-bit codes at
+// 4096 x 8192 in bf16).  Rows that do not start on 16-byte boundaries take a lane per element.
 #include "ipc_mx.cuh"
 
 namespace ipc {
@@ -52,6 +52,7 @@ __device__ __forceinline__ void ld_codes(const void* p, uint32_t (&w)[2]) {
 }
 __device__ __forceinline__ void ld_codes(const void* p, uint32_t (&w)[1]) { w[0] = __ldg(reinterpret_cast<const uint32_t*>(p)); }
 __device__ __forceinline__ void st_codes(void* p, const uint32_t (&w)[2]) { *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]); }
+__device__ __forceinline__ void st_codes(void* p, const uint32_t (&w)[4]) { *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]); }
 __device__ __forceinline__ void st_codes(void* p, const uint32_t (&w)[1]) { *reinterpret_cast<uint32_t*>(p) = w[0]; }
 // the largest of a block's magnitudes, the block spread over G neighbouring lanes
 template <int G>
@@ -91,7 +92,8 @@ __device__ __forceinline__ void zero_words(int* zero, int n) {
 }
 
 // ---------------------------------------------------------------------------- 8 bits
-// VEC: rows start on 16-byte boundaries (so B is a multiple of a vector); 4 threads a block (8 in fp32).
+// VEC: rows start on 16-byte boundaries (so B is a multiple of a vector); 2 threads a block (8 in fp32): the kernel is bound by
+// the instructions it issues, and 16 numbers a thread share a magnitude, a scale and two addresses.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(THREADS) mx8_store_kernel(const T* __restrict__ x, signed char* __restrict__ codes,
                                                             unsigned char* __restrict__ scales, int D, int B, int nb) {
@@ -100,23 +102,29 @@ __global__ void __launch_bounds__(THREADS) mx8_store_kernel(const T* __restrict_
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const long long ldc = (long long)nb * MX_BLOCK;
   if constexpr (VEC) {
-    constexpr int N = Vec<T>::N, TPR = TCOL / N, RPI = THREADS / TPR;  // threads a row, rows at a time
+    constexpr int V = Vec<T>::N, NV = sizeof(T) == 2 ? 2 : 1, N = V * NV;  // vectors and numbers of a thread
+    constexpr int TPR = TCOL / N, RPI = THREADS / TPR;                     // threads a row, rows at a time
     const int c = c0 + N * (tid % TPR);
-    uint4 raw[TR / RPI];
+    uint4 raw[TR / RPI][NV];
 #pragma unroll
     for (int it = 0; it < TR / RPI; ++it) {  // all loads first
       const int d = d0 + tid / TPR + RPI * it;
-      raw[it] = make_uint4(0, 0, 0, 0);
-      if (d < D && c < B) raw[it] = __ldg(reinterpret_cast<const uint4*>(x + (long long)d * B + c));
+#pragma unroll
+      for (int h = 0; h < NV; ++h) {
+        raw[it][h] = make_uint4(0, 0, 0, 0);
+        if (d < D && c + V * h < B) raw[it][h] = __ldg(reinterpret_cast<const uint4*>(x + (long long)d * B + c) + h);
+      }
     }
 #pragma unroll
     for (int it = 0; it < TR / RPI; ++it) {
       const int r = tid / TPR + RPI * it, d = d0 + r;
-      const uint32_t byte = mx8_scale_byte(group_max<MX_BLOCK / N>(Vec<T>::max_bits(raw[it])));
+      uint32_t m = Vec<T>::max_bits(raw[it][0]);
+      if constexpr (NV == 2) m = max(m, Vec<T>::max_bits(raw[it][1]));
+      const uint32_t byte = mx8_scale_byte(group_max<MX_BLOCK / N>(m));
       const float inv = mx_inv_scale(byte);
       if (c % MX_BLOCK == 0) s_scale[(c - c0) / MX_BLOCK][r] = (unsigned char)byte;
       if (d < D && c < ldc) {
-        const T* h = reinterpret_cast<const T*>(&raw[it]);
+        const T* h = reinterpret_cast<const T*>(raw[it]);
         uint32_t w[N / 4];
 #pragma unroll
         for (int q = 0; q < N / 4; ++q) {
@@ -125,8 +133,10 @@ __global__ void __launch_bounds__(THREADS) mx8_store_kernel(const T* __restrict_
 #pragma unroll
           for (int j = 0; j < 4; ++j) t[j] = __float_as_uint(fmaf(St<T>::ld(h[4 * q + j]), inv, 12582912.f));
           w[q] = __byte_perm(__byte_perm(t[0], t[1], 0x0040), __byte_perm(t[2], t[3], 0x0040), 0x5410);
-          if (byte == MX_NAN_BYTE) w[q] = 0;
         }
+        if (byte == MX_NAN_BYTE)
+#pragma unroll
+          for (int q = 0; q < N / 4; ++q) w[q] = 0;
         st_codes(codes + (long long)d * ldc + c, w);
       }
     }
@@ -347,8 +357,13 @@ __device__ __forceinline__ Two<T, PAIR> load_two(const T* row, int lane, bool in
   }
   return t;
 }
+// CTAs of an SM that the registers are held to: the loads of a CTA are all in flight at once, and other CTAs work meanwhile
+// (8192 x 4096, bf16: 24 us with two, 22 with four); the transcendental f need the registers.
+__host__ __device__ constexpr int turned_ctas(size_t size, int act, bool pair) {
+  return size != 2 || (act != IPC_ACT_RELU && act != IPC_ACT_IDENTITY) ? 2 : pair ? 4 : 3;
+}
 template <typename T, int ACT, bool PAIR>
-__global__ void __launch_bounds__(THREADS) mx4_turned_kernel(const T* __restrict__ x, unsigned char* __restrict__ codes,
+__global__ void __launch_bounds__(THREADS, turned_ctas(sizeof(T), ACT, PAIR)) mx4_turned_kernel(const T* __restrict__ x, unsigned char* __restrict__ codes,
                                                              unsigned char* __restrict__ scales, int R, int K, int kp) {
   __shared__ __align__(16) unsigned char s_code[TUR][144];  // 128 bytes of codes per sample, rows 16 bytes apart mod 128
   __shared__ __align__(16) unsigned char s_scale[TUR][TB];
@@ -387,11 +402,10 @@ __global__ void __launch_bounds__(THREADS) mx4_turned_kernel(const T* __restrict
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     float f[MX_BLOCK];
+    if constexpr (!PACKED) {
 #pragma unroll
-    for (int i = 0; i < MX_BLOCK; ++i) {
-      f[i] = St<T>::ld(v[i].v[h]);
-      if constexpr (!PACKED) {
-        f[i] = act_full<ACT>(f[i]);
+      for (int i = 0; i < MX_BLOCK; ++i) {
+        f[i] = act_full<ACT>(St<T>::ld(v[i].v[h]));
         if (ACT == IPC_ACT_SIGMOID && !(in[h] && kb + i < K)) f[i] = 0.f;  // (the other f are 0 at 0)
         top[h] = max(top[h], abs_bits(f[i]));
       }
@@ -404,7 +418,7 @@ __global__ void __launch_bounds__(THREADS) mx4_turned_kernel(const T* __restrict
     for (int q = 0; q < 4; ++q) {
       float a[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) a[j] = f[8 * q + j] * inv;
+      for (int j = 0; j < 8; ++j) a[j] = (PACKED ? St<T>::ld(v[8 * q + j].v[h]) : f[8 * q + j]) * inv;
       w[q] = byte == MX_NAN_BYTE ? 0u : mx4_pack8(a);
     }
     *reinterpret_cast<uint4*>(&s_code[rl[h]][16 * warp]) = o;
@@ -434,23 +448,26 @@ __global__ void __launch_bounds__(THREADS) mx4_restore_kernel(const unsigned cha
   const int r0 = blockIdx.y * TR, c0 = blockIdx.x * TCOL;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if constexpr (VEC) {
-    constexpr int N = 8, TPR = TCOL / N, RPI = THREADS / TPR;
-    const int c = c0 + N * (tid % TPR);
+    constexpr int N = 8, TPR = TCOL / N, RPI = THREADS / TPR, IT = TR / RPI;
+    const int c = c0 + N * (tid % TPR), rf = r0 + tid / TPR;
     if (c >= K) return;
-    uint32_t q[TR / RPI], byte[TR / RPI];
+    // (a tile's 32 rows lie 16 bytes apart in their scale atom)
+    const unsigned char* cp = codes + (long long)rf * (kp / 2) + c / 2;
+    const unsigned char* sp = scales + mx4_scale_at(r0, c / MX_BLOCK, kp / 128) + 16 * (tid / TPR);
+    T* op = out + (long long)rf * K + c;
+    const long long cs = (long long)RPI * (kp / 2), os = (long long)RPI * K;
+    uint32_t q[IT], byte[IT];
 #pragma unroll
-    for (int it = 0; it < TR / RPI; ++it) {  // all loads first
-      const int r = r0 + tid / TPR + RPI * it;
+    for (int it = 0; it < IT; ++it) {  // all loads first
       q[it] = byte[it] = 0;
-      if (r < R) {
-        q[it] = __ldg(reinterpret_cast<const uint32_t*>(codes + (long long)r * (kp / 2) + c / 2));
-        byte[it] = __ldg(scales + mx4_scale_at(r, c / MX_BLOCK, kp / 128));
+      if (rf + RPI * it < R) {
+        q[it] = __ldg(reinterpret_cast<const uint32_t*>(cp + it * cs));
+        byte[it] = __ldg(sp + 16 * RPI * it);
       }
     }
 #pragma unroll
-    for (int it = 0; it < TR / RPI; ++it) {
-      const int r = r0 + tid / TPR + RPI * it;
-      if (r >= R) continue;
+    for (int it = 0; it < IT; ++it) {
+      if (rf + RPI * it >= R) break;
       const float sc = mx_scale(byte[it]);
       uint32_t h[4];
       mx4_unpack8(q[it], h);
@@ -463,7 +480,7 @@ __global__ void __launch_bounds__(THREADS) mx4_restore_kernel(const unsigned cha
       }
 #pragma unroll
       for (int g = 0; g < N; g += Vec<T>::N)  // (K is a multiple of a vector)
-        if (c + g < K) Vec<T>::store(out + (long long)r * K + c + g, *reinterpret_cast<float(*)[Vec<T>::N]>(v + g));
+        if (c + g < K) Vec<T>::store(op + it * os + g, *reinterpret_cast<float(*)[Vec<T>::N]>(v + g));
     }
   } else {
     constexpr int RW = TR / (THREADS / 32);
