@@ -358,12 +358,13 @@ __device__ __forceinline__ Two<T, PAIR> load_two(const T* row, int lane, bool in
   return t;
 }
 // CTAs of an SM that the registers are held to: the loads of a CTA are all in flight at once, and other CTAs work meanwhile
-// (8192 x 4096, bf16: 24 us with two, 22 with four); the transcendental f need the registers.
-__host__ __device__ constexpr int turned_ctas(size_t size, int act, bool pair) {
-  return size != 2 || (act != IPC_ACT_RELU && act != IPC_ACT_IDENTITY) ? 2 : pair ? 4 : 3;
+// (8192 x 4096, bf16: 21.7 us with two, 18.3 with three, 19.7 with four; reading alone, in these 128-byte pieces, takes 17);
+// the transcendental f need the registers.
+__host__ __device__ constexpr int turned_ctas(size_t size, int act) {
+  return size != 2 || (act != IPC_ACT_RELU && act != IPC_ACT_IDENTITY) ? 2 : 3;
 }
 template <typename T, int ACT, bool PAIR>
-__global__ void __launch_bounds__(THREADS, turned_ctas(sizeof(T), ACT, PAIR)) mx4_turned_kernel(const T* __restrict__ x, unsigned char* __restrict__ codes,
+__global__ void __launch_bounds__(THREADS, turned_ctas(sizeof(T), ACT)) mx4_turned_kernel(const T* __restrict__ x, unsigned char* __restrict__ codes,
                                                              unsigned char* __restrict__ scales, int R, int K, int kp) {
   __shared__ __align__(16) unsigned char s_code[TUR][144];  // 128 bytes of codes per sample, rows 16 bytes apart mod 128
   __shared__ __align__(16) unsigned char s_scale[TUR][TB];
