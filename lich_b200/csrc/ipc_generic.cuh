@@ -74,6 +74,7 @@ struct GemmArgs {
   // first TAIL_FLAG_BYTES, zeroed by an earlier kernel of the stream); null: no such split
   void* tail_ws;
   size_t tail_bytes;
+  int early;        // the kernel before it in the stream prepares operands and lets this one set up meanwhile
   int ragged;       // WD, G, BK: rows of out start anywhere (odd Ng, or a view); lda and ldb still suit TMA
 };
 

@@ -6,6 +6,7 @@
 // whole sectors (with two vectors a thread the stores reach L2 as half sectors: 22 us against 17 us for 8-bit codes at
 // 4096 x 8192 in bf16).  Rows that do not start on 16-byte boundaries take a lane per element.
 #include "ipc_mx.cuh"
+#include "ipc_ptx.cuh"
 
 namespace ipc {
 namespace {
@@ -230,6 +231,7 @@ template <typename T, int ACT, bool VEC>
 __global__ void __launch_bounds__(THREADS)
     mx8_restore_kernel(const signed char* __restrict__ codes, const unsigned char* __restrict__ scales,
                        T* __restrict__ out, int D, int cols, int nb, long long ld_out, int* zero, int n_zero) {
+  grid_let_next_start();
   zero_words(zero, n_zero);
   restore_tile<T, ACT, VEC>(codes, scales, out, D, cols, nb, ld_out);
 }
@@ -532,6 +534,7 @@ int pack_blocks(const PackJob& j) {
   return (int)(n < 148 * 8 ? n : 148 * 8);
 }
 __global__ void __launch_bounds__(THREADS) mx8_pack_kernel(const PackJob a, const PackJob b, int blocks_a) {
+  grid_let_next_start();
   if ((int)blockIdx.x < blocks_a)
     pack_rows(a, blockIdx.x, blocks_a);
   else
@@ -543,6 +546,7 @@ __global__ void __launch_bounds__(THREADS)
     mx8_restore_pack_kernel(const signed char* __restrict__ codes, const unsigned char* __restrict__ scales,
                             T* __restrict__ out, int D, int cols, int nb, long long ld_out, const PackJob j, int rows_r, int* zero,
                             int n_zero) {
+  grid_let_next_start();
   zero_words(zero, n_zero);
   if ((int)blockIdx.y < rows_r)
     restore_tile<T, ACT, true>(codes, scales, out, D, cols, nb, ld_out);

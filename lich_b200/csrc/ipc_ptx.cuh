@@ -110,6 +110,11 @@ __device__ __forceinline__ void mbar_drain(uint32_t bar, uint32_t parity) {
   }
 }
 
+// Programmatic dependent launch: the earlier kernel lets the next one start once all its CTAs run; the next one waits
+// here for its completion (neither does anything in a kernel launched the ordinary way).
+__device__ __forceinline__ void grid_let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // ---- CTA-pair (cta_group::2) helpers: a 256 x BN tile computed by two CTAs of a cluster, each holding
 // 128 rows of A and BN/2 columns of B; the even CTA (the leader) issues the MMAs, the odd CTA's TMA
 // loads complete on the leader's stage barriers, the commits arrive at both CTAs' barriers.

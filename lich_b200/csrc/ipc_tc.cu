@@ -420,6 +420,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
   if constexpr (PAIR) cluster_sync();  // both CTAs' barriers exist before either signals the other's
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  grid_wait();  // what an earlier kernel prepares (GemmArgs::early) is complete from here on
   const int nk = (p.Kg + TC_BK - 1) / TC_BK;
   // an epilogue thread has read its part of an accumulator: arrive on the leader's tempty barrier
   auto release_acc = [&](uint32_t bar) {
@@ -1208,18 +1209,31 @@ int launch_tc_t(const GemmArgs& a, int dtype, cudaStream_t s, float* ws, size_t 
     cfg.blockDim = dim3(TC_THREADS, 1, 1);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = 2;
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = a.early ? 2 : 1;
     err = cudaLaunchKernelEx(&cfg, kern, ta, tb, te[0], te[1], te[2], p);
     if (err != cudaSuccess) return set_error(IPC_ERR_CUDA, "tcgen05 pair GEMM launch: %s", cudaGetErrorString(err));
   } else {
     const int grid = p.tiles < cap ? p.tiles : cap;
-    kern<<<grid, TC_THREADS, smem, s>>>(ta, tb, te[0], te[1], te[2], p);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(TC_THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = a.early ? 1 : 0;
+    err = cudaLaunchKernelEx(&cfg, kern, ta, tb, te[0], te[1], te[2], p);
+    if (err != cudaSuccess) return set_error(IPC_ERR_CUDA, "tcgen05 GEMM launch: %s", cudaGetErrorString(err));
   }
   count_launch();
   int rc2 = check_launch("tcgen05 GEMM");
