@@ -13,7 +13,7 @@
 // Scale factors: the MMA takes those of 128 rows x 4 blocks from 4 columns, in each lane quarter lane i, column c the
 // bytes of row 32 c + i: 16 bytes of an atom a lane, so a warp moves an atom with one 16-byte load and one tcgen05.st.
 // tcgen05.cp would do it in one instruction of the MMA thread, but runs in order with the MMAs: six copies before a
-// stage's four MMAs made 4096 x 4096 x 8192 take 69 us instead of 56 (and as much with the copies a stage ahead).
+// stage's four MMAs made 4096 x 4096 x 8192 take 69 us instead of 60 (74 to 77 with the copies a stage ahead).
 //
 // Tensor memory: 512 columns hold the scale factors of two stages (24 columns each at most) and two accumulators, so
 // that a tile's epilogue runs beside the next tile's MMAs.  Two of 256 columns leave no room: they overlap in 64

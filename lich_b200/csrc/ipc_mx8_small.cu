@@ -98,7 +98,8 @@ __device__ __forceinline__ uint4 shifted(const Row8<VEC>& r, int left) {
   return make_uint4(o[0], o[1], o[2], o[3]);
 }
 
-// Whether f(x^) is kept in two parts: relu and identity give c * 2^s, which 16 bits hold.
+// Whether f(x^) is kept in two parts: relu and identity give c * 2^s, which 16 bits hold (below fp16's smallest normal
+// number to within half its smallest step).
 __host__ __device__ constexpr bool s_low(int act, int mode) {
   return mode != MODE_BK && act != IPC_ACT_RELU && act != IPC_ACT_IDENTITY;
 }

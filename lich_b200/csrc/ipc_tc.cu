@@ -119,9 +119,10 @@ struct TcParams {
   long long ld_ck;
   int ragged;     // WD, G, BK: rows of out start on any element: stored a lane per column, not in 16-byte vectors
   // The last round of tiles (W, WD, G; one group, splits == 1): units from tail_from on are the halves of the remaining
-  // tiles, tail_kps K blocks the first.  The first half owns the tile; the second leaves its fp32 accumulators in
+  // tiles, tail_kps K blocks the first.  The second half owns the tile; the first leaves its fp32 accumulators in
   // tail_ws, [tile][CTA of the pair][warp][32-column chunk][4 registers][lane], and raises a flag per warp; the owner's
-  // warps wait for theirs and add them.
+  // warps wait for theirs and add them.  The owner sits on the next higher CTA (pair): blocks start in order, so whoever
+  // waits waits for one that has started, even if other kernels hold some SMs.
   int tail_from, tail_kps;
   int* tail_flags;
   float* tail_ws;
@@ -625,17 +626,17 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
             __syncwarp();
             if (t + units < p.tiles) fetch_states(t + units);
           }
-          const bool halved = TAIL && t >= p.tail_from, owner = halved && ((t - p.tail_from) & 1) == 0;
+          const bool halved = TAIL && t >= p.tail_from, owner = halved && ((t - p.tail_from) & 1) == 1;
           const long long slot = halved ? tail_slot(p, t, NCTA, rank, warp - 2) : 0;
           if (owner && ok) ok = tail_wait(p, slot, abort_flag);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           tc_fence_after();
           const uint32_t trow = tmem_base + ((uint32_t)(32 * q) << 16) + acc * BN;
-          float4 other[TAIL ? 8 : 1];  // the second half's accumulators, a chunk ahead
+          float4 other[TAIL ? 8 : 1];  // the first half's accumulators, a chunk ahead
           if constexpr (TAIL)
             if (owner) tail_get<HC / 32>(p, slot, 0, lane, other);
-          if (halved && !owner) {  // the second half: to the workspace
+          if (halved && !owner) {  // the first half: to the workspace
 #pragma unroll 1
             for (int c = 0; c < HC / 32; ++c) {
               uint32_t raw[32];
@@ -834,7 +835,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
           tile_coords(p, t, BN, g, m0, n0, sp, TM, rank);
           const int r0 = m0 + 32 * q, nw = n0 + c_lo;
           bool ok = mbar_wait(tfull0 + 8 * acc, aphase, abort_flag);
-          const bool halved = t >= p.tail_from, owner = halved && ((t - p.tail_from) & 1) == 0;
+          const bool halved = t >= p.tail_from, owner = halved && ((t - p.tail_from) & 1) == 1;
           const long long slot = halved ? tail_slot(p, t, NCTA, rank, warp - 2) : 0;
           if (owner && ok) ok = tail_wait(p, slot, abort_flag);
           ok = __all_sync(0xffffffffu, ok);

@@ -478,3 +478,24 @@ def test_delta_with_a_halved_last_round(M, K, B):
     want = w0[rows].double() + 0.01 * ref
     _within(w[rows.to(DEV)], want, (0.01 * err) * (1 + U[dt]) + (U[dt] + 2.0 ** -22) * (want.abs() + 0.01 * ref.abs()))
     assert N.device_status() == 0
+
+
+@pytest.mark.parametrize("B", [3, 16, 200])
+def test_forward_over_the_range_of_the_scales(B):
+    """Features 2^110 and 2^-120 times the others' size, and weights that undo a factor of 2^100: every block is scaled by
+    its own two powers of two, so the bound is that of equal sizes."""
+    mx = _mx()
+    M, K = 150, 512
+    for wf, af in ((1.0, 1.0), (2.0 ** -100, 2.0 ** 100), (2.0 ** 100, 2.0 ** -100)):
+        w = _rand((M, K), 1, K ** -0.5) * wf
+        x = torch.randn(K, B, generator=torch.Generator().manual_seed(2)) * af
+        if af == 1.0:
+            x[32:64] *= 2.0 ** 110
+            x[64:96] *= 2.0 ** -120
+            w[5:40, 32:64] = 0  # rows without the large features
+        wv, wq, wsc = X.quant4(w)
+        av, aq, asc = X.quant4(x.t().contiguous())
+        out = torch.full((M, B), 9.0, device=DEV)
+        mx.build_mxfp4_forward(M, K, B, "float32")(wq.to(DEV), wsc.to(DEV), aq.to(DEV), asc.to(DEV), out)
+        ref = wv @ av.t()
+        _within(out, ref, (wv.abs() @ av.abs().t()) * K * 2.0 ** -23 + U[torch.float32] * ref.abs() + TINY[torch.float32])
