@@ -6,7 +6,9 @@ Each ``csrc/*.cu`` is compiled by nvcc (``-gencode arch=compute_100a,code=sm_100
 in parallel, then linked into one shared library with the CUDA runtime
 linked statically, so the library depends only on the driver.  The build is
 incremental: an object is rebuilt when its source or any ``csrc/*.cuh`` /
-``include/*.h`` header is newer.
+``include/*.h`` header is newer.  ``csrc/mx_call.cpp``, the Python call layer of
+the microscaled operators, is compiled against torch's headers into
+``lich_b200/_lib/_mx_call.so`` (again whenever torch's version changes).
 """
 from __future__ import annotations
 
@@ -23,6 +25,7 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 OBJ = PKG / "_lib" / "obj"
 LIB = PKG / "_lib" / "libipc_b200.so"
+CALL = PKG / "_lib" / "_mx_call.so"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr",
@@ -54,8 +57,37 @@ def _compile(src: Path, extra: list[str], verbose: bool) -> Path:
     return obj
 
 
+def _build_call(verbose: bool, force: bool) -> None:
+    import sysconfig
+
+    import torch
+
+    src, stamp = CSRC / "mx_call.cpp", OBJ / "mx_call.torch"
+    made_for = f"{torch.__version__} {sys.version}"
+    newest = max(src.stat().st_mtime, (ROOT / "include" / "ipc_b200.h").stat().st_mtime)
+    if (not force and CALL.exists() and CALL.stat().st_mtime >= newest and stamp.exists()
+            and stamp.read_text() == made_for):
+        return
+    inc = Path(torch.__file__).resolve().parent / "include"
+    libs = Path(torch.__file__).resolve().parent / "lib"
+    cuda = Path(nvcc()).resolve().parents[1] / "include"
+    tmp = CALL.with_suffix(".so.tmp")
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I", sysconfig.get_paths()["include"],
+           "-isystem", str(inc), "-isystem", str(inc / "torch" / "csrc" / "api" / "include"), "-isystem", str(cuda),
+           str(src), "-o", str(tmp), f"-L{libs}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed on {src.name}:\n{r.stdout}\n{r.stderr}")
+    os.replace(tmp, CALL)
+    stamp.write_text(made_for)
+
+
 def build(verbose: bool = False, ptxas_info: bool = False, force: bool = False) -> Path:
     OBJ.mkdir(parents=True, exist_ok=True)
+    _build_call(verbose, force)
     srcs = sorted(CSRC.glob("*.cu"))
     hdr_t = _headers_mtime()
     extra = ["-Xptxas", "-v"] if ptxas_info else []

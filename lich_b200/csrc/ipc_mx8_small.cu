@@ -205,6 +205,21 @@ __global__ void __launch_bounds__(STHREADS) mx8_small_kernel(const __grid_consta
   };
 
   float acc[4][4] = {};
+  // BK: the states of this thread's results (two codes at a time, one scale block per warp), read before the sum needs them
+  const int gq = lane >> 2, tq = lane & 3;
+  uint32_t code2[BKM ? 4 : 1][2], sbyte[2];
+  if constexpr (BKM) {
+    const int blk = (n0 + wn * 32) / MX_BLOCK;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int m = m0 + wm * 16 + gq + 8 * h;
+      const bool in = m < p.Mg && n0 + wn * 32 < p.Ng;  // (a row's codes are padded to whole blocks)
+      sbyte[h] = in ? p.cks[(long long)blk * p.Mg + m] : 0u;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        code2[j][h] = in ? __ldg(reinterpret_cast<const uint16_t*>(p.ck + (long long)m * p.ld_ck + n0 + wn * 32 + 8 * j + 2 * tq)) : 0u;
+    }
+  }
   if (k_lo < k_hi) fetch(k_lo);
   int buf = 0;
   for (int k0 = k_lo; k0 < k_hi; k0 += SK, buf ^= 1) {
@@ -265,7 +280,6 @@ __global__ void __launch_bounds__(STHREADS) mx8_small_kernel(const __grid_consta
 #pragma unroll
         for (int r = 0; r < 4; ++r) acc[j][r] += red[c * SM * SN + (4 * j + r) * STHREADS + tid];
   }
-  const int gq = lane >> 2, tq = lane & 3;
 #pragma unroll
   for (int j = 0; j < 4; ++j)
 #pragma unroll
@@ -273,7 +287,7 @@ __global__ void __launch_bounds__(STHREADS) mx8_small_kernel(const __grid_consta
       const int m = m0 + wm * 16 + gq + (r >= 2 ? 8 : 0), n = n0 + wn * 32 + 8 * j + 2 * tq + (r & 1);
       if (m < p.Mg && n < p.Ng) {
         if constexpr (BKM) {
-          const float x = (float)p.ck[(long long)m * p.ld_ck + n] * mx_scale(p.cks[(long long)(n / MX_BLOCK) * p.Mg + m]);
+          const float x = (float)(signed char)(code2[j][r >> 1] >> (8 * (r & 1))) * mx_scale(sbyte[r >> 1]);
           reinterpret_cast<T*>(p.out)[(long long)m * p.Ng + n] = St<T>::st(act_df_hw<ACT>(x) * acc[j][r]);
         } else {
           epilogue<T, IPC_ACT_IDENTITY, MODE>(p, 0, m, n, acc[j][r]);

@@ -24,8 +24,10 @@ The reference has no counterpart: it keeps and multiplies fp16 only (``tilelang_
 """
 from __future__ import annotations
 
-from ctypes import byref, c_size_t
-from functools import lru_cache
+import importlib.machinery
+import importlib.util
+from ctypes import byref, c_size_t, c_void_p, cast
+from functools import lru_cache, wraps
 
 import torch
 
@@ -33,6 +35,20 @@ from . import _native as N
 from .tilelang_kernels import KernelConfig, _algo
 
 N.load()
+
+
+def _load_call():
+    """``csrc/mx_call.cpp``: the checked call in C++ (built beside the library)."""
+    path = N.LIB_PATH.parent / "_mx_call.so"
+    if not path.exists():
+        raise RuntimeError(f"native module {path} is missing: build it with `python -m lich_b200.build`")
+    loader = importlib.machinery.ExtensionFileLoader("_mx_call", str(path))
+    module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_mx_call", loader))
+    loader.exec_module(module)
+    return module
+
+
+_Call = _load_call().Call
 
 BLOCK = 32
 # what torch.cuda.current_device() and current_stream().cuda_stream come down to, at a tenth of their cost
@@ -65,11 +81,22 @@ class _MxOp:
     """Shape-specialised callable over the C ABI: ``spec`` names each tensor argument's shape and dtype."""
 
     kind = "op"
+    call_kind = -1  # the kind and ...
+    call_ints: tuple = ()  # ... the attributes that the C++ call passes on as integers
+    alpha = 0.0
 
     def __init__(self, entry: str, spec):
         self.spec = tuple((torch.Size(s), d) for s, d in spec)
         self._fn = getattr(N.load(), entry)
         self._ws: dict = {}
+
+    def fast(self):
+        """This operator as a C++ callable, which comes back here for everything but a plain call."""
+        return _Call(self, self.call_kind, cast(self._fn, c_void_p).value, list(self.spec),
+                     tuple(int(getattr(self, n)) for n in self.call_ints), float(self.alpha))
+
+    def _failed(self, rc: int) -> None:
+        N.check(rc)
 
     def _stream(self, tensors):
         """The current stream of the tensors' device, after checking the tensors against ``spec``; None when that device is
@@ -121,6 +148,7 @@ class _MxOp:
 
 class CheckpointKernel(_MxOp):
     kind = "checkpoint"
+    call_kind, call_ints = 0, ("D", "B", "dt")
 
     def __init__(self, D, B, dtype):
         c, s = checkpoint_shapes(D, B)
@@ -138,6 +166,7 @@ class CheckpointKernel(_MxOp):
 
 class CheckpointRestoreKernel(_MxOp):
     kind = "checkpoint_restore"
+    call_kind, call_ints = 1, ("D", "B", "act", "dt")
 
     def __init__(self, D, B, activation, dtype):
         c, s = checkpoint_shapes(D, B)
@@ -155,6 +184,7 @@ class CheckpointRestoreKernel(_MxOp):
 
 class CheckpointWeightKernel(_MxOp):
     kind = "weight_checkpoint"
+    call_kind, call_ints = 2, ("mode", "M", "K", "B", "act", "dt", "algo")
 
     def __init__(self, mode, M, K, B, activation, dtype, alpha, out_dtype, cfg):
         c, s = checkpoint_shapes(K, B)
@@ -181,6 +211,7 @@ class CheckpointWeightKernel(_MxOp):
 
 class CheckpointBackwardKernel(_MxOp):
     kind = "error_backward_checkpoint"
+    call_kind, call_ints = 3, ("M", "K", "B", "act", "dt", "algo")
 
     def __init__(self, M, K, B, activation, dtype, cfg):
         c, s = checkpoint_shapes(K, B)
@@ -206,6 +237,7 @@ class CheckpointBackwardKernel(_MxOp):
 
 class Mxfp4QuantizeKernel(_MxOp):
     kind = "mxfp4_quantize"
+    call_kind, call_ints = 4, ("R", "K", "turned", "act", "dt")
 
     def __init__(self, R, K, activation, dtype, turned):
         c, s = mxfp4_shapes(R, K)
@@ -225,6 +257,7 @@ class Mxfp4QuantizeKernel(_MxOp):
 
 class Mxfp4RestoreKernel(_MxOp):
     kind = "mxfp4_restore"
+    call_kind, call_ints = 5, ("R", "K", "dt")
 
     def __init__(self, R, K, dtype):
         c, s = mxfp4_shapes(R, K)
@@ -242,6 +275,7 @@ class Mxfp4RestoreKernel(_MxOp):
 
 class Mxfp4ForwardKernel(_MxOp):
     kind = "mxfp4_forward"
+    call_kind, call_ints = 6, ("M", "K", "B", "dt")
 
     def __init__(self, M, K, B, dtype):
         wc, ws = mxfp4_shapes(M, K)
@@ -260,6 +294,15 @@ class Mxfp4ForwardKernel(_MxOp):
             N.check(rc)
 
 
+def _builder(build):
+    """A cached builder of C++ callables."""
+    @lru_cache(maxsize=256)
+    @wraps(build)
+    def cached(*args, **kw):
+        return build(*args, **kw).fast()
+    return cached
+
+
 def _validate(*sizes, activation="identity", dtype):
     if min(int(n) for n in sizes) < 0:
         raise ValueError(f"negative size in {sizes}")
@@ -267,21 +310,21 @@ def _validate(*sizes, activation="identity", dtype):
     N.dtype_code(N.torch_dtype(dtype))
 
 
-@lru_cache(maxsize=256)
+@_builder
 def build_checkpoint(D: int, B: int, dtype: str):
     """``kernel(x [D, B], codes, scales)``: the states in 8 bits."""
     _validate(D, B, dtype=dtype)
     return CheckpointKernel(D, B, dtype)
 
 
-@lru_cache(maxsize=256)
+@_builder
 def build_checkpoint_restore(D: int, B: int, activation: str, dtype: str):
     """``kernel(codes, scales, out [D, B])``: ``out = f(x^)``."""
     _validate(D, B, activation=activation, dtype=dtype)
     return CheckpointRestoreKernel(D, B, activation, dtype)
 
 
-@lru_cache(maxsize=256)
+@_builder
 def build_weight_update_checkpoint(M: int, K: int, B: int, activation: str, dtype: str, alpha: float,
                                    cfg: KernelConfig = KernelConfig()):
     """``kernel(w [M, K], e [M, B], codes, scales)``: ``W += alpha * E @ f(x^)^T`` in place."""
@@ -289,7 +332,7 @@ def build_weight_update_checkpoint(M: int, K: int, B: int, activation: str, dtyp
     return CheckpointWeightKernel(N.MODE_WEIGHT, M, K, B, activation, dtype, alpha, N.torch_dtype(dtype), cfg)
 
 
-@lru_cache(maxsize=256)
+@_builder
 def build_weight_delta_checkpoint(M: int, K: int, B: int, activation: str, dtype: str, alpha: float,
                                   delta_dtype: str = "float32", cfg: KernelConfig = KernelConfig()):
     """``kernel(dw [M, K], e [M, B], codes, scales, accumulate=False)``: ``dw = alpha * E @ f(x^)^T``, in float32 (which
@@ -302,7 +345,7 @@ def build_weight_delta_checkpoint(M: int, K: int, B: int, activation: str, dtype
     return CheckpointWeightKernel(mode, M, K, B, activation, dtype, alpha, out, cfg)
 
 
-@lru_cache(maxsize=256)
+@_builder
 def build_error_backward_checkpoint(M: int, K: int, B: int, activation: str, dtype: str,
                                     cfg: KernelConfig = KernelConfig()):
     """``kernel(w [M, K], e [M, B], codes, scales, e_up [K, B])``: ``e_up = f'(x^) * (W^T @ E)``."""
@@ -310,7 +353,7 @@ def build_error_backward_checkpoint(M: int, K: int, B: int, activation: str, dty
     return CheckpointBackwardKernel(M, K, B, activation, dtype, cfg)
 
 
-@lru_cache(maxsize=256)
+@_builder
 def build_mxfp4_quantize(R: int, K: int, activation: str, dtype: str, turned: bool = False):
     """``kernel(x, codes, scales)``: ``f(x)`` as a 4-bit operand of ``R`` rows; ``x`` is ``[R, K]``, or with ``turned``
     the feature-major ``[K, R]``."""
@@ -318,14 +361,14 @@ def build_mxfp4_quantize(R: int, K: int, activation: str, dtype: str, turned: bo
     return Mxfp4QuantizeKernel(R, K, activation, dtype, turned)
 
 
-@lru_cache(maxsize=256)
+@_builder
 def build_mxfp4_restore(R: int, K: int, dtype: str):
     """``kernel(codes, scales, out [R, K])``: the values a 4-bit operand stands for."""
     _validate(R, K, dtype=dtype)
     return Mxfp4RestoreKernel(R, K, dtype)
 
 
-@lru_cache(maxsize=256)
+@_builder
 def build_mxfp4_forward(M: int, K: int, B: int, dtype: str):
     """``kernel(w, w_scales, a, a_scales, out [M, B])``: ``out = W4 @ A4^T``, sums in float32, stored in ``dtype``."""
     _validate(M, K, B, dtype=dtype)

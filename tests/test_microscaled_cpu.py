@@ -93,3 +93,24 @@ def test_abi_refuses_bad_arguments():
     assert lib.ipc_mxfp4_forward(None, None, None, None, None, 4, 4, -1, 1, None) == A
     n = ctypes.c_size_t(0)
     assert lib.ipc_mx8_weight_ws_bytes(3, -1, 4, 4, 1, 0, ctypes.byref(n)) == A
+
+
+def test_the_call_layer_hands_everything_unusual_to_the_operator():
+    from lich_b200 import microscaled as mx
+    k = mx.build_checkpoint(4, 40, "float16")
+    assert k.kind == "checkpoint" and (k.D, k.B) == (4, 40)  # attributes are the operator's
+    with pytest.raises(AttributeError):
+        k.nothing
+    x = torch.zeros(4, 40, dtype=torch.float16)
+    c, s = mx.empty_checkpoint(4, 40, device="cpu")
+    with pytest.raises(TypeError):
+        k(x, c)
+    with pytest.raises(TypeError):
+        k(x, c, s, s)
+    with pytest.raises(ValueError, match="not a CUDA tensor"):
+        k(x, codes=c, scales=s)
+    with pytest.raises(ValueError, match="argument 0 is not a tensor"):
+        k(1, c, s)
+    with pytest.raises(ValueError):
+        mx._Call(object(), 0, 0, [], (), 0.0)
+    assert mx.build_mxfp4_forward(4, 5, 6, dtype="float16") is mx.build_mxfp4_forward(4, 5, 6, dtype="float16")

@@ -499,3 +499,22 @@ def test_forward_over_the_range_of_the_scales(B):
         mx.build_mxfp4_forward(M, K, B, "float32")(wq.to(DEV), wsc.to(DEV), aq.to(DEV), asc.to(DEV), out)
         ref = wv @ av.t()
         _within(out, ref, (wv.abs() @ av.abs().t()) * K * 2.0 ** -23 + U[torch.float32] * ref.abs() + TINY[torch.float32])
+
+
+def test_call_layer_takes_parameters_and_keywords():
+    """A parameter is not a plain tensor and a keyword no plain call: both go through the Python operator."""
+    mx = _mx()
+    M, K, B = 40, 50, 60
+    e, c, s, ref, err = _delta_case(M, K, B, torch.float32, "tanh")
+    k = mx.build_weight_delta_checkpoint(M, K, B, "tanh", "float32", 1.0)
+    dw = torch.zeros(M, K, device=DEV)
+    k(dw, e.to(DEV), c, s)
+    again = torch.zeros(M, K, device=DEV)
+    k(again, torch.nn.Parameter(e.to(DEV), requires_grad=False), c, s)
+    assert torch.equal(dw, again)
+    k(again, e=e.to(DEV), codes=c, scales=s, accumulate=True)
+    _within(again, 2 * ref, 2 * err + 2.0 ** -22 * 2 * ref.abs())
+    with pytest.raises(ValueError):
+        k(dw.half(), e.to(DEV), c, s)
+    with pytest.raises(ValueError):
+        k(dw, e, c, s)  # one tensor on the CPU
