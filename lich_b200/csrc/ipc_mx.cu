@@ -14,6 +14,11 @@ namespace {
 constexpr int TR = 32;        // rows of a tile
 constexpr int TCOL = 256;     // columns of a tile: 8 blocks
 constexpr int THREADS = 256;
+// A lane per element: up to a warp per row of the tile, so that small odd matrices need one round of loads (1000 x 777: 5 us a
+// kernel with 256 threads, 3.3 with 1024).  The 8-bit kernels keep 256 where tiles fill the GPU anyway (4095 x 4095: 22 us
+// against 25 and 29; the 4-bit ones, whose loads are all in registers, 34 and 38 against 27 and 36).
+constexpr int LANE_THREADS = 1024;
+__host__ __device__ constexpr int threads_of(bool vec) { return vec ? THREADS : LANE_THREADS; }
 constexpr int TB = TCOL / MX_BLOCK;
 
 template <typename T>
@@ -96,7 +101,7 @@ __device__ __forceinline__ void zero_words(int* zero, int n) {
 // VEC: rows start on 16-byte boundaries (so B is a multiple of a vector); 2 threads a block (8 in fp32): the kernel is bound by
 // the instructions it issues, and 16 numbers a thread share a magnitude, a scale and two addresses.
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(THREADS) mx8_store_kernel(const T* __restrict__ x, signed char* __restrict__ codes,
+__global__ void __launch_bounds__(threads_of(VEC)) mx8_store_kernel(const T* __restrict__ x, signed char* __restrict__ codes,
                                                             unsigned char* __restrict__ scales, int D, int B, int nb) {
   __shared__ unsigned char s_scale[TB][TR];
   const int d0 = blockIdx.y * TR, c0 = blockIdx.x * TCOL;
@@ -142,7 +147,7 @@ __global__ void __launch_bounds__(THREADS) mx8_store_kernel(const T* __restrict_
       }
     }
   } else {
-    for (int r = warp; r < TR; r += THREADS / 32) {
+    for (int r = warp; r < TR; r += (int)blockDim.x / 32) {
       const int d = d0 + r;
       float v[TB];
 #pragma unroll
@@ -160,8 +165,8 @@ __global__ void __launch_bounds__(THREADS) mx8_store_kernel(const T* __restrict_
     }
   }
   __syncthreads();
-  const int j = c0 / MX_BLOCK + warp;  // eight warps, eight blocks; a lane per row
-  if (j < nb && d0 + lane < D) scales[(long long)j * D + d0 + lane] = s_scale[warp][lane];
+  const int j = c0 / MX_BLOCK + warp;  // a warp per block, a lane per row
+  if (warp < TB && j < nb && d0 + lane < D) scales[(long long)j * D + d0 + lane] = s_scale[warp][lane];
 }
 
 template <typename T, int ACT, bool VEC>
@@ -207,7 +212,7 @@ __device__ __forceinline__ void restore_tile(const signed char* __restrict__ cod
       }
     }
   } else {
-    for (int r = warp; r < TR; r += THREADS / 32) {
+    for (int r = warp; r < TR; r += (int)blockDim.x / 32) {
       const int d = d0 + r;
       if (d >= D) break;
       int q[TB];
@@ -228,7 +233,7 @@ __device__ __forceinline__ void restore_tile(const signed char* __restrict__ cod
 }
 
 template <typename T, int ACT, bool VEC>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(threads_of(VEC))
     mx8_restore_kernel(const signed char* __restrict__ codes, const unsigned char* __restrict__ scales,
                        T* __restrict__ out, int D, int cols, int nb, long long ld_out, int* zero, int n_zero) {
   grid_let_next_start();
@@ -239,7 +244,7 @@ __global__ void __launch_bounds__(THREADS)
 // ---------------------------------------------------------------------------- 4 bits
 // Rows as stored ([R, K], weights): the mapping of mx8_store_kernel, blocks along the row.
 template <typename T, int ACT, bool VEC>
-__global__ void __launch_bounds__(THREADS) mx4_rows_kernel(const T* __restrict__ x, unsigned char* __restrict__ codes,
+__global__ void __launch_bounds__(threads_of(VEC)) mx4_rows_kernel(const T* __restrict__ x, unsigned char* __restrict__ codes,
                                                            unsigned char* __restrict__ scales, int R, int K, int kp) {
   __shared__ __align__(16) unsigned char s_scale[TR][TB];
   const int r0 = blockIdx.y * TR, c0 = blockIdx.x * TCOL;
@@ -280,18 +285,18 @@ __global__ void __launch_bounds__(THREADS) mx4_rows_kernel(const T* __restrict__
       }
     }
   } else {
-    constexpr int RW = TR / (THREADS / 32);  // rows of a warp, all loads first
+    constexpr int RW = TR / (LANE_THREADS / 32);  // rows of a warp, all loads first
     float in[RW][TB];
 #pragma unroll
     for (int i = 0; i < RW; ++i)
 #pragma unroll
       for (int j = 0; j < TB; ++j) {
-        const int r = r0 + warp + THREADS / 32 * i, c = c0 + MX_BLOCK * j + lane;
+        const int r = r0 + warp + LANE_THREADS / 32 * i, c = c0 + MX_BLOCK * j + lane;
         in[i][j] = (r < R && c < K) ? St<T>::ld(x[(long long)r * K + c]) : 0.f;
       }
 #pragma unroll
     for (int i = 0; i < RW; ++i) {
-      const int rr = warp + THREADS / 32 * i, r = r0 + rr;
+      const int rr = warp + LANE_THREADS / 32 * i, r = r0 + rr;
       float (&v)[TB] = in[i];
 #pragma unroll
       for (int j = 0; j < TB; ++j) {
@@ -445,7 +450,7 @@ __global__ void __launch_bounds__(THREADS, turned_ctas(sizeof(T), ACT)) mx4_turn
 }
 
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(THREADS) mx4_restore_kernel(const unsigned char* __restrict__ codes,
+__global__ void __launch_bounds__(threads_of(VEC)) mx4_restore_kernel(const unsigned char* __restrict__ codes,
                                                               const unsigned char* __restrict__ scales,
                                                               T* __restrict__ out, int R, int K, int kp) {
   const int r0 = blockIdx.y * TR, c0 = blockIdx.x * TCOL;
@@ -486,13 +491,13 @@ __global__ void __launch_bounds__(THREADS) mx4_restore_kernel(const unsigned cha
         if (c + g < K) Vec<T>::store(op + it * os + g, *reinterpret_cast<float(*)[Vec<T>::N]>(v + g));
     }
   } else {
-    constexpr int RW = TR / (THREADS / 32);
+    constexpr int RW = TR / (LANE_THREADS / 32);
     uint32_t q[RW][TB], byte[RW][TB];
 #pragma unroll
     for (int i = 0; i < RW; ++i)  // all loads first
 #pragma unroll
       for (int j = 0; j < TB; ++j) {
-        const int r = r0 + warp + THREADS / 32 * i, c = c0 + MX_BLOCK * j + lane;
+        const int r = r0 + warp + LANE_THREADS / 32 * i, c = c0 + MX_BLOCK * j + lane;
         const bool in = r < R && c < K;
         q[i][j] = in ? __ldg(codes + (long long)r * (kp / 2) + c / 2) : 0u;
         byte[i][j] = in ? __ldg(scales + mx4_scale_at(r, c / MX_BLOCK, kp / 128)) : 0u;
@@ -501,7 +506,7 @@ __global__ void __launch_bounds__(THREADS) mx4_restore_kernel(const unsigned cha
     for (int i = 0; i < RW; ++i)
 #pragma unroll
       for (int j = 0; j < TB; ++j) {
-        const int r = r0 + warp + THREADS / 32 * i, c = c0 + MX_BLOCK * j + lane;
+        const int r = r0 + warp + LANE_THREADS / 32 * i, c = c0 + MX_BLOCK * j + lane;
         uint32_t h[4];
         mx4_unpack8((q[i][j] >> (4 * (lane & 1))) & 15u, h);
         if (r < R && c < K)
@@ -559,6 +564,8 @@ bool rows_aligned(const void* p, long long ld) {
   return ((reinterpret_cast<uintptr_t>(p) | (uintptr_t)(ld * (long long)sizeof(T))) & 15) == 0;
 }
 
+int lane_threads(const dim3& grid) { return (long long)grid.x * grid.y >= 296 ? THREADS : LANE_THREADS; }
+
 int grid_of(const char* what, long long rows, int tile, long long cols, dim3* grid) {
   const long long gy = (rows + tile - 1) / tile, gx = (cols + TCOL - 1) / TCOL;
   if (gy > 65535 || gx > 0x7fffffffLL) return set_error(IPC_ERR_ARG, "%s: %lld rows are too many", what, rows);
@@ -578,7 +585,7 @@ int launch_mx8_store(const void* x, signed char* codes, unsigned char* scales, i
     if (rows_aligned<TT>(x, B))
       mx8_store_kernel<TT, true><<<grid, THREADS, 0, s>>>(xt, codes, scales, D, B, nb);
     else
-      mx8_store_kernel<TT, false><<<grid, THREADS, 0, s>>>(xt, codes, scales, D, B, nb);
+      mx8_store_kernel<TT, false><<<grid, lane_threads(grid), 0, s>>>(xt, codes, scales, D, B, nb);
   });
   count_launch();
   return check_launch("8-bit store");
@@ -597,7 +604,7 @@ int launch_mx8_restore(const signed char* codes, const unsigned char* scales, vo
       if (vec)
         mx8_restore_kernel<TT, AC, true><<<grid, THREADS, 0, s>>>(codes, scales, ot, D, B, nb, ld_out, zero, n_zero);
       else
-        mx8_restore_kernel<TT, AC, false><<<grid, THREADS, 0, s>>>(codes, scales, ot, D, B, nb, ld_out, zero, n_zero);
+        mx8_restore_kernel<TT, AC, false><<<grid, lane_threads(grid), 0, s>>>(codes, scales, ot, D, B, nb, ld_out, zero, n_zero);
     });
   });
   count_launch();
@@ -662,7 +669,7 @@ int launch_mx4_quantize(const void* x, unsigned char* codes, unsigned char* scal
       else if (vec)
         mx4_rows_kernel<TT, AC, true><<<grid, THREADS, 0, s>>>(xt, codes, scales, R, K, kp);
       else
-        mx4_rows_kernel<TT, AC, false><<<grid, THREADS, 0, s>>>(xt, codes, scales, R, K, kp);
+        mx4_rows_kernel<TT, AC, false><<<grid, LANE_THREADS, 0, s>>>(xt, codes, scales, R, K, kp);
     });
   });
   count_launch();
@@ -680,7 +687,7 @@ int launch_mx4_restore(const unsigned char* codes, const unsigned char* scales, 
     if (rows_aligned<TT>(out, K))
       mx4_restore_kernel<TT, true><<<grid, THREADS, 0, s>>>(codes, scales, ot, R, K, kp);
     else
-      mx4_restore_kernel<TT, false><<<grid, THREADS, 0, s>>>(codes, scales, ot, R, K, kp);
+      mx4_restore_kernel<TT, false><<<grid, LANE_THREADS, 0, s>>>(codes, scales, ot, R, K, kp);
   });
   count_launch();
   return check_launch("4-bit restore");
