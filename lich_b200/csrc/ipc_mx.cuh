@@ -88,6 +88,12 @@ __device__ __forceinline__ long long mx4_scale_at(int r, int j, int atoms_k) {
   return ((long long)(r >> 7) * atoms_k + (j >> 2)) * 512 + (r & 31) * 16 + ((r >> 5) & 3) * 4 + (j & 3);
 }
 
+// The largest of 16, 8, 4 and 2 bytes that divides an address and a row stride.
+inline int row_alignment(const void* p, long long row_bytes) {
+  const unsigned long long bits = reinterpret_cast<unsigned long long>(p) | (unsigned long long)row_bytes;
+  return bits % 16 == 0 ? 16 : bits % 8 == 0 ? 8 : bits % 4 == 0 ? 4 : 2;
+}
+
 int launch_mx8_store(const void* x, signed char* codes, unsigned char* scales, int D, int B, int dtype, cudaStream_t s);
 // out[d][b] = cast(f(codes * 2^s)), rows ld_out >= B apart; n_zero words at `zero` are cleared beside it
 int launch_mx8_restore(const signed char* codes, const unsigned char* scales, void* out, int D, int B, long long ld_out,

@@ -53,7 +53,7 @@ struct Mx4Params {
   int tiles_m, tiles_n, tiles, raster;
   void* out;
   long long ld_out;
-  int vec;  // rows of out start on 16-byte boundaries
+  int vec;  // bytes of a store: the largest of 16, 8, 4, 2 on whose boundaries the rows of out start
 };
 
 __device__ __forceinline__ bool f_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
@@ -312,30 +312,16 @@ __global__ void __launch_bounds__(F_THREADS, 1)
           }
           __syncwarp();
           const int ne = n + EW * e;
-          if (p.vec) {
-            constexpr int VE = 16 / (int)sizeof(T);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const int r = 8 * k + (lane >> 2), j = lane & 3;
-              const uint4 v = lds128(xb + r * 64 + ((j ^ ((r >> 1) & 3)) << 4));
-              if (r0 + r < p.M && ne + VE * j < p.N)
-                *reinterpret_cast<uint4*>(out + (long long)(r0 + r) * p.ld_out + ne + VE * j) = v;
-            }
-          } else {  // rows of any alignment: a lane per column
-            const int col = lane % EW;
-            const int j = col * (int)sizeof(T) / 16, in = col * (int)sizeof(T) % 16;
-#pragma unroll 4
-            for (int r = lane / EW; r < 32; r += 32 / EW) {
-              const uint32_t a = xb + r * 64 + ((j ^ ((r >> 1) & 3)) << 4) + in;
-              T v;
-              if constexpr (sizeof(T) == 4) {
-                v = __uint_as_float(lds32(a));
-              } else {
-                const uint16_t h = lds16(a);
-                v = *reinterpret_cast<const T*>(&h);
-              }
-              if (r0 + r < p.M && ne + col < p.N) out[(long long)(r0 + r) * p.ld_out + ne + col] = v;
-            }
+          char* dst = reinterpret_cast<char*>(out + (long long)r0 * p.ld_out + ne);
+          const long long ld = p.ld_out * (long long)sizeof(T);
+          const int rows = p.M - r0, bytes = min(p.N - ne, EW) * (int)sizeof(T);
+          auto swz = [](int r) { return (r >> 1) & 3; };
+          switch (p.vec) {
+            case 16: store_rows<64, 16>(dst, ld, rows, bytes, xb, lane, swz); break;
+            case 8: store_rows<64, 8>(dst, ld, rows, bytes, xb, lane, swz); break;
+            case 4: store_rows<64, 4>(dst, ld, rows, bytes, xb, lane, swz); break;
+            default:
+              if constexpr (sizeof(T) == 2) store_rows<64, 2>(dst, ld, rows, bytes, xb, lane, swz);
           }
           __syncwarp();
         }
@@ -542,7 +528,7 @@ int launch_tiles(const unsigned char* w, const unsigned char* wsc, const unsigne
   p.raster = 16;
   p.out = out;
   p.ld_out = B;
-  p.vec = ((reinterpret_cast<uintptr_t>(out) | (uintptr_t)((long long)B * (long long)sizeof(T))) & 15) == 0;
+  p.vec = row_alignment(out, (long long)B * (long long)sizeof(T));
   constexpr int SMEM = f_stages(BN) * f_stage_bytes(BN) + F_EPI_WARPS * F_EPI_BYTES + 1024 + 256;
   static_assert(SMEM <= 232448, "shared memory of a 4-bit product CTA");
   cudaError_t err = ensure_kernel_smem<mx4_gemm_kernel<T, BN>>(SMEM);

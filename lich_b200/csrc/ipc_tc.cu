@@ -117,7 +117,7 @@ struct TcParams {
   const signed char* ck;  // BK: the 8-bit states' codes, their row stride, and their scale bytes [block][row]
   const unsigned char* cks;
   long long ld_ck;
-  int ragged;     // WD, G, BK: rows of out start on any element: stored a lane per column, not in 16-byte vectors
+  int ragged;     // WD, G, BK: rows of out start on any element; bytes of a store (WD 4: a lane per column; G, BK 8, 4, 2); else 0
   // The last round of tiles (W, WD, G; one group, splits == 1): units from tail_from on are the halves of the remaining
   // tiles, tail_kps K blocks the first.  The second half owns the tile; the first leaves its fp32 accumulators in
   // tail_ws, [tile][CTA of the pair][warp][32-column chunk][4 registers][lane], and raises a flag per warp; the owner's
@@ -690,6 +690,16 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
               release_acc(tempty0 + 8 * acc);
             }
             __syncwarp();
+            if ((MODE == MODE_G || MODE == MODE_BK) && p.ragged > 2) {
+              const int nc = nw + 64 * cc;
+              char* o = reinterpret_cast<char*>(dst + g * p.gs_out + (long long)r0 * p.ld_out + nc);
+              const int rows = p.Mg - r0, bytes = 2 * min(p.Ng - nc, 64);
+              auto swz = [](int r) { return r & 7; };
+              if (p.ragged == 8) store_rows<128, 8>(o, 2 * p.ld_out, rows, bytes, xb, lane, swz);
+              else store_rows<128, 4>(o, 2 * p.ld_out, rows, bytes, xb, lane, swz);
+              __syncwarp();
+              continue;
+            }
             if ((MODE == MODE_G || MODE == MODE_BK) && p.ragged) {
               const int nc = nw + 64 * cc + lane;
 #pragma unroll 4
@@ -1120,7 +1130,7 @@ int launch_tc_t(const GemmArgs& a, int dtype, cudaStream_t s, float* ws, size_t 
   // a roughly square block of output tiles and re-reads each operand block about as often as the other
   p.raster = (tune != nullptr && tune->raster > 0) ? tune->raster : (PAIR ? TC_RASTER / 2 : TC_RASTER);
   p.opt = a.opt;
-  p.ragged = a.ragged;
+  p.ragged = !a.ragged ? 0 : MODE == MODE_WD ? 4 : std::min(8, row_alignment(a.out, a.Ng * 2LL));
   p.ws_ld = (a.Ng + 7) / 8 * 8;
   p.ck = a.ck; p.cks = a.cks; p.ld_ck = a.ld_ck;
   // split-K: a weight update with fewer output tiles than half the SMs and a long batch reduction
