@@ -339,15 +339,17 @@ int ipc_mx8_store(const void* x, signed char* codes, unsigned char* scales, int 
 int ipc_mx8_restore(const signed char* codes, const unsigned char* scales, void* out, int D, int B, int act, int dtype,
                     void* stream);
 /*
- * Weight update from a checkpoint of x_up [K, B], A = cast(f(x^)), e [M, B]:
+ * Weight update from a checkpoint of x_up [K, B], A = f(x^), e [M, B]:
  *   IPC_MODE_WEIGHT  W = cast(W + scale * E @ A^T)          (out = W [M, K], in/out)
  *   IPC_MODE_WDELTA  dw = scale * E @ A^T in fp32; IPC_FLAG_ACCUMULATE adds into dw
  *   IPC_MODE_WGRAD   out = cast(scale * E @ A^T) in `dtype`
  * The workspace (16-byte aligned; *_ws_bytes gives its size, which may be 0) need
  * not be initialised; calls that share one must be ordered on one stream.
- * IPC_ALGO_AUTO runs large products on the tcgen05 GEMMs and the rest, of any
- * size and alignment, in one launch of an mma.sync kernel (IPC_ALGO_SIMT asks for
- * it); fp32 storage runs on the generic kernel.  IPC_ALGO_OUTER is IPC_ERR_ARG.
+ * IPC_ALGO_AUTO runs large products on the tcgen05 GEMMs (f(x^) rounded to
+ * `dtype`), a few samples in fp32 FMAs, and the rest, of any size and alignment,
+ * in one launch of an mma.sync kernel that keeps f(x^) in two parts
+ * (IPC_ALGO_SIMT asks for it); fp32 storage otherwise runs on the generic kernel.
+ * IPC_ALGO_OUTER is IPC_ERR_ARG.
  */
 #define IPC_MODE_WGRAD 6
 int ipc_mx8_weight(int mode, void* out, const void* e, const signed char* codes, const unsigned char* scales, int M,
