@@ -518,3 +518,74 @@ def test_call_layer_takes_parameters_and_keywords():
         k(dw.half(), e.to(DEV), c, s)
     with pytest.raises(ValueError):
         k(dw, e, c, s)  # one tensor on the CPU
+
+
+@pytest.mark.parametrize("dt", ALL)
+@pytest.mark.parametrize("M,K,B", [(640, 640, 8), (651, 641, 3), (1000, 520, 1), (300, 2001, 15), (2000, 264, 4),
+                                   (1999, 331, 2), (4096, 136, 1), (77, 5203, 5)])
+def test_products_of_a_few_samples(M, K, B, dt):
+    """Single samples and handfuls at sizes that take the fp32 kernels: whole and ragged rows, a reduction that is split
+    over a cluster, every mode."""
+    mx = _mx()
+    act = ACTS[(M + K + B) % 6]
+    e, c, s, ref, err = _delta_case(M, K, B, dt, act, 40)
+    ed, alpha = e.to(DEV), 0.5
+    dw = torch.full((M, K), 7.0, device=DEV)
+    k = mx.build_weight_delta_checkpoint(M, K, B, act, NAME[dt], alpha)
+    k(dw, ed, c, s)
+    _within(dw, alpha * ref, alpha * err + 2.0 ** -23 * alpha * ref.abs())
+    k(dw, ed, c, s, accumulate=True)
+    _within(dw, 2 * alpha * ref, 2 * alpha * err + 2.0 ** -22 * 2 * alpha * ref.abs())
+    if dt is not torch.float32:
+        g = torch.full((M, K), 7.0, device=DEV, dtype=dt)
+        mx.build_weight_delta_checkpoint(M, K, B, act, NAME[dt], alpha, NAME[dt])(g, ed, c, s)
+        _within(g, alpha * ref, (alpha * err) * (1 + U[dt]) + U[dt] * alpha * ref.abs() + TINY[dt])
+    w0 = _rand((M, K), 42, 0.05, dt)
+    w = w0.to(DEV)
+    mx.build_weight_update_checkpoint(M, K, B, act, NAME[dt], 0.01)(w, ed, c, s)
+    want = w0.double() + 0.01 * ref
+    _within(w, want, (0.01 * err) * (1 + U[dt]) + (U[dt] + 2.0 ** -22) * (want.abs() + 0.01 * ref.abs()) + TINY[dt])
+    xhat = X.load8(c.cpu(), s.cpu(), B)
+    acc, S = w0.double().t() @ e.double(), w0.double().abs().t() @ e.double().abs()
+    rb = X.backward(w0, e, xhat, act)
+    tol = _slope_err(act, xhat, dt) * (acc.abs() + S * M * 2.0 ** -23) + X.slope(act, xhat).abs() * S * M * 2.0 ** -23
+    outs = []
+    for shift in (0, 1):  # W on and off a boundary of two elements
+        flat = torch.zeros(M * K + 1, device=DEV, dtype=dt)
+        flat[shift:shift + M * K] = w0.reshape(-1).to(DEV)
+        up = torch.full((K, B), 7.0, device=DEV, dtype=dt)
+        mx.build_error_backward_checkpoint(M, K, B, act, NAME[dt])(flat[shift:shift + M * K].view(M, K), ed, c, s, up)
+        _within(up, rb, tol * (1 + U[dt]) + (U[dt] + 2.0 ** -23) * rb.abs() + TINY[dt])
+        outs.append(up)
+    again = torch.full((K, B), 7.0, device=DEV, dtype=dt)
+    mx.build_error_backward_checkpoint(M, K, B, act, NAME[dt])(w0.to(DEV), ed, c, s, again)
+    assert torch.equal(again, outs[0])
+
+
+@pytest.mark.parametrize("M,K,B", [(2048, 2048, 100), (700, 1004, 612), (900, 902, 514), (1001, 903, 501)])
+def test_products_of_large_ragged_rows(M, K, B):
+    """Rows on boundaries of 8, 4 and 2 bytes at sizes that take the tensor cores by themselves."""
+    mx = _mx()
+    dt = torch.bfloat16
+    e, c, s, ref, err = _delta_case(M, K, B, dt, "silu", 50)
+    ed, alpha = e.to(DEV), 1.0 / B
+    for name in ("float32", "bfloat16"):
+        out = torch.full((M, K), 7.0, device=DEV, dtype=getattr(torch, name))
+        mx.build_weight_delta_checkpoint(M, K, B, "silu", "bfloat16", alpha, name)(out, ed, c, s)
+        u = U[out.dtype] + 2.0 ** -23
+        _within(out, alpha * ref, (alpha * err) * (1 + u) + u * alpha * ref.abs() + TINY[out.dtype])
+    w0 = _rand((M, K), 52, 0.05, dt)
+    xhat = X.load8(c.cpu(), s.cpu(), B)
+    acc, S = w0.double().t() @ e.double(), w0.double().abs().t() @ e.double().abs()
+    rb = X.backward(w0, e, xhat, "silu")
+    tol = _slope_err("silu", xhat, dt) * (acc.abs() + S * M * 2.0 ** -23) + X.slope("silu", xhat).abs() * S * M * 2.0 ** -23
+    up = torch.full((K, B), 7.0, device=DEV, dtype=dt)
+    mx.build_error_backward_checkpoint(M, K, B, "silu", "bfloat16")(w0.to(DEV), ed, c, s, up)
+    _within(up, rb, tol * (1 + U[dt]) + (U[dt] + 2.0 ** -23) * rb.abs() + TINY[dt])
+    wv, wq, wsc = X.quant4(_rand((M, K), 53, K ** -0.5))
+    av, aq, asc = X.quant4(_rand((B, K), 54))
+    for odt in ALL:
+        out = torch.full((M, B), 9.0, device=DEV, dtype=odt)
+        mx.build_mxfp4_forward(M, K, B, NAME[odt])(wq.to(DEV), wsc.to(DEV), aq.to(DEV), asc.to(DEV), out)
+        r4 = wv @ av.t()
+        _within(out, r4, (wv.abs() @ av.abs().t()) * K * 2.0 ** -23 + U[odt] * r4.abs() * (1 + 2.0 ** -8) + TINY[odt])
