@@ -71,6 +71,10 @@ PyObject* call(PyObject* self, PyObject* const* args, size_t nargsf, PyObject* k
   }
   if (!plain || device != (int)c10::cuda::current_device()) return PyObject_Vectorcall(c->op, args, nargsf, kwnames);
   cudaStream_t s = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)device).stream();
+  // The workspace this call launches with.  All threads share the object, and one on another stream may replace what it
+  // remembers as soon as this thread gives up the interpreter lock: nothing of *c that changes is read after that.
+  void* ws = c->ws;
+  size_t ws_bytes = c->ws_bytes;
   if ((c->kind == WEIGHT || c->kind == BACKWARD) && (c->ws_device != device || c->ws_stream != s)) {
     PyObject* r = PyObject_CallMethod(c->op, "_workspace", "iK", device, (unsigned long long)(uintptr_t)s);
     if (r == nullptr) return nullptr;
@@ -78,8 +82,8 @@ PyObject* call(PyObject* self, PyObject* const* args, size_t nargsf, PyObject* k
     PyObject* at = nullptr;
     const int ok = PyArg_ParseTuple(r, "OK", &at, &bytes);
     if (ok) {
-      c->ws = at == Py_None ? nullptr : reinterpret_cast<void*>((uintptr_t)PyLong_AsUnsignedLongLong(at));
-      c->ws_bytes = (size_t)bytes;
+      c->ws = ws = at == Py_None ? nullptr : reinterpret_cast<void*>((uintptr_t)PyLong_AsUnsignedLongLong(at));
+      c->ws_bytes = ws_bytes = (size_t)bytes;
       c->ws_device = device;
       c->ws_stream = s;
     }
@@ -100,11 +104,11 @@ PyObject* call(PyObject* self, PyObject* const* args, size_t nargsf, PyObject* k
       break;
     case WEIGHT:
       rc = reinterpret_cast<decltype(&ipc_mx8_weight)>(c->fn)(v[0], p[0], p[1], i8(2), u8(3), v[1], v[2], v[3], c->alpha, 0,
-                                                              v[4], v[5], v[6], c->ws, c->ws_bytes, s);
+                                                              v[4], v[5], v[6], ws, ws_bytes, s);
       break;
     case BACKWARD:
       rc = reinterpret_cast<decltype(&ipc_mx8_backward)>(c->fn)(p[4], p[0], p[1], i8(2), u8(3), v[0], v[1], v[2], v[3],
-                                                                v[4], v[5], c->ws, c->ws_bytes, s);
+                                                                v[4], v[5], ws, ws_bytes, s);
       break;
     case QUANTIZE:
       rc = reinterpret_cast<decltype(&ipc_mxfp4_quantize)>(c->fn)(p[0], u8(1), u8(2), v[0], v[1], v[2], v[3], v[4], s);

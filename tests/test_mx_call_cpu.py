@@ -1,0 +1,96 @@
+"""The C++ call layer of the microscaled operators (``csrc/mx_call.cpp``) on the CPU: the file itself, with its device
+queries turned to the host (``mx_call_host.cpp``), around Python operators and C entries of the tests' own."""
+import ctypes
+import importlib.machinery
+import importlib.util
+import os
+import subprocess
+import sysconfig
+import threading
+from pathlib import Path
+
+import pytest
+import torch
+
+HERE = Path(__file__).resolve().parent
+
+
+@pytest.fixture(scope="module")
+def call_path(tmp_path_factory):
+    from lich_b200 import build
+    so = tmp_path_factory.mktemp("mx_call") / "_mx_call.so"
+    inc, libs = Path(torch.__file__).parent / "include", Path(torch.__file__).parent / "lib"
+    cuda = Path(build.nvcc()).resolve().parents[1] / "include"
+    subprocess.run([os.environ.get("CXX", "g++"), "-O0", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+                    f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+                    "-I", sysconfig.get_paths()["include"], "-isystem", str(inc), "-isystem",
+                    str(inc / "torch" / "csrc" / "api" / "include"), "-isystem", str(cuda),
+                    str(HERE / "mx_call_host.cpp"), "-o", str(so), f"-L{libs}", f"-Wl,-rpath,{libs}",
+                    "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"], check=True)
+    return so
+
+
+def _load(path):
+    loader = importlib.machinery.ExtensionFileLoader("_mx_call", str(path))
+    module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_mx_call", loader))
+    loader.exec_module(module)
+    return module.Call
+
+
+@pytest.fixture(scope="module")
+def Call(call_path):
+    return _load(call_path)
+
+
+# the C entry of a weight product: (mode, out, e, codes, scales, M, K, B, scale, flags, act, dtype, algo, ws, bytes, stream)
+ENTRY = ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_int, *[ctypes.c_void_p] * 4, *[ctypes.c_int] * 3, ctypes.c_float,
+                         *[ctypes.c_int] * 4, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p)
+
+
+def _weight_call(Call, entry, workspace):
+    """A weight product of 2 x 3 from 32 samples whose Python operator gives out ``workspace(device, stream)``."""
+    class Op:
+        def _workspace(self, device, stream):
+            return workspace(device, stream)
+
+        def _failed(self, rc):
+            raise RuntimeError(f"entry returned {rc}")
+
+        def __call__(self, *args, **kw):
+            raise ValueError("handed back")
+
+    f32 = torch.float32
+    spec = [(torch.Size((2, 3)), f32), (torch.Size((2, 32)), f32), (torch.Size((3, 32)), torch.int8),
+            (torch.Size((1, 3)), torch.uint8)]
+    call = Call(Op(), 2, ctypes.cast(entry, ctypes.c_void_p).value, spec, (3, 2, 3, 32, 0, 0, 0), 1.0)
+    return call, tuple(torch.zeros(s, dtype=d) for s, d in spec)
+
+
+def test_threads_on_two_streams_keep_to_their_own_workspaces(Call):
+    """One operator is shared by all threads.  Each has its own stream here, and each stream its workspace; while a thread
+    is in the C entry's call without the interpreter lock, another one takes its turn."""
+    seen, owner = [], {}
+
+    @ENTRY
+    def entry(mode, out, e, codes, scales, M, K, B, scale, flags, act, dtype, algo, ws, n, stream):
+        seen.append((ws, n, stream))
+        return 0
+
+    def workspace(device, stream):
+        buf = owner.setdefault(stream, torch.empty(64 * (1 + len(owner)), dtype=torch.uint8))
+        return buf.data_ptr(), buf.numel()
+
+    call, args = _weight_call(Call, entry, workspace)
+    gate = threading.Barrier(2)
+
+    def run():
+        gate.wait()
+        for _ in range(40):
+            call(*args)
+
+    threads = [threading.Thread(target=run) for _ in range(2)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert len(seen) == 80 and len(owner) == 2
+    for ws, n, stream in seen:
+        assert (ws, n) == (owner[stream].data_ptr(), owner[stream].numel())
