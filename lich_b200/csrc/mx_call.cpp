@@ -58,19 +58,27 @@ PyObject* call(PyObject* self, PyObject* const* args, size_t nargsf, PyObject* k
   const int n = kTensors[c->kind];
   void* p[kMost] = {};
   int device = -1;
+  cudaStream_t s = nullptr;
   bool plain = PyVectorcall_NARGS(nargsf) == n && (kwnames == nullptr || PyTuple_GET_SIZE(kwnames) == 0);
-  for (int i = 0; plain && i < n; ++i) {
-    if (!THPVariable_CheckExact(args[i])) {
-      plain = false;
-      break;
+  // Nothing may leave a C function by a C++ exception, and torch throws at tensors without storage of their own (torch.vmap,
+  // torch.func), at layouts that are not dense and at errors of the device: the Python operator, which meets the same, raises.
+  try {
+    for (int i = 0; plain && i < n; ++i) {
+      if (!THPVariable_CheckExact(args[i])) {
+        plain = false;
+        break;
+      }
+      const at::Tensor& t = THPVariable_Unpack(args[i]);
+      if (i == 0) device = t.is_cuda() ? (int)t.get_device() : -1;
+      plain = device >= 0 && fits(t, c->spec[i], device);
+      if (plain) p[i] = t.data_ptr();
     }
-    const at::Tensor& t = THPVariable_Unpack(args[i]);
-    if (i == 0) device = t.is_cuda() ? (int)t.get_device() : -1;
-    plain = device >= 0 && fits(t, c->spec[i], device);
-    if (plain) p[i] = t.data_ptr();
+    plain = plain && device == (int)c10::cuda::current_device();
+    if (plain) s = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)device).stream();
+  } catch (...) {
+    plain = false;
   }
-  if (!plain || device != (int)c10::cuda::current_device()) return PyObject_Vectorcall(c->op, args, nargsf, kwnames);
-  cudaStream_t s = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)device).stream();
+  if (!plain) return PyObject_Vectorcall(c->op, args, nargsf, kwnames);
   // The workspace this call launches with.  All threads share the object, and one on another stream may replace what it
   // remembers as soon as this thread gives up the interpreter lock: nothing of *c that changes is read after that.
   void* ws = c->ws;
@@ -156,8 +164,12 @@ PyObject* make(PyTypeObject* type, PyObject* args, PyObject*) {
       break;
     }
     c->spec[i].dtype = reinterpret_cast<THPDtype*>(dtype)->scalar_type;
-    for (Py_ssize_t d = 0; d < PyTuple_GET_SIZE(shape); ++d)
-      c->spec[i].shape.push_back(PyLong_AsLongLong(PyTuple_GET_ITEM(shape, d)));
+    try {
+      for (Py_ssize_t d = 0; d < PyTuple_GET_SIZE(shape); ++d)
+        c->spec[i].shape.push_back(PyLong_AsLongLong(PyTuple_GET_ITEM(shape, d)));
+    } catch (const std::bad_alloc&) {
+      PyErr_NoMemory();
+    }
   }
   if (PyErr_Occurred()) {
     Py_DECREF(c);

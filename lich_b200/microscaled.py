@@ -109,7 +109,7 @@ class _MxOp:
             else:
                 if dev >= 0:
                     return _current_stream(dev) if dev == _current_device() else None
-        except AttributeError:
+        except (AttributeError, RuntimeError):  # not a tensor; one that cannot be asked for its device or strides
             pass
         raise ValueError(self._refusal(tensors))
 
@@ -127,6 +127,8 @@ class _MxOp:
                 return f"{self.kind}: argument {i} is {t.dtype}, kernel was built for {dtype}"
             if not t.is_cuda:
                 return f"{self.kind}: argument {i} is not a CUDA tensor"
+            if t.layout is not torch.strided:
+                return f"{self.kind}: argument {i} is {t.layout}, not a dense tensor"
             if not t.is_contiguous():
                 return f"{self.kind}: argument {i} is not contiguous"
         return f"{self.kind}: tensors on different devices"

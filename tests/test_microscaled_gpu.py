@@ -589,3 +589,17 @@ def test_products_of_large_ragged_rows(M, K, B):
         mx.build_mxfp4_forward(M, K, B, NAME[odt])(wq.to(DEV), wsc.to(DEV), aq.to(DEV), asc.to(DEV), out)
         r4 = wv @ av.t()
         _within(out, r4, (wv.abs() @ av.abs().t()) * K * 2.0 ** -23 + U[odt] * r4.abs() * (1 + 2.0 ** -8) + TINY[odt])
+
+
+def test_tensors_without_an_address_are_refused():
+    """Under torch.vmap a tensor passes for a plain one and throws when asked for its address; a sparse one has no strides."""
+    mx = _mx()
+    c, s = mx.empty_checkpoint(4, 40, device=DEV)
+    k = mx.build_checkpoint(4, 40, "float16")
+    x = torch.zeros(3, 4, 40, device=DEV, dtype=torch.float16)
+    with pytest.raises(RuntimeError):
+        torch.vmap(lambda t: k(t, c, s))(x)
+    with pytest.raises(ValueError, match="not a dense tensor"):
+        k(x[0].to_sparse(), c, s)
+    k(x[0], c, s)
+    assert not c.any()

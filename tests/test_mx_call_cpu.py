@@ -5,6 +5,7 @@ import importlib.machinery
 import importlib.util
 import os
 import subprocess
+import sys
 import sysconfig
 import threading
 from pathlib import Path
@@ -94,3 +95,38 @@ def test_threads_on_two_streams_keep_to_their_own_workspaces(Call):
     assert len(seen) == 80 and len(owner) == 2
     for ws, n, stream in seen:
         assert (ws, n) == (owner[stream].data_ptr(), owner[stream].numel())
+
+
+ABORTS = """
+import sys
+sys.path[:0] = {path!r}
+import torch
+from test_mx_call_cpu import ENTRY, _load, _weight_call
+
+@ENTRY
+def entry(*args):
+    return 0
+
+call, args = _weight_call(_load({so!r}), entry, lambda device, stream: (None, 0))
+assert call(*args) is None
+out, e, codes, scales = args
+batched = torch.zeros(5, 2, 32)
+for case in (lambda: torch.vmap(lambda t: call(out, t, codes, scales))(batched),   # no storage of its own
+             lambda: torch.func.grad(lambda t: (call(out, t, codes, scales), t.sum())[1])(e),
+             lambda: call(out, e.to_sparse(), codes, scales)):                   # no dense layout to ask for
+    try:
+        case()
+    except ValueError as exc:
+        assert "handed back" in str(exc), exc
+        print("refused")
+"""
+
+
+def test_what_throws_in_the_call_goes_to_the_operator(call_path):
+    """Tensors under torch.vmap or torch.func have the type and the shape that the call asks for and throw when asked for
+    their address, sparse ones when asked for their layout.  In a process of its own: an exception that leaves a C
+    function ends it."""
+    code = ABORTS.format(path=[str(HERE), str(HERE.parent)], so=str(call_path))
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
+    assert r.stdout.split() == ["refused"] * 3
