@@ -40,11 +40,12 @@ struct Call {
   int v[8];      // the entry's integer arguments
   float alpha;
   Spec* spec;
-  // the workspace of the last stream it ran on (WEIGHT, BACKWARD); the operator owns it
+  // the workspace of the last stream it ran on (WEIGHT, BACKWARD), and what owns that memory
   int ws_device;
   cudaStream_t ws_stream;
   void* ws;
   size_t ws_bytes;
+  PyObject* ws_owner;
 };
 
 bool fits(const at::Tensor& t, const Spec& s, int device) {
@@ -87,13 +88,15 @@ PyObject* call(PyObject* self, PyObject* const* args, size_t nargsf, PyObject* k
     PyObject* r = PyObject_CallMethod(c->op, "_workspace", "iK", device, (unsigned long long)(uintptr_t)s);
     if (r == nullptr) return nullptr;
     unsigned long long bytes = 0;
-    PyObject* at = nullptr;
-    const int ok = PyArg_ParseTuple(r, "OK", &at, &bytes);
+    PyObject *at = nullptr, *owner = nullptr;
+    const int ok = PyArg_ParseTuple(r, "OK|O", &at, &bytes, &owner);
     if (ok) {
       c->ws = ws = at == Py_None ? nullptr : reinterpret_cast<void*>((uintptr_t)PyLong_AsUnsignedLongLong(at));
       c->ws_bytes = ws_bytes = (size_t)bytes;
       c->ws_device = device;
       c->ws_stream = s;
+      Py_XINCREF(owner);
+      Py_XSETREF(c->ws_owner, owner);
     }
     Py_DECREF(r);
     if (!ok || PyErr_Occurred()) return nullptr;
@@ -183,6 +186,7 @@ PyObject* make(PyTypeObject* type, PyObject* args, PyObject*) {
 void drop(PyObject* self) {
   Call* c = reinterpret_cast<Call*>(self);
   delete[] c->spec;
+  Py_XDECREF(c->ws_owner);
   Py_XDECREF(c->op);
   Py_TYPE(self)->tp_free(self);
 }

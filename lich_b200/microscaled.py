@@ -26,6 +26,7 @@ from __future__ import annotations
 
 import importlib.machinery
 import importlib.util
+import threading
 from ctypes import byref, c_size_t, c_void_p, cast
 from functools import lru_cache, wraps
 
@@ -49,6 +50,7 @@ def _load_call():
 
 
 _Call = _load_call().Call
+_ws_lock = threading.Lock()
 
 BLOCK = 32
 # what torch.cuda.current_device() and current_stream().cuda_stream come down to, at a tenth of their cost
@@ -134,15 +136,19 @@ class _MxOp:
         return f"{self.kind}: tensors on different devices"
 
     def _workspace(self, dev: int, stream: int):
-        """(address, bytes) of this operator's workspace for one stream of a device: calls on two streams may overlap."""
+        """(address, bytes, owner) of this operator's workspace for one stream of a device: calls on two streams may
+        overlap.  One per stream whichever threads ask first; the memory lives as long as ``owner`` is held."""
         ws = self._ws.get((dev, stream))
         if ws is None:
-            n = c_size_t(0)
-            with torch.cuda.device(dev):
-                N.check(self._ws_bytes(byref(n)))
-                buf = torch.empty(int(n.value), device=f"cuda:{dev}", dtype=torch.uint8) if n.value else None
-            ws = self._ws[dev, stream] = (None if buf is None else buf.data_ptr(), int(n.value), buf)
-        return ws[:2]
+            with _ws_lock:
+                ws = self._ws.get((dev, stream))
+                if ws is None:
+                    n = c_size_t(0)
+                    with torch.cuda.device(dev):
+                        N.check(self._ws_bytes(byref(n)))
+                        buf = torch.empty(int(n.value), device=f"cuda:{dev}", dtype=torch.uint8) if n.value else None
+                    ws = self._ws[dev, stream] = (None if buf is None else buf.data_ptr(), int(n.value), buf)
+        return ws
 
     def get_kernel_source(self) -> str:
         return f"lich_b200 {self.kind} {self.spec} (prebuilt sm_100a kernel, include/ipc_b200.h)"
@@ -204,7 +210,7 @@ class CheckpointWeightKernel(_MxOp):
             raise ValueError(f"{self.kind}: only a weight delta in float32 accumulates")
         if s is None:
             return self._elsewhere(out, e, codes, scales, accumulate=accumulate)
-        ws, n = self._workspace(out.get_device(), s)
+        ws, n, _ = self._workspace(out.get_device(), s)
         rc = self._fn(self.mode, out.data_ptr(), e.data_ptr(), codes.data_ptr(), scales.data_ptr(), self.M, self.K, self.B,
                       self.alpha, N.FLAG_ACCUMULATE if accumulate else 0, self.act, self.dt, self.algo, ws, n, s)
         if rc:
@@ -230,7 +236,7 @@ class CheckpointBackwardKernel(_MxOp):
         s = self._stream((w, e, codes, scales, e_up))
         if s is None:
             return self._elsewhere(w, e, codes, scales, e_up)
-        ws, n = self._workspace(w.get_device(), s)
+        ws, n, _ = self._workspace(w.get_device(), s)
         rc = self._fn(e_up.data_ptr(), w.data_ptr(), e.data_ptr(), codes.data_ptr(), scales.data_ptr(), self.M, self.K,
                       self.B, self.act, self.dt, self.algo, ws, n, s)
         if rc:

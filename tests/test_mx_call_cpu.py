@@ -1,5 +1,6 @@
 """The C++ call layer of the microscaled operators (``csrc/mx_call.cpp``) on the CPU: the file itself, with its device
 queries turned to the host (``mx_call_host.cpp``), around Python operators and C entries of the tests' own."""
+import contextlib
 import ctypes
 import importlib.machinery
 import importlib.util
@@ -8,6 +9,8 @@ import subprocess
 import sys
 import sysconfig
 import threading
+import time
+import weakref
 from pathlib import Path
 
 import pytest
@@ -130,3 +133,72 @@ def test_what_throws_in_the_call_goes_to_the_operator(call_path):
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, r.stderr[-2000:]
     assert r.stdout.split() == ["refused"] * 3
+
+
+class _Owner:
+    pass
+
+
+def test_the_call_holds_the_workspace_that_it_remembers(Call):
+    """The address is used for every later call on the stream, so what owns the memory has to live as long, whatever the
+    operator's own table holds by then."""
+    seen, owners = [], []
+
+    @ENTRY
+    def entry(mode, out, e, codes, scales, M, K, B, scale, flags, act, dtype, algo, ws, n, stream):
+        seen.append(ws)
+        return 0
+
+    def workspace(device, stream):
+        owner = _Owner()
+        owners.append(weakref.ref(owner))
+        return 4096, 64, owner
+
+    call, args = _weight_call(Call, entry, workspace)
+    call(*args)
+    assert owners[0]() is not None
+    call(*args)
+    assert len(owners) == 1 and seen == [4096, 4096]
+    t = threading.Thread(target=call, args=args)  # another stream: the first one's memory is let go
+    t.start(), t.join()
+    assert len(owners) == 2 and owners[0]() is None and owners[1]() is not None
+    del call
+    assert owners[1]() is None
+
+
+def _no_gpu(monkeypatch, made):
+    """Workspaces of ``lich_b200.microscaled`` in CPU memory; making one takes its time and lets other threads run."""
+    from lich_b200 import microscaled as mx
+    real = torch.empty
+
+    def empty(n, **kw):
+        time.sleep(0.05)
+        made.append(real(n, dtype=torch.uint8))
+        return made[-1]
+
+    def ws_bytes(self, n):
+        n._obj.value = self.M * 256
+        return 0
+
+    monkeypatch.setattr(mx.torch.cuda, "device", lambda dev: contextlib.nullcontext())
+    monkeypatch.setattr(mx.torch, "empty", empty)
+    monkeypatch.setattr(mx.CheckpointWeightKernel, "_ws_bytes", ws_bytes)
+    return mx
+
+
+def test_threads_that_meet_at_the_first_call_get_one_workspace(monkeypatch):
+    made, got = [], []
+    mx = _no_gpu(monkeypatch, made)
+    k = mx.build_weight_delta_checkpoint(11, 13, 64, "tanh", "bfloat16", 0.125)
+    gate = threading.Barrier(4)
+
+    def first():
+        gate.wait()
+        got.append(k._workspace(0, 7))
+
+    threads = [threading.Thread(target=first) for _ in range(4)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert len(made) == 1 and len({g[0] for g in got}) == 1 and got[0][1] == 11 * 256
+    assert got[0][0] == made[0].data_ptr()
+    assert k._workspace(0, 8)[0] != got[0][0] and len(made) == 2  # another stream
