@@ -27,6 +27,7 @@ from __future__ import annotations
 import importlib.machinery
 import importlib.util
 import threading
+import weakref
 from ctypes import byref, c_size_t, c_void_p, cast
 from functools import lru_cache, wraps
 
@@ -50,6 +51,18 @@ def _load_call():
 
 
 _Call = _load_call().Call
+
+
+class _Scratch:
+    """Device memory that operators share, freed when the last one that holds it goes."""
+
+    def __init__(self, n: int, device):
+        self.bytes = n
+        self._buf = torch.empty(n, device=device, dtype=torch.uint8) if n else None
+        self.address = None if self._buf is None else self._buf.data_ptr()
+
+
+_scratch: weakref.WeakValueDictionary = weakref.WeakValueDictionary()
 _ws_lock = threading.Lock()
 
 BLOCK = 32
@@ -135,20 +148,27 @@ class _MxOp:
                 return f"{self.kind}: argument {i} is not contiguous"
         return f"{self.kind}: tensors on different devices"
 
+    def _ws_key(self) -> tuple:
+        """What the size of the workspace depends on."""
+        raise NotImplementedError
+
     def _workspace(self, dev: int, stream: int):
-        """(address, bytes, owner) of this operator's workspace for one stream of a device: calls on two streams may
-        overlap.  One per stream whichever threads ask first; the memory lives as long as ``owner`` is held."""
+        """(address, bytes, owner) of the workspace for one stream of a device: calls on two streams may overlap.
+        Operators that differ in what the workspace does not depend on (the factor alpha) share it.  One per stream
+        whichever threads ask first; the memory lives as long as an ``owner`` is held, which each operator does."""
         ws = self._ws.get((dev, stream))
         if ws is None:
             with _ws_lock:
-                ws = self._ws.get((dev, stream))
+                key = self._ws_key() + (dev, stream)
+                ws = _scratch.get(key)
                 if ws is None:
                     n = c_size_t(0)
                     with torch.cuda.device(dev):
                         N.check(self._ws_bytes(byref(n)))
-                        buf = torch.empty(int(n.value), device=f"cuda:{dev}", dtype=torch.uint8) if n.value else None
-                    ws = self._ws[dev, stream] = (None if buf is None else buf.data_ptr(), int(n.value), buf)
-        return ws
+                        ws = _Scratch(int(n.value), f"cuda:{dev}")
+                    _scratch[key] = ws
+                self._ws[dev, stream] = ws
+        return ws.address, ws.bytes, ws
 
     def get_kernel_source(self) -> str:
         return f"lich_b200 {self.kind} {self.spec} (prebuilt sm_100a kernel, include/ipc_b200.h)"
@@ -201,6 +221,9 @@ class CheckpointWeightKernel(_MxOp):
         self.mode, self.M, self.K, self.B = mode, int(M), int(K), int(B)
         self.act, self.dt, self.alpha, self.algo = N.act_code(activation), N.dtype_code(dtype), float(alpha), _algo(cfg)
 
+    def _ws_key(self) -> tuple:
+        return "weight", self.mode, self.M, self.K, self.B, self.dt, self.algo
+
     def _ws_bytes(self, n) -> int:
         return N.load().ipc_mx8_weight_ws_bytes(self.mode, self.M, self.K, self.B, self.dt, self.algo, n)
 
@@ -228,6 +251,9 @@ class CheckpointBackwardKernel(_MxOp):
                          [((M, K), dt), ((M, B), dt), (c, torch.int8), (s, torch.uint8), ((K, B), dt)])
         self.M, self.K, self.B = int(M), int(K), int(B)
         self.act, self.dt, self.algo = N.act_code(activation), N.dtype_code(dtype), _algo(cfg)
+
+    def _ws_key(self) -> tuple:
+        return "backward", self.M, self.K, self.B, self.dt, self.algo
 
     def _ws_bytes(self, n) -> int:
         return N.load().ipc_mx8_backward_ws_bytes(self.M, self.K, self.B, self.dt, self.algo, n)

@@ -2,6 +2,7 @@
 queries turned to the host (``mx_call_host.cpp``), around Python operators and C entries of the tests' own."""
 import contextlib
 import ctypes
+import gc
 import importlib.machinery
 import importlib.util
 import os
@@ -202,3 +203,21 @@ def test_threads_that_meet_at_the_first_call_get_one_workspace(monkeypatch):
     assert len(made) == 1 and len({g[0] for g in got}) == 1 and got[0][1] == 11 * 256
     assert got[0][0] == made[0].data_ptr()
     assert k._workspace(0, 8)[0] != got[0][0] and len(made) == 2  # another stream
+
+
+def test_operators_that_differ_in_the_factor_share_a_workspace(monkeypatch):
+    """alpha is an argument of the launch: a schedule that changes it every step makes operators, not workspaces, and the
+    memory goes when the last operator of its shape does."""
+    made = []
+    mx = _no_gpu(monkeypatch, made)
+    ops = [mx.CheckpointWeightKernel(0, 17, 19, 64, "tanh", "bfloat16", 0.1 / (1 + i), torch.bfloat16, mx.KernelConfig())
+           for i in range(5)]
+    assert len({op._workspace(0, 7)[0] for op in ops}) == 1 and len(made) == 1
+    other = mx.CheckpointWeightKernel(0, 23, 19, 64, "tanh", "bfloat16", 0.1, torch.bfloat16, mx.KernelConfig())
+    assert other._workspace(0, 7)[0] != ops[0]._workspace(0, 7)[0] and len(made) == 2
+    held = len(mx._scratch)
+    op, ops = ops[-1], None
+    assert op._workspace(0, 7)[0] == made[0].data_ptr() and len(mx._scratch) == held
+    op = None
+    gc.collect()
+    assert len(mx._scratch) == held - 1
