@@ -4,8 +4,9 @@ with their product.
 Blocks of 32 numbers share one power of two (formats and layouts: ``include/ipc_b200.h``).  Like the builders of
 ``lich_b200.tilelang_kernels`` each ``build_*`` returns a cached callable specialised for its shape, activation and
 dtype that writes its output tensors in place on the current CUDA stream, raises ``ValueError`` for tensors of another
-shape, dtype, device or layout before anything is launched, and owns (per device and stream) whatever workspace it
-needs.
+shape, dtype, device or layout before anything is launched, and holds (per device and stream) whatever workspace it
+needs.  Large products with a checkpoint need one of the size of the states in 16 bits; a program that runs many of them in
+order passes one buffer of its own instead: ``kernel(..., workspace=buffer)``, ``kernel.workspace_bytes()`` long.
 
     codes, scales = empty_checkpoint(D, B, device=dev)                       # states x [D, B] kept in 8 bits
     build_checkpoint(D, B, "bfloat16")(x, codes, scales)
@@ -104,6 +105,7 @@ class _MxOp:
         self.spec = tuple((torch.Size(s), d) for s, d in spec)
         self._fn = getattr(N.load(), entry)
         self._ws: dict = {}
+        self._need: int | None = None
 
     def fast(self):
         """This operator as a C++ callable, which comes back here for everything but a plain call."""
@@ -162,13 +164,31 @@ class _MxOp:
                 key = self._ws_key() + (dev, stream)
                 ws = _scratch.get(key)
                 if ws is None:
-                    n = c_size_t(0)
                     with torch.cuda.device(dev):
-                        N.check(self._ws_bytes(byref(n)))
-                        ws = _Scratch(int(n.value), f"cuda:{dev}")
+                        ws = _Scratch(self.workspace_bytes(), f"cuda:{dev}")
                     _scratch[key] = ws
                 self._ws[dev, stream] = ws
         return ws.address, ws.bytes, ws
+
+    def workspace_bytes(self) -> int:
+        """Bytes of workspace a call needs (0 for most small shapes)."""
+        if self._need is None:
+            n = c_size_t(0)
+            N.check(self._ws_bytes(byref(n)))
+            self._need = int(n.value)
+        return self._need
+
+    def _given(self, workspace, dev: int):
+        """(address, bytes) of a caller's workspace, after checking it."""
+        if not isinstance(workspace, torch.Tensor) or not workspace.is_cuda or workspace.get_device() != dev:
+            raise ValueError(f"{self.kind}: the workspace is no tensor on the operands' device")
+        if not workspace.is_contiguous():
+            raise ValueError(f"{self.kind}: the workspace is not contiguous")
+        n, need = workspace.numel() * workspace.element_size(), self.workspace_bytes()
+        if n < need or workspace.data_ptr() % 16:
+            raise ValueError(f"{self.kind}: a workspace of {n} bytes at {workspace.data_ptr():#x}, {need} bytes needed on a "
+                             "16-byte boundary")
+        return workspace.data_ptr(), n
 
     def get_kernel_source(self) -> str:
         return f"lich_b200 {self.kind} {self.spec} (prebuilt sm_100a kernel, include/ipc_b200.h)"
@@ -227,13 +247,14 @@ class CheckpointWeightKernel(_MxOp):
     def _ws_bytes(self, n) -> int:
         return N.load().ipc_mx8_weight_ws_bytes(self.mode, self.M, self.K, self.B, self.dt, self.algo, n)
 
-    def __call__(self, out, e, codes, scales, *, accumulate: bool = False):
+    def __call__(self, out, e, codes, scales, *, accumulate: bool = False, workspace=None):
         s = self._stream((out, e, codes, scales))
         if accumulate and self.mode != N.MODE_WDELTA:
             raise ValueError(f"{self.kind}: only a weight delta in float32 accumulates")
         if s is None:
-            return self._elsewhere(out, e, codes, scales, accumulate=accumulate)
-        ws, n, _ = self._workspace(out.get_device(), s)
+            return self._elsewhere(out, e, codes, scales, accumulate=accumulate, workspace=workspace)
+        dev = out.get_device()
+        ws, n = self._workspace(dev, s)[:2] if workspace is None else self._given(workspace, dev)
         rc = self._fn(self.mode, out.data_ptr(), e.data_ptr(), codes.data_ptr(), scales.data_ptr(), self.M, self.K, self.B,
                       self.alpha, N.FLAG_ACCUMULATE if accumulate else 0, self.act, self.dt, self.algo, ws, n, s)
         if rc:
@@ -258,11 +279,12 @@ class CheckpointBackwardKernel(_MxOp):
     def _ws_bytes(self, n) -> int:
         return N.load().ipc_mx8_backward_ws_bytes(self.M, self.K, self.B, self.dt, self.algo, n)
 
-    def __call__(self, w, e, codes, scales, e_up):
+    def __call__(self, w, e, codes, scales, e_up, *, workspace=None):
         s = self._stream((w, e, codes, scales, e_up))
         if s is None:
-            return self._elsewhere(w, e, codes, scales, e_up)
-        ws, n, _ = self._workspace(w.get_device(), s)
+            return self._elsewhere(w, e, codes, scales, e_up, workspace=workspace)
+        dev = w.get_device()
+        ws, n = self._workspace(dev, s)[:2] if workspace is None else self._given(workspace, dev)
         rc = self._fn(e_up.data_ptr(), w.data_ptr(), e.data_ptr(), codes.data_ptr(), scales.data_ptr(), self.M, self.K,
                       self.B, self.act, self.dt, self.algo, ws, n, s)
         if rc:

@@ -100,11 +100,24 @@ class _FusedOp:
         workspace per stream: calls of one (cached) operator on two streams may overlap."""
         key = (dev, N.stream_handle(dev), mode, flags)
         if key not in self._ws:
-            with torch.cuda.device(dev):
-                n = N.workspace_bytes(mode, M=self.M, K=self.K, B=self.B, groups=self.groups, flags=flags,
-                                      dtype=self.torch_dtype, algo=str(getattr(self.cfg, "backend", "auto")).lower())
+            n = self._workspace_need(dev, mode, flags)
             self._ws[key] = torch.empty((n + 15) // 16 * 4, device=dev, dtype=torch.float32) if n > 0 else None
         return self._ws[key]
+
+    def _workspace_need(self, dev: torch.device, mode: int, flags: int) -> int:
+        with torch.cuda.device(dev):
+            return N.workspace_bytes(mode, M=self.M, K=self.K, B=self.B, groups=self.groups, flags=flags,
+                                     dtype=self.torch_dtype, algo=self._algo_name())
+
+    def _given_workspace(self, workspace: torch.Tensor, dev: torch.device, mode: int, flags: int):
+        """The part of a caller's workspace (uint8) that a call takes, or None when it needs none."""
+        need = self._workspace_need(dev, mode, flags)
+        if need == 0:
+            return None
+        if (not isinstance(workspace, torch.Tensor) or workspace.dtype != torch.uint8 or workspace.device != dev
+                or not workspace.is_contiguous() or workspace.numel() < need or workspace.data_ptr() % 16):
+            raise ValueError(f"{self.kind}: the workspace is not {need} bytes (uint8, contiguous, 16-byte aligned) on {dev}")
+        return workspace.view(-1)[:need]
 
     def _check(self, tensors):
         if len(tensors) != len(self.shapes):
@@ -143,12 +156,17 @@ class PredictionErrorKernel(_FusedOp):
         self.M, self.K, self.B = int(M), int(K), int(B)
         self.saved = bool(saved_activation)
 
-    def __call__(self, x_upper, w, x_lower, e):
+    def workspace_bytes(self, device) -> int:
+        """Bytes of workspace a call on ``device`` needs (what ``workspace=`` has to hold)."""
+        return self._workspace_need(device, N.MODE_PRED, 0 if self.saved else N.FLAG_ACTIVATE_B)
+
+    def __call__(self, x_upper, w, x_lower, e, *, workspace=None):
         dev = self._check((x_upper, w, x_lower, e))
         s = N.stream_handle(dev)
         lib = N.load()
         flags = 0 if self.saved else N.FLAG_ACTIVATE_B
-        ws = self._workspace(dev, N.MODE_PRED, flags)
+        ws = (self._workspace(dev, N.MODE_PRED, flags) if workspace is None else
+              self._given_workspace(workspace, dev, N.MODE_PRED, flags))
         if ws is not None or self.cfg.tune() is not None:  # tensor cores: f(X_upper) stored once, then tcgen05
             N.fused_gemm(N.MODE_PRED, w, x_upper, e, x_lower, M=self.M, K=self.K, B=self.B, groups=self.groups,
                          flags=flags, act=self.activation, dtype=self.torch_dtype, algo=self._algo_name(),
@@ -221,9 +239,14 @@ class ForwardKernel(_FusedOp):
         super().__init__([(K, B), (M, K), (M, B)], activation, dtype, cfg, groups)
         self.M, self.K, self.B = int(M), int(K), int(B)
 
-    def __call__(self, x_upper, w, out):
+    def workspace_bytes(self, device) -> int:
+        """Bytes of workspace a call on ``device`` needs (what ``workspace=`` has to hold)."""
+        return self._workspace_need(device, N.MODE_FORWARD, N.FLAG_ACTIVATE_B)
+
+    def __call__(self, x_upper, w, out, *, workspace=None):
         dev = self._check((x_upper, w, out))
-        ws = self._workspace(dev, N.MODE_FORWARD, N.FLAG_ACTIVATE_B)
+        ws = (self._workspace(dev, N.MODE_FORWARD, N.FLAG_ACTIVATE_B) if workspace is None else
+              self._given_workspace(workspace, dev, N.MODE_FORWARD, N.FLAG_ACTIVATE_B))
         if ws is not None or self.cfg.tune() is not None:
             N.fused_gemm(N.MODE_FORWARD, w, x_upper, out, M=self.M, K=self.K, B=self.B, groups=self.groups,
                          flags=N.FLAG_ACTIVATE_B, act=self.activation, dtype=self.torch_dtype,

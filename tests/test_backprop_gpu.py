@@ -127,3 +127,55 @@ def test_predictor_follows_refresh_and_refuses():
     adam = TileLangIPC(IPCConfig(dims=dims, dtype=dt, optimizer="adamw"), device=DEV)
     with pytest.raises(ValueError):
         CheckpointedBackprop(adam)
+
+
+def test_a_step_holds_what_it_says():
+    """Wide layers, whose products need a copy of the states in 16 bits: one for all of them, and the errors of layers 1 and
+    2 where the forward sweep's buffers were.  Nothing is left in the operators' own workspaces."""
+    from lich_b200 import microscaled as mx
+    from lich_b200.backprop import CheckpointedBackprop
+    dims, B, dt = (10, 512, 512, 512, 784), 4104, torch.bfloat16
+    m = _model(dims, dt, alpha=1e-4)
+    x, y = (t.to(DEV) for t in _batch(dims, B, dt))
+    bp = CheckpointedBackprop(m)
+    torch.cuda.synchronize()
+    scratch, before = sum(s.bytes for s in mx._scratch.values()), torch.cuda.memory_allocated(DEV)
+    bp.train_step(x, y)
+    held = torch.cuda.memory_allocated(DEV) - before
+    states = sum(dims[1:]) * B
+    assert bp.checkpoint_bytes(B) == sum(dims[1:]) * (4128 + 129)
+    # checkpoints; two state buffers and the errors of layers 0 and 3; a workspace that the widest f(x^) is the most of
+    most = bp.checkpoint_bytes(B) + 2 * B * (2 * 512 + 512 + 10) + 2 * B * 784 + (17 << 20)
+    assert bp.held_bytes(B) <= most
+    assert sum(s.bytes for s in mx._scratch.values()) == scratch  # (entries of operators that need none may be new)
+    assert held <= bp.held_bytes(B) + 512 * 20  # (the allocator rounds each up to 512 bytes)
+    w = [t.clone() for t in m.w]
+    bp.train_step(x, y)
+    assert torch.cuda.memory_allocated(DEV) - before <= held + sum(t.numel() * 2 + 512 for t in w)
+    assert states * 2 > bp.checkpoint_bytes(B)
+    k = mx.build_weight_update_checkpoint(512, 784, B, "tanh", "bfloat16", 1e-4)
+    args = (torch.zeros(512, 784, device=DEV, dtype=dt), torch.zeros(512, B, device=DEV, dtype=dt),
+            *mx.empty_checkpoint(784, B, device=DEV))
+    for ws in (torch.empty(k.workspace_bytes() - 1, device=DEV, dtype=torch.uint8), torch.empty(1 << 30, dtype=torch.uint8),
+               torch.empty(k.workspace_bytes() + 1, device=DEV, dtype=torch.uint8)[1:], 5):
+        with pytest.raises(ValueError, match="workspace"):
+            k(*args, workspace=ws)
+    with pytest.raises(ValueError):
+        bp.train_step(x, y.cpu())
+
+
+def test_a_changing_rate_changes_the_step():
+    from dataclasses import replace
+
+    from lich_b200.backprop import CheckpointedBackprop
+    dims, B, dt = (10, 64, 784), 128, torch.float32
+    x, y = (t.to(DEV) for t in _batch(dims, B, dt))
+    moved = []
+    for alpha in (1e-3, 2e-3):
+        m = _model(dims, dt, alpha=1e-3)
+        bp = CheckpointedBackprop(m)
+        w0 = m.w[0].clone()
+        m.cfg = replace(m.cfg, alpha=alpha)
+        bp.train_step(x, y)
+        moved.append((m.w[0] - w0).double())
+    assert (moved[1] - 2 * moved[0]).abs().max() <= 2.0 ** -20 * m.w[0].abs().max()
