@@ -139,7 +139,7 @@ def test_a_step_holds_what_it_says():
     x, y = (t.to(DEV) for t in _batch(dims, B, dt))
     bp = CheckpointedBackprop(m)
     torch.cuda.synchronize()
-    scratch, before = sum(s.bytes for s in mx._scratch.values()), torch.cuda.memory_allocated(DEV)
+    before = torch.cuda.memory_allocated(DEV)
     bp.train_step(x, y)
     held = torch.cuda.memory_allocated(DEV) - before
     states = sum(dims[1:]) * B
@@ -147,7 +147,7 @@ def test_a_step_holds_what_it_says():
     # checkpoints; two state buffers and the errors of layers 0 and 3; a workspace that the widest f(x^) is the most of
     most = bp.checkpoint_bytes(B) + 2 * B * (2 * 512 + 512 + 10) + 2 * B * 784 + (17 << 20)
     assert bp.held_bytes(B) <= most
-    assert sum(s.bytes for s in mx._scratch.values()) == scratch  # (entries of operators that need none may be new)
+    assert not any(s.bytes for k, s in mx._scratch.items() if B in k)
     assert held <= bp.held_bytes(B) + 512 * 20  # (the allocator rounds each up to 512 bytes)
     w = [t.clone() for t in m.w]
     bp.train_step(x, y)
