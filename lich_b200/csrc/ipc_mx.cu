@@ -70,27 +70,6 @@ __device__ __forceinline__ uint32_t group_max(uint32_t m) {
 
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
-// f in fp32.  sigmoid and silu take the exponential of -|v|, which cannot overflow: 1 / (1 + e^-v) itself is 0 below
-// v = -88.7, where sigmoid(v) is still a (subnormal) number.  Far below 0 silu is v e^v, whose e^v alone would be
-// rounded as a subnormal before v multiplies it: the last factor e^-32 is applied at the end.
-template <int ACT>
-__device__ __forceinline__ float act_full(float v) {
-  if constexpr (ACT == IPC_ACT_SIGMOID || ACT == IPC_ACT_SILU) {
-    if (ACT == IPC_ACT_SILU && v < -64.f) return v * expf(v + 32.f) * 1.26641655e-14f;
-    const float z = expf(-fabsf(v));
-    const float n = v >= 0.f ? 1.f : z;
-    return (ACT == IPC_ACT_SILU ? v * n : n) / (1.f + z);
-  }
-  return act_f<ACT>(v);
-}
-// f of a value that is then stored in T: the MUFU forms for 16-bit storage (their error is about one rounding
-// step of fp16), CUDA's own functions for fp32.
-template <typename T, int ACT>
-__device__ __forceinline__ float act_for(float v) {
-  if constexpr (sizeof(T) == 2) return act_f_hw<ACT>(v);
-  return act_full<ACT>(v);
-}
-
 // words of a later kernel's workspace, cleared by the first CTA
 __device__ __forceinline__ void zero_words(int* zero, int n) {
   if (blockIdx.x == 0 && blockIdx.y == 0)
@@ -201,7 +180,7 @@ __device__ __forceinline__ void restore_tile(const signed char* __restrict__ cod
 #pragma unroll
       for (int q = 0; q < N / 4; ++q) mx8_floats(w[it][q], v + 4 * q);
 #pragma unroll
-      for (int j = 0; j < N; ++j) v[j] = act_for<T, ACT>(v[j] * sc);
+      for (int j = 0; j < N; ++j) v[j] = mx_f<T, ACT>(v[j] * sc);
       T* o = out + (long long)d * ld_out + c;
       if (c + N <= cols) {
         Vec<T>::store(o, v);
@@ -226,7 +205,7 @@ __device__ __forceinline__ void restore_tile(const signed char* __restrict__ cod
 #pragma unroll
       for (int j = 0; j < TB; ++j) {
         const int c = c0 + MX_BLOCK * j + lane;
-        if (c < cols) out[(long long)d * ld_out + c] = St<T>::st(act_for<T, ACT>((float)q[j] * mx_scale(byte[j])));
+        if (c < cols) out[(long long)d * ld_out + c] = St<T>::st(mx_f<T, ACT>((float)q[j] * mx_scale(byte[j])));
       }
     }
   }
@@ -269,7 +248,7 @@ __global__ void __launch_bounds__(threads_of(VEC)) mx4_rows_kernel(const T* __re
 #pragma unroll
       for (int j = 0; j < N; ++j) {
         const T* h = reinterpret_cast<const T*>(raw[it]);
-        v[j] = act_full<ACT>(St<T>::ld(h[j]));
+        v[j] = mx_f<float, ACT>(St<T>::ld(h[j]));
         if (ACT == IPC_ACT_SIGMOID && !(r < R && c + j < K)) v[j] = 0.f;  // (the other f are 0 at 0)
       }
       uint32_t m = 0;
@@ -301,8 +280,8 @@ __global__ void __launch_bounds__(threads_of(VEC)) mx4_rows_kernel(const T* __re
 #pragma unroll
       for (int j = 0; j < TB; ++j) {
         const int c = c0 + MX_BLOCK * j + lane;
-        if (ACT != IPC_ACT_RELU && ACT != IPC_ACT_IDENTITY) v[j] = (r < R && c < K) ? act_full<ACT>(v[j]) : 0.f;
-        else v[j] = act_full<ACT>(v[j]);
+        if (ACT != IPC_ACT_RELU && ACT != IPC_ACT_IDENTITY) v[j] = (r < R && c < K) ? mx_f<float, ACT>(v[j]) : 0.f;
+        else v[j] = mx_f<float, ACT>(v[j]);
         const uint32_t byte = mx4_scale_byte(__reduce_max_sync(0xffffffffu, abs_bits(v[j])));
         if (lane == 0) s_scale[rr][j] = (unsigned char)byte;
         const float lo = byte == MX_NAN_BYTE ? 0.f : v[j] * mx_inv_scale(byte);
@@ -329,14 +308,14 @@ __global__ void __launch_bounds__(threads_of(VEC)) mx4_rows_kernel(const T* __re
 // shared memory, so that a sample's 128 bytes leave together.
 // PAIR: rows start on boundaries of two elements and a lane takes two neighbouring samples; otherwise samples lane, lane + 32.
 constexpr int TUR = 64;
-// relu of two 16-bit numbers (like act_f, 0 for a NaN)
+// relu of two 16-bit numbers (a NaN stays one)
 template <typename T>
 __device__ __forceinline__ uint32_t relu2(uint32_t w) {
   if constexpr (std::is_same<T, __half>::value) {
-    const __half2 r = __hmax2(*reinterpret_cast<__half2*>(&w), __float2half2_rn(0.f));
+    const __half2 r = __hmax2_nan(*reinterpret_cast<__half2*>(&w), __float2half2_rn(0.f));
     return *reinterpret_cast<const uint32_t*>(&r);
   } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-    const __nv_bfloat162 r = __hmax2(*reinterpret_cast<__nv_bfloat162*>(&w), __float2bfloat162_rn(0.f));
+    const __nv_bfloat162 r = __hmax2_nan(*reinterpret_cast<__nv_bfloat162*>(&w), __float2bfloat162_rn(0.f));
     return *reinterpret_cast<const uint32_t*>(&r);
   }
   return w;
@@ -413,7 +392,7 @@ __global__ void __launch_bounds__(THREADS, turned_ctas(sizeof(T), ACT)) mx4_turn
     if constexpr (!PACKED) {
 #pragma unroll
       for (int i = 0; i < MX_BLOCK; ++i) {
-        f[i] = act_full<ACT>(St<T>::ld(v[i].v[h]));
+        f[i] = mx_f<float, ACT>(St<T>::ld(v[i].v[h]));
         if (ACT == IPC_ACT_SIGMOID && !(in[h] && kb + i < K)) f[i] = 0.f;  // (the other f are 0 at 0)
         top[h] = max(top[h], abs_bits(f[i]));
       }

@@ -78,6 +78,35 @@ __device__ __forceinline__ void mx4_unpack8(uint32_t codes, uint32_t (&h)[4]) {
       : "r"(codes));
 }
 
+// f and f' of states read back, in fp32, and f of what is quantised.  They are the framework's but for two things.
+//   relu keeps a NaN: a block that held an infinity or a NaN reads back as NaNs, and taking those for 0 would hide it.
+//   sigmoid and silu in fp32 take the exponential of -|x|, which cannot overflow: 1 / (1 + e^-x) itself is 0 below
+//   x = -88.7, where sigmoid(x) is still a (subnormal) number.  Far below 0 silu is x e^x, whose e^x alone would be
+//   rounded as a subnormal before x multiplies it: the last factor e^-32 is applied at the end.
+template <int ACT>
+__device__ __forceinline__ float mx_f32(float x) {
+  if constexpr (ACT == IPC_ACT_SIGMOID || ACT == IPC_ACT_SILU) {
+    if (ACT == IPC_ACT_SILU && x < -64.f) return x * expf(x + 32.f) * 1.26641655e-14f;
+    const float z = expf(-fabsf(x));
+    const float n = x >= 0.f ? 1.f : z;
+    return (ACT == IPC_ACT_SILU ? x * n : n) / (1.f + z);
+  }
+  return act_f<ACT>(x);
+}
+// T: the storage type.  16 bits take the MUFU forms.
+template <typename T, int ACT>
+__device__ __forceinline__ float mx_f(float x) {
+  if constexpr (ACT == IPC_ACT_RELU) return x <= 0.f ? 0.f : x;
+  if constexpr (sizeof(T) == 2) return act_f_hw<ACT>(x);
+  return mx_f32<ACT>(x);
+}
+template <typename T, int ACT>
+__device__ __forceinline__ float mx_df(float x) {
+  if constexpr (ACT == IPC_ACT_RELU) return x > 0.f ? 1.f : x <= 0.f ? 0.f : x;
+  if constexpr (sizeof(T) == 2) return act_df_hw<ACT>(x);
+  return act_df<ACT>(x);
+}
+
 // Layouts.  8 bits: codes [D][32 * ceil(B/32)], scale bytes [ceil(B/32)][D], blocks along the batch.
 // 4 bits, R rows of K columns: codes [R][Kp/2], Kp = 128 * ceil(K/128), lower column in the lower nibble; scale
 // bytes in atoms of 128 rows x 4 blocks, [ceil(R/128)][Kp/128][32][4][4] with row r, block j at

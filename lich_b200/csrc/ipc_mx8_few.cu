@@ -17,17 +17,6 @@ namespace {
 constexpr int FEW = 16;
 constexpr int OR = 8, OM = 8 * OR, OK = 256, OTHREADS = 256;  // rows of a thread, of a CTA; columns
 
-template <typename T, int ACT>
-__device__ __forceinline__ float few_f(float v) {
-  if constexpr (sizeof(T) == 2) return act_f_hw<ACT>(v);
-  return act_f<ACT>(v);
-}
-template <typename T, int ACT>
-__device__ __forceinline__ float few_df(float v) {
-  if constexpr (sizeof(T) == 2) return act_df_hw<ACT>(v);
-  return act_df<ACT>(v);
-}
-
 // ------------------------------------------------------------------------------------- W, WD, G
 // VEC: rows of out start on 16-byte boundaries; a thread owns 8 neighbouring columns (else columns lane, lane + 32, ...) of
 // 8 rows, so that a sample costs 10 shared-memory wavefronts for 64 FMAs.
@@ -50,7 +39,7 @@ __global__ void __launch_bounds__(OTHREADS) mx8_outer_kernel(const __grid_consta
       mx8_floats(c.w, v + 12);
 #pragma unroll
       for (int b = 0; b < FEW; ++b)
-        if (b < B) sA[b][tid] = few_f<T, ACT>(v[b] * sc);
+        if (b < B) sA[b][tid] = mx_f<T, ACT>(v[b] * sc);
     }
   }
   const T* E = reinterpret_cast<const T*>(p.A);
@@ -231,7 +220,7 @@ __global__ void __launch_bounds__(BTHREADS) mx8_columns_kernel(const __grid_cons
     const int k = c0 + i / NB, b = i % NB;
     if (k < p.Mg && b < B) {
       const float x = (float)p.ck[(long long)k * p.ld_ck + b] * mx_scale(p.cks[k]);
-      reinterpret_cast<T*>(p.out)[(long long)k * B + b] = St<T>::st(few_df<T, ACT>(x) * sum);
+      reinterpret_cast<T*>(p.out)[(long long)k * B + b] = St<T>::st(mx_df<T, ACT>(x) * sum);
     }
   }
 }

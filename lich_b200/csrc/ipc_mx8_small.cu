@@ -188,7 +188,7 @@ __global__ void __launch_bounds__(STHREADS) mx8_small_kernel(const __grid_consta
         T* lo = reinterpret_cast<T*>(l);
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const float f = in && k0 + c + e < k_hi ? act_f_hw<ACT>(q[e] * sc) : 0.f;
+          const float f = in && k0 + c + e < k_hi ? mx_f<T, ACT>(q[e] * sc) : 0.f;
           h[e] = St<T>::st(f);
           if constexpr (LOW) lo[e] = St<T>::st(f - St<T>::ld(h[e]));
         }
@@ -288,7 +288,7 @@ __global__ void __launch_bounds__(STHREADS) mx8_small_kernel(const __grid_consta
       if (m < p.Mg && n < p.Ng) {
         if constexpr (BKM) {
           const float x = (float)(signed char)(code2[j][r >> 1] >> (8 * (r & 1))) * mx_scale(sbyte[r >> 1]);
-          reinterpret_cast<T*>(p.out)[(long long)m * p.Ng + n] = St<T>::st(act_df_hw<ACT>(x) * acc[j][r]);
+          reinterpret_cast<T*>(p.out)[(long long)m * p.Ng + n] = St<T>::st(mx_df<T, ACT>(x) * acc[j][r]);
         } else {
           epilogue<T, IPC_ACT_IDENTITY, MODE>(p, 0, m, n, acc[j][r]);
         }

@@ -603,3 +603,70 @@ def test_tensors_without_an_address_are_refused():
         k(x[0].to_sparse(), c, s)
     k(x[0], c, s)
     assert not c.any()
+
+
+@pytest.mark.parametrize("dt", ALL)
+@pytest.mark.parametrize("D,B", [(33, 96), (20, 131)])
+def test_every_f_keeps_a_block_that_was_not_finite(D, B, dt):
+    """A NaN or an infinity leaves a block of NaNs: f of it is NaN, relu's too, and a quantised f(x) is marked where f(x)
+    itself is not finite."""
+    mx = _mx()
+    x = _rand((D, B), 60, 1.0, dt)
+    x[3, 5], x[4, 40], x[5, 70] = float("nan"), float("inf"), -float("inf")
+    c, s = mx.empty_checkpoint(D, B, device=DEV)
+    mx.build_checkpoint(D, B, NAME[dt])(x.to(DEV), c, s)
+    marked = X.load8(c.cpu(), s.cpu(), B).isnan()
+    assert marked.sum() == 96
+    for act in ACTS:
+        out = torch.zeros(D, B, device=DEV, dtype=dt)
+        mx.build_checkpoint_restore(D, B, act, NAME[dt])(c, s, out)
+        assert torch.equal(out.cpu().isnan(), marked)
+        for turned in (False, True):
+            R, K = (B, D) if turned else (D, B)
+            q, sc = mx.empty_mxfp4(R, K, device=DEV)
+            mx.build_mxfp4_quantize(R, K, act, NAME[dt], turned)(x.to(DEV), q, sc)
+            back = torch.zeros(R, K, device=DEV)
+            mx.build_mxfp4_restore(R, K, "float32")(q, sc, back)
+            v = O.act_forward(act, x.double())
+            v = torch.where(x.isneginf(), torch.full_like(v, 0.0 if act != "identity" else -math.inf), v)  # (the limit)
+            if act in ("silu", "gelu"):
+                v[5, 70] = float("nan")  # -inf times 0, as f is computed
+            if act == "tanh":
+                v[5, 70] = -1.0
+            want = X.quant4(v.t().contiguous() if turned else v)[0].isnan()
+            assert torch.equal(back.cpu().isnan(), want)
+
+
+NSIZES = [("auto", 20, 30, 3), ("auto", 700, 648, 4), ("simt", 40, 72, 200), ("simt", 33, 65, 97), ("tcgen05", 136, 264, 520),
+          ("tcgen05", 130, 259, 517), ("tcgen05", 256, 512, 4608)]
+
+
+@pytest.mark.parametrize("dt", ALL)
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("backend,M,K,B", NSIZES)
+def test_products_mark_states_that_were_not_finite_on_every_kernel(backend, M, K, B, act, dt):
+    """One state that overflowed marks its block in the error sent up (where f' depends on the state) and its feature in
+    the weights' gradient, and nothing else."""
+    from lich_b200.tilelang_kernels import KernelConfig
+    if dt is torch.float32:
+        backend = "auto" if backend == "tcgen05" else backend
+    mx = _mx()
+    cfg = KernelConfig(backend=backend)
+    x = _rand((K, B), 61, 1.0, dt)
+    x[5, B - 1] = float("inf")
+    c, s = _ckpt(x)
+    bad = X.load8(c.cpu(), s.cpu(), B).isnan()
+    assert bad.any()
+    w, e = _rand((M, K), 62, 0.1, dt), _rand((M, B), 63, 0.1, dt)
+    up = torch.zeros(K, B, device=DEV, dtype=dt)
+    mx.build_error_backward_checkpoint(M, K, B, act, NAME[dt], cfg)(w.to(DEV), e.to(DEV), c, s, up)
+    assert torch.equal(up.cpu().isnan(), bad & (act != "identity"))
+    want = torch.zeros(M, K, dtype=torch.bool)
+    want[:, 5] = True
+    for name in {"float32", NAME[dt]}:
+        dw = torch.zeros(M, K, device=DEV, dtype=getattr(torch, name))
+        mx.build_weight_delta_checkpoint(M, K, B, act, NAME[dt], 1.0, name, cfg)(dw, e.to(DEV), c, s)
+        assert torch.equal(dw.cpu().isnan(), want)
+    wd = w.to(DEV)
+    mx.build_weight_update_checkpoint(M, K, B, act, NAME[dt], 0.5, cfg)(wd, e.to(DEV), c, s)
+    assert torch.equal(wd.cpu().isnan(), want)
