@@ -670,3 +670,19 @@ def test_products_mark_states_that_were_not_finite_on_every_kernel(backend, M, K
     wd = w.to(DEV)
     mx.build_weight_update_checkpoint(M, K, B, act, NAME[dt], 0.5, cfg)(wd, e.to(DEV), c, s)
     assert torch.equal(wd.cpu().isnan(), want)
+
+
+@pytest.mark.parametrize("K", [64, 512, 2000])
+@pytest.mark.parametrize("B", [3, 16, 200])
+def test_forward_of_scales_that_undo_one_another(B, K):
+    """Weights of 2^124 times activations of 2^-124 and the other way round: a block's sum of codes is up to 1152 and
+    overflows if it meets the large scale first."""
+    mx = _mx()
+    M = 150
+    for wf, af in ((124, -124), (-124, 124), (124, -140), (-120, 110)):
+        wv, wq, wsc = X.quant4(torch.exp2(torch.tensor(float(wf))) * _rand((M, K), 70))
+        av, aq, asc = X.quant4((_rand((B, K), 71).double() * 2.0 ** af).float())
+        out = torch.full((M, B), 9.0, device=DEV)
+        mx.build_mxfp4_forward(M, K, B, "float32")(wq.to(DEV), wsc.to(DEV), aq.to(DEV), asc.to(DEV), out)
+        ref = wv @ av.t()
+        _within(out, ref, (wv.abs() @ av.abs().t()) * K * 2.0 ** -23 + U[torch.float32] * ref.abs() + TINY[torch.float32])
