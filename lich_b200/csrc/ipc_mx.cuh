@@ -78,33 +78,78 @@ __device__ __forceinline__ void mx4_unpack8(uint32_t codes, uint32_t (&h)[4]) {
       : "r"(codes));
 }
 
-// f and f' of states read back, in fp32, and f of what is quantised.  They are the framework's but for two things.
-//   relu keeps a NaN: a block that held an infinity or a NaN reads back as NaNs, and taking those for 0 would hide it.
-//   sigmoid and silu in fp32 take the exponential of -|x|, which cannot overflow: 1 / (1 + e^-x) itself is 0 below
-//   x = -88.7, where sigmoid(x) is still a (subnormal) number.  Far below 0 silu is x e^x, whose e^x alone would be
-//   rounded as a subnormal before x multiplies it: the last factor e^-32 is applied at the end.
-template <int ACT>
-__device__ __forceinline__ float mx_f32(float x) {
-  if constexpr (ACT == IPC_ACT_SIGMOID || ACT == IPC_ACT_SILU) {
+// f and f' of states read back, in fp32, and f of what is quantised.  They are written with an exponential z of a negative
+// number and r = 1 / (1 + z), so that no term is the small difference of large ones: f' of a saturated state and gelu of
+// a negative one keep their relative accuracy (1 - tanh(x)^2 at x = 5, with tanh off by 2^-11, has no correct digit left;
+// neither has 1 + tanh(u) in gelu at x = -4), and nothing overflows.
+//   tanh'    = 4 z r^2            z = e^-2|x|
+//   sigmoid' = z r^2              z = e^-|x|
+//   silu'    = s + x z r^2        ... s = sigmoid(x) = r or z r
+//   gelu     = x s                z = e^-2|u|, u = k (x + c x^3), s = sigmoid(2 u) = r or z r
+//   gelu'    = s + 2 x u' z r^2
+// In 16-bit storage z and r are ex2.approx and rcp.approx (2^-22 and 2^-23), in fp32 CUDA's expf and a division.  f' is off
+// by about 2^-20 of itself, plus the exponent's rounding (its size times 2^-22).  tanh itself is tanh.approx in 16-bit
+// storage, off by 2^-11 of itself, about one rounding of fp16.
+// relu keeps a NaN: a block that held an infinity or a NaN reads back as NaNs, and taking those for 0 would hide it.
+// T: the storage type.
+template <typename T>
+__device__ __forceinline__ float mx_exp(float x) {  // x <= 0
+  if constexpr (sizeof(T) == 2) {
+    float z;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(z) : "f"(1.4426950408889634f * x));
+    return z;
+  }
+  return expf(x);
+}
+template <typename T>
+__device__ __forceinline__ float mx_recip(float x) {
+  if constexpr (sizeof(T) == 2) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+  }
+  return 1.f / x;
+}
+__device__ __forceinline__ float mx_gelu_u(float x) { return kGeluK * (x + kGeluC * x * x * x); }
+
+template <typename T, int ACT>
+__device__ __forceinline__ float mx_f(float x) {
+  if constexpr (ACT == IPC_ACT_RELU) {
+    return x <= 0.f ? 0.f : x;
+  } else if constexpr (ACT == IPC_ACT_GELU) {
+    if constexpr (sizeof(T) == 2) return x * sigmoid_hw(2.f * mx_gelu_u(x));
+    const float z = mx_exp<T>(-2.f * fabsf(mx_gelu_u(x)));
+    return x * (x >= 0.f ? 1.f : z) / (1.f + z);
+  } else if constexpr (sizeof(T) == 2) {
+    return act_f_hw<ACT>(x);
+  } else if constexpr (ACT == IPC_ACT_SIGMOID || ACT == IPC_ACT_SILU) {
+    // 1 / (1 + e^-x) itself is 0 below x = -88.7, where sigmoid(x) is still a (subnormal) number.  Far below 0 silu is x e^x,
+    // whose e^x alone would be rounded as a subnormal before x multiplies it: the last factor e^-32 comes at the end.
     if (ACT == IPC_ACT_SILU && x < -64.f) return x * expf(x + 32.f) * 1.26641655e-14f;
     const float z = expf(-fabsf(x));
     const float n = x >= 0.f ? 1.f : z;
     return (ACT == IPC_ACT_SILU ? x * n : n) / (1.f + z);
+  } else {
+    return act_f<ACT>(x);
   }
-  return act_f<ACT>(x);
-}
-// T: the storage type.  16 bits take the MUFU forms.
-template <typename T, int ACT>
-__device__ __forceinline__ float mx_f(float x) {
-  if constexpr (ACT == IPC_ACT_RELU) return x <= 0.f ? 0.f : x;
-  if constexpr (sizeof(T) == 2) return act_f_hw<ACT>(x);
-  return mx_f32<ACT>(x);
 }
 template <typename T, int ACT>
 __device__ __forceinline__ float mx_df(float x) {
-  if constexpr (ACT == IPC_ACT_RELU) return x > 0.f ? 1.f : x <= 0.f ? 0.f : x;
-  if constexpr (sizeof(T) == 2) return act_df_hw<ACT>(x);
-  return act_df<ACT>(x);
+  if constexpr (ACT == IPC_ACT_RELU) {
+    return x > 0.f ? 1.f : x <= 0.f ? 0.f : x;
+  } else if constexpr (ACT == IPC_ACT_TANH) {
+    const float z = mx_exp<T>(-2.f * fabsf(x)), r = mx_recip<T>(1.f + z);
+    return 4.f * z * r * r;
+  } else if constexpr (ACT == IPC_ACT_SIGMOID || ACT == IPC_ACT_SILU || ACT == IPC_ACT_GELU) {
+    const float z = mx_exp<T>(ACT == IPC_ACT_GELU ? -2.f * fabsf(mx_gelu_u(x)) : -fabsf(x)), r = mx_recip<T>(1.f + z);
+    const float d = z * r * r;
+    if constexpr (ACT == IPC_ACT_SIGMOID) return d;
+    const float s = x >= 0.f ? r : z * r;
+    const float t = ACT == IPC_ACT_SILU ? x * d : 2.f * kGeluK * (1.f + 3.f * kGeluC * x * x) * x * d;
+    return z == 0.f ? s : s + t;  // (the square of a large x is infinite, and 0 times that no number)
+  } else {
+    return act_df<ACT>(x);
+  }
 }
 
 // Layouts.  8 bits: codes [D][32 * ceil(B/32)], scale bytes [ceil(B/32)][D], blocks along the batch.

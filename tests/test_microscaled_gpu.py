@@ -686,3 +686,75 @@ def test_forward_of_scales_that_undo_one_another(B, K):
         mx.build_mxfp4_forward(M, K, B, "float32")(wq.to(DEV), wsc.to(DEV), aq.to(DEV), asc.to(DEV), out)
         ref = wv @ av.t()
         _within(out, ref, (wv.abs() @ av.abs().t()) * K * 2.0 ** -23 + U[torch.float32] * ref.abs() + TINY[torch.float32])
+
+
+# Slopes of saturated states, and gelu of negative ones, relative to their own size.  With z the exponential e^-|2x| (tanh),
+# e^-|x| (sigmoid, silu) or e^-|2u| (gelu, u its inner polynomial) and r = 1 / (1 + z), every term is a product of z, r and
+# numbers of the size of x: ex2.approx is off by 2^-22, rcp.approx by 2^-23, and the exponent, of size a, by a few
+# roundings of 2^-24 (gelu's u by four): 2^-19 (1 + a) in 16-bit storage, 2^-20 (1 + a) in fp32; exponentials below
+# 2^-126 may be 0.
+def _stable(act, x):
+    """(f, f', sum of the magnitudes of the terms of f', the exponent a) in 64 bits without cancellation."""
+    u = math.sqrt(2 / math.pi) * (x + 0.044715 * x ** 3)
+    a = {"tanh": 2 * x.abs(), "sigmoid": x.abs(), "silu": x.abs(), "gelu": 2 * u.abs()}[act]
+    z = torch.exp(-a)
+    r = 1 / (1 + z)
+    s = torch.where(x >= 0, r, z * r)
+    if act == "tanh":
+        return torch.tanh(x), 4 * z * r * r, 4 * z * r * r, a
+    if act == "sigmoid":
+        return s, z * r * r, z * r * r, a
+    t = x * z * r * r * (1 if act == "silu" else 2 * math.sqrt(2 / math.pi) * (1 + 3 * 0.044715 * x * x))
+    return x * s, s + t, s + t.abs(), a
+
+
+@pytest.mark.parametrize("dt", ALL)
+@pytest.mark.parametrize("act", ["tanh", "sigmoid", "silu", "gelu"])
+@pytest.mark.parametrize("backend,M,K,B", [("auto", 24, 40, 3), ("simt", 40, 72, 200), ("tcgen05", 136, 264, 520)])
+def test_slopes_of_saturated_states(backend, M, K, B, act, dt):
+    from lich_b200.tilelang_kernels import KernelConfig
+    if dt is torch.float32 and backend == "tcgen05":
+        backend = "auto"
+    mx = _mx()
+    x = _rand((K, B), 80)
+    x = (torch.sign(x) * (4 + 4 * torch.rand(K, B, generator=torch.Generator().manual_seed(81)))).to(dt)
+    c, s = _ckpt(x)
+    xhat = X.load8(c.cpu(), s.cpu(), B)
+    w, e = _rand((M, K), 82, 0.5, dt), _rand((M, B), 83, 1.0, dt)
+    up = torch.zeros(K, B, device=DEV, dtype=dt)
+    mx.build_error_backward_checkpoint(M, K, B, act, NAME[dt], KernelConfig(backend=backend))(w.to(DEV), e.to(DEV), c, s, up)
+    _, slope, size, a = _stable(act, xhat)
+    acc, S = w.double().t() @ e.double(), w.double().abs().t() @ e.double().abs()
+    ref = slope * acc
+    rel = (2.0 ** -20 if dt is torch.float32 else 2.0 ** -19) * (1 + a)
+    tol = (size * rel + 2.0 ** -125) * (acc.abs() + S * M * 2.0 ** -23) + slope.abs() * S * M * 2.0 ** -23
+    _within(up, ref, tol * (1 + U[dt]) + (U[dt] + 2.0 ** -23) * ref.abs() + TINY[dt])
+
+
+@pytest.mark.parametrize("dt", ALL)
+@pytest.mark.parametrize("B", [64, 67])
+def test_gelu_of_negative_states(B, dt):
+    mx = _mx()
+    D = 40
+    x = (6 * (2 * torch.rand(D, B, generator=torch.Generator().manual_seed(90)) - 1)).to(dt)
+    c, s = _ckpt(x)
+    xhat = X.load8(c.cpu(), s.cpu(), B)
+    out = torch.zeros(D, B, device=DEV, dtype=dt)
+    mx.build_checkpoint_restore(D, B, "gelu", NAME[dt])(c, s, out)
+    f, _, _, a = _stable("gelu", xhat)
+    rel = (2.0 ** -20 if dt is torch.float32 else 2.0 ** -19) * (1 + a)
+    _within(out, f, (rel * f.abs() + 2.0 ** -125) * (1 + U[dt]) + U[dt] * f.abs() + TINY[dt])
+
+
+@pytest.mark.parametrize("act", ["tanh", "sigmoid", "silu", "gelu"])
+def test_slopes_of_very_large_states(act):
+    """bf16 and fp32 states far beyond where f saturates, whose squares and cubes overflow: the slope is 1 or 0."""
+    mx = _mx()
+    for dt in (torch.bfloat16, torch.float32):
+        x = torch.tensor([1e20, -1e20, 3e13, -3e13, 1e30, -1e30, 200.0, -200.0], dtype=dt).repeat_interleave(32)[None]
+        c, s = _ckpt(x)
+        w, e = torch.ones(1, 1, dtype=dt, device=DEV), torch.ones(1, 256, dtype=dt, device=DEV)
+        up = torch.full((1, 256), 9.0, device=DEV, dtype=dt)
+        mx.build_error_backward_checkpoint(1, 1, 256, act, NAME[dt])(w, e, c, s, up)
+        want = (x > 0).float() if act in ("silu", "gelu") else torch.zeros(1, 256)
+        assert torch.equal(up.cpu().float(), want)
