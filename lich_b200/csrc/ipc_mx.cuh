@@ -92,34 +92,39 @@ __device__ __forceinline__ void mx4_unpack8(uint32_t codes, uint32_t (&h)[4]) {
 // storage, off by 2^-11 of itself, about one rounding of fp16.
 // relu keeps a NaN: a block that held an infinity or a NaN reads back as NaNs, and taking those for 0 would hide it.
 // T: the storage type.
-template <typename T>
-__device__ __forceinline__ float mx_exp(float x) {  // x <= 0
-  if constexpr (sizeof(T) == 2) {
-    float z;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(z) : "f"(1.4426950408889634f * x));
-    return z;
-  }
-  return expf(x);
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kGelu1 = 2.f * kGeluK, kGelu3 = 2.f * kGeluK * kGeluC;  // 2 u = x (kGelu1 + kGelu3 x^2)
+
+__device__ __forceinline__ float mx_ex2(float x) {
+  float z;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(z) : "f"(x));
+  return z;
 }
 template <typename T>
-__device__ __forceinline__ float mx_recip(float x) {
+__device__ __forceinline__ float mx_exp(float a, float x) {  // e^(a x), a x <= 0, a constant
+  if constexpr (sizeof(T) == 2) return mx_ex2(a * kLog2e * x);
+  return expf(a * x);
+}
+template <typename T>
+__device__ __forceinline__ float mx_recip(float x) {  // 1 <= x <= 2 in fp32
   if constexpr (sizeof(T) == 2) {
     float r;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
   }
-  return 1.f / x;
+  return __fdividef(1.f, x);
 }
-__device__ __forceinline__ float mx_gelu_u(float x) { return kGeluK * (x + kGeluC * x * x * x); }
 
 template <typename T, int ACT>
 __device__ __forceinline__ float mx_f(float x) {
   if constexpr (ACT == IPC_ACT_RELU) {
     return x <= 0.f ? 0.f : x;
   } else if constexpr (ACT == IPC_ACT_GELU) {
-    if constexpr (sizeof(T) == 2) return x * sigmoid_hw(2.f * mx_gelu_u(x));
-    const float z = mx_exp<T>(-2.f * fabsf(mx_gelu_u(x)));
-    return x * (x >= 0.f ? 1.f : z) / (1.f + z);
+    if constexpr (sizeof(T) == 2) {
+      return x * mx_recip<T>(1.f + mx_ex2(x * fmaf(-kGelu3 * kLog2e, x * x, -kGelu1 * kLog2e)));  // (z of either sign)
+    }
+    const float z = mx_exp<T>(-1.f, fabsf(x) * fmaf(kGelu3, x * x, kGelu1));
+    return x * (x >= 0.f ? 1.f : z) * mx_recip<T>(1.f + z);
   } else if constexpr (sizeof(T) == 2) {
     return act_f_hw<ACT>(x);
   } else if constexpr (ACT == IPC_ACT_SIGMOID || ACT == IPC_ACT_SILU) {
@@ -138,15 +143,16 @@ __device__ __forceinline__ float mx_df(float x) {
   if constexpr (ACT == IPC_ACT_RELU) {
     return x > 0.f ? 1.f : x <= 0.f ? 0.f : x;
   } else if constexpr (ACT == IPC_ACT_TANH) {
-    const float z = mx_exp<T>(-2.f * fabsf(x)), r = mx_recip<T>(1.f + z);
+    const float z = mx_exp<T>(-2.f, fabsf(x)), r = mx_recip<T>(1.f + z);
     return 4.f * z * r * r;
   } else if constexpr (ACT == IPC_ACT_SIGMOID || ACT == IPC_ACT_SILU || ACT == IPC_ACT_GELU) {
-    const float z = mx_exp<T>(ACT == IPC_ACT_GELU ? -2.f * fabsf(mx_gelu_u(x)) : -fabsf(x)), r = mx_recip<T>(1.f + z);
-    const float d = z * r * r;
+    // (from |x| = 20 on z is 0, and 0 times the infinite square of a large x would be no number)
+    const float x2 = ACT == IPC_ACT_GELU ? fminf(x * x, 400.f) : 0.f;
+    const float z = ACT == IPC_ACT_GELU ? mx_exp<T>(-1.f, fabsf(x) * fmaf(kGelu3, x2, kGelu1)) : mx_exp<T>(-1.f, fabsf(x));
+    const float r = mx_recip<T>(1.f + z), zr = z * r, d = zr * r;
     if constexpr (ACT == IPC_ACT_SIGMOID) return d;
-    const float s = x >= 0.f ? r : z * r;
-    const float t = ACT == IPC_ACT_SILU ? x * d : 2.f * kGeluK * (1.f + 3.f * kGeluC * x * x) * x * d;
-    return z == 0.f ? s : s + t;  // (the square of a large x is infinite, and 0 times that no number)
+    const float s = x >= 0.f ? r : zr;
+    return fmaf(ACT == IPC_ACT_SILU ? x : x * fmaf(3.f * kGelu3, x2, kGelu1), d, s);
   } else {
     return act_df<ACT>(x);
   }
