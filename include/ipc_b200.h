@@ -393,7 +393,7 @@ int ipc_device_status(int* status, int clear);
  * IPC_NET_SYNC_BYTES of device memory.  No reference counterpart. */
 int ipc_selftest_barrier_timeout(void* sync, int limit_us, void* stream);
 
-/* Cap on the CTAs of the persistent tensor-core GEMM (max_ctas = 0: one per
+/* Cap on the CTAs of the persistent tensor-core GEMMs, 4-bit ones among them (max_ctas = 0: one per
  * SM, the default).  Its CTAs otherwise fill every SM, so a collective
  * launched beside it (the data-parallel path's NCCL all-reduce of the weight
  * deltas, issued while later layers' deltas are still being formed) waits for

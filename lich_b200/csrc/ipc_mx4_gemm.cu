@@ -3,7 +3,7 @@
 // The tensor core multiplies the 4-bit codes as they are stored and applies both scale bytes itself
 // (tcgen05.mma.kind::mxf4.block_scale): the products are exact and the sums fp32.
 //
-// One persistent CTA per SM walks output tiles of 128 x BN.  (CTA pairs, 256 x 256 tiles, were slower: 76 us against 69
+// One persistent CTA per SM (or as many as ipc_set_max_ctas leaves) walks output tiles of 128 x BN.  (CTA pairs, 256 x 256 tiles, were slower: 76 us against 69
 // at 4096 x 4096 x 8192 with tcgen05.cp, and 127 against 60 with the scale warps, whose signal then crosses SMs.)
 // Warp 0 loads K blocks of 256 columns (128 bytes a row, 128-byte swizzle) and their scale atoms with TMA into a
 // ring of stages; warps 10..13 put a stage's scale factors into tensor memory, each into its lane quarter; warp 1 issues the
@@ -25,6 +25,7 @@
 
 #include "ipc_mx.cuh"
 #include "ipc_ptx.cuh"
+#include "ipc_tc.cuh"
 
 namespace ipc {
 
@@ -505,15 +506,6 @@ int f_map_scales(CUtensorMap* map, const void* base, long long atoms, long long 
   return r == CUDA_SUCCESS ? IPC_OK : set_error(IPC_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
 }
 
-int f_sms() {
-  static int n[64] = {0};
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (dev < 0 || dev >= 64) return 148;
-  if (n[dev] == 0) cudaDeviceGetAttribute(&n[dev], cudaDevAttrMultiProcessorCount, dev);
-  return n[dev] > 0 ? n[dev] : 148;
-}
-
 template <typename T, int BN>
 int launch_tiles(const unsigned char* w, const unsigned char* wsc, const unsigned char* a, const unsigned char* asc,
                  void* out, int M, int K, int B, cudaStream_t s) {
@@ -539,7 +531,7 @@ int launch_tiles(const unsigned char* w, const unsigned char* wsc, const unsigne
   static_assert(SMEM <= 232448, "shared memory of a 4-bit product CTA");
   cudaError_t err = ensure_kernel_smem<mx4_gemm_kernel<T, BN>>(SMEM);
   if (err != cudaSuccess) return set_error(IPC_ERR_CUDA, "4-bit product smem attribute: %s", cudaGetErrorString(err));
-  const int sms = f_sms();
+  const int sms = grid_cap();
   mx4_gemm_kernel<T, BN><<<p.tiles < sms ? p.tiles : sms, F_THREADS, SMEM, s>>>(ta, tb, tsa, tsb, p);
   count_launch();
   return check_launch("4-bit product");
@@ -557,7 +549,7 @@ int launch_mx4_gemm(const unsigned char* w, const unsigned char* wsc, const unsi
                     void* out, int M, int K, int B, int dtype, cudaStream_t s) {
   // Tile width: every CTA takes ceil(tiles / SMs) tiles; a 128-column tile takes 0.75 of a 256-column tile's time
   // (4096 x 4096 x 8192: 14 rounds in 90 us against 7 in 60), so 256 columns unless 128 save a quarter of the rounds.
-  const long long sms = f_sms(), tm = (M + 127) / 128;
+  const long long sms = grid_cap(), tm = (M + 127) / 128;
   const long long w256 = (tm * ((B + 255) / 256) + sms - 1) / sms, w128 = (tm * ((B + 127) / 128) + sms - 1) / sms;
   const bool wide = B > 128 && 4 * w256 <= 3 * w128;
   IPC_DISPATCH_DT(dtype, TT, {

@@ -1020,11 +1020,14 @@ int num_sms() {
   return n[dev] > 0 ? n[dev] : 148;
 }
 
-// CTAs a persistent launch may use: every SM, or fewer while a caller leaves SMs to a collective.
+}  // namespace
+
 int grid_cap() {
   const int n = num_sms(), c = g_max_ctas.load(std::memory_order_relaxed);
   return (c > 0 && c < n) ? c : n;
 }
+
+namespace {
 
 // Split-K second pass: out = epilogue(sum over splits of the fp32 partials), summed in split order
 // (deterministic).  W: W = cast(W + scale * sum); WD: dw = (accumulate ? dw : 0) + scale * sum.

@@ -22,6 +22,8 @@ int launch_tc(const GemmArgs& p, int mode, int act, int dtype, cudaStream_t s, f
               size_t ws_bytes = 0, const TcTune* tune = nullptr);
 // Cap on the CTAs of a persistent tensor-core launch (0 = one per SM); see ipc_set_max_ctas.
 int set_max_ctas(int max_ctas);
+// CTAs a persistent tensor-core launch may use: every SM, or fewer while a caller leaves SMs to a collective.
+int grid_cap();
 // Device status word written by bounded waits (0 = fine); clear != 0 resets it.
 int read_device_status(int* status, int clear);
 // The same for the bounded grid barriers of the wide small-batch step kernel (ipc_widenet.cu).

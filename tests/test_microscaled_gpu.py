@@ -758,3 +758,38 @@ def test_slopes_of_very_large_states(act):
         mx.build_error_backward_checkpoint(1, 1, 256, act, NAME[dt])(w, e, c, s, up)
         want = (x > 0).float() if act in ("silu", "gelu") else torch.zeros(1, 256)
         assert torch.equal(up.cpu().float(), want)
+
+
+def test_forward_leaves_the_sms_it_is_told_to():
+    """Under a cap of 4 CTAs the 64 tiles take 16 rounds instead of one; the result is the same."""
+    from lich_b200 import _native as N
+    mx = _mx()
+    M = K = B = 1024
+    _, wq, wsc = X.quant4(_rand((M, K), 100))
+    _, aq, asc = X.quant4(_rand((B, K), 101))
+    args = [t.to(DEV) for t in (wq, wsc, aq, asc)]
+    k = mx.build_mxfp4_forward(M, K, B, "bfloat16")
+    outs, times = [], []
+    try:
+        for cap in (0, 4):
+            N.set_max_ctas(cap)
+            out = torch.empty(M, B, device=DEV, dtype=torch.bfloat16)
+            k(*args, out)
+            torch.cuda.synchronize()
+            g = torch.cuda.CUDAGraph()  # (200 calls one after another: the host would take longer than the GPU)
+            with torch.cuda.graph(g):
+                for _ in range(200):
+                    k(*args, out)
+            g.replay()
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            torch.cuda.synchronize()
+            a.record()
+            g.replay()
+            b.record()
+            torch.cuda.synchronize()
+            outs.append(out)
+            times.append(a.elapsed_time(b))
+    finally:
+        N.set_max_ctas(0)
+    assert torch.equal(*outs)
+    assert times[1] > 3 * times[0]
