@@ -22,6 +22,7 @@
 
 #include <cstring>
 #include <mutex>
+#include <type_traits>
 
 #include "ipc_mx.cuh"
 #include "ipc_ptx.cuh"
@@ -341,8 +342,9 @@ __global__ void __launch_bounds__(F_THREADS, 1)
 // A whole tile of the kernel above costs its set-up (8 us for a single sample) whatever it holds.  Here a warp owns 16
 // rows x 8 NB samples and a part of K; codes go from global memory to registers, are widened to fp16 (exact) and multiplied by
 // mma.sync a block of 32 columns at a time (two MMAs into zeros), and the block's sum c (up to 1152) is scaled into the fp32
-// accumulator, by the smaller of its two scales first: by the larger one a sum could overflow that the other brings back,
-// and c * 2^-127 is still exact (c a multiple of 1/4).  Which of a block's columns an MMA's k stands for is free as long
+// accumulator: (c * 2^sw) * 2^sa.  Where 2^sw is so large that this could overflow though 2^sa brings it back, the smaller
+// scale comes first (c * 2^-127 is still exact, c a multiple of 1/4; always doing so takes 4096 x 4096 x 1 from 7.4 us
+// to 7.9).  Which of a block's columns an MMA's k stands for is free as long
 // as both operands agree, so lane t of a quad takes 8 neighbouring columns: 4 bytes of each row.  The KW warps of a row block add up in
 // shared memory in warp order.  One read of W: 4096 x 4096 x 1 is 8.9 MB.
 constexpr int G_WARPS = 8;
@@ -353,10 +355,17 @@ __device__ __forceinline__ void g_mma(float (&c)[4], uint32_t a0, uint32_t a1, u
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// acc + c * 2^s0 * 2^s1 (positive floats compare as their bits do, NaN above all)
+// acc + c * 2^s0 * 2^s1; with LARGE the smaller scale first (positive floats compare as their bits do, NaN above all)
+template <bool LARGE>
 __device__ __forceinline__ float g_scaled(float acc, float c, float s0, float s1) {
   const uint32_t a = __float_as_uint(s0), b = __float_as_uint(s1);
-  return fmaf(c * __uint_as_float(min(a, b)), __uint_as_float(max(a, b)), acc);
+  if constexpr (LARGE) return fmaf(c * __uint_as_float(min(a, b)), __uint_as_float(max(a, b)), acc);
+  return fmaf(c * s0, s1, acc);
+}
+// whether one of four scale bytes is 240 (2^113) or more
+__device__ __forceinline__ bool g_large(uint32_t bytes) {
+  const uint32_t two = bytes & (bytes >> 1);
+  return (two & (two >> 2) & 0x10101010u) != 0;
 }
 // the four scale bytes of an atom's row (0 for a row past the operand: its codes are not read either)
 __device__ __forceinline__ uint32_t g_scales(const unsigned char* sc, int r, int rows, int atom, int atoms) {
@@ -404,26 +413,32 @@ __global__ void __launch_bounds__(32 * G_WARPS)
   if (part < atoms) fetch(cur, part);
   for (int at = part; at < atoms; at += kw) {
     if (at + kw < atoms) fetch(next, at + kw);  // the next atom's loads under this one's MMAs
+    auto atom = [&](auto large) {
+      constexpr bool LARGE = decltype(large)::value;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      uint32_t x0[4], x1[4];
-      mx4_unpack8(cur.cw[j][0], x0);
-      mx4_unpack8(cur.cw[j][1], x1);
-      const float f0 = mx_scale((cur.sw[0] >> (8 * j)) & 255u), f1 = mx_scale((cur.sw[1] >> (8 * j)) & 255u);
+      for (int j = 0; j < 4; ++j) {
+        uint32_t x0[4], x1[4];
+        mx4_unpack8(cur.cw[j][0], x0);
+        mx4_unpack8(cur.cw[j][1], x1);
+        const float f0 = mx_scale((cur.sw[0] >> (8 * j)) & 255u), f1 = mx_scale((cur.sw[1] >> (8 * j)) & 255u);
 #pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        uint32_t y[4];
-        mx4_unpack8(cur.ca[j][b], y);
-        float c[4] = {};
-        g_mma(c, x0[0], x1[0], x0[1], x1[1], y[0], y[1]);
-        g_mma(c, x0[2], x1[2], x0[3], x1[3], y[2], y[3]);
-        const float h0 = mx_scale((cur.sa[b][0] >> (8 * j)) & 255u), h1 = mx_scale((cur.sa[b][1] >> (8 * j)) & 255u);
-        acc[b][0] = g_scaled(acc[b][0], c[0], f0, h0);
-        acc[b][1] = g_scaled(acc[b][1], c[1], f0, h1);
-        acc[b][2] = g_scaled(acc[b][2], c[2], f1, h0);
-        acc[b][3] = g_scaled(acc[b][3], c[3], f1, h1);
+        for (int b = 0; b < NB; ++b) {
+          uint32_t y[4];
+          mx4_unpack8(cur.ca[j][b], y);
+          float c[4] = {};
+          g_mma(c, x0[0], x1[0], x0[1], x1[1], y[0], y[1]);
+          g_mma(c, x0[2], x1[2], x0[3], x1[3], y[2], y[3]);
+          const float h0 = mx_scale((cur.sa[b][0] >> (8 * j)) & 255u), h1 = mx_scale((cur.sa[b][1] >> (8 * j)) & 255u);
+          acc[b][0] = g_scaled<LARGE>(acc[b][0], c[0], f0, h0);
+          acc[b][1] = g_scaled<LARGE>(acc[b][1], c[1], f0, h1);
+          acc[b][2] = g_scaled<LARGE>(acc[b][2], c[2], f1, h0);
+          acc[b][3] = g_scaled<LARGE>(acc[b][3], c[3], f1, h1);
+        }
       }
-    }
+    };
+    // (the same for all lanes: an MMA is the whole warp's)
+    if (__any_sync(0xffffffffu, g_large(cur.sw[0]) || g_large(cur.sw[1]))) atom(std::true_type{});
+    else atom(std::false_type{});
     cur = next;
   }
   if (kw > 1) {
