@@ -69,6 +69,11 @@ __device__ __forceinline__ uint32_t group_max(uint32_t m) {
 }
 
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+// ... of f(x): relu leaves no sign bit (nor does the NaN that max.NaN gives)
+template <int ACT>
+__device__ __forceinline__ uint32_t f_bits(float v) {
+  return ACT == IPC_ACT_RELU ? __float_as_uint(v) : abs_bits(v);
+}
 
 // words of a later kernel's workspace, cleared by the first CTA
 __device__ __forceinline__ void zero_words(int* zero, int n) {
@@ -253,7 +258,7 @@ __global__ void __launch_bounds__(threads_of(VEC)) mx4_rows_kernel(const T* __re
       }
       uint32_t m = 0;
 #pragma unroll
-      for (int j = 0; j < N; ++j) m = max(m, abs_bits(v[j]));
+      for (int j = 0; j < N; ++j) m = max(m, f_bits<ACT>(v[j]));
       const uint32_t byte = mx4_scale_byte(group_max<MX_BLOCK / N>(m));
       if (c % MX_BLOCK == 0) s_scale[rr][(c - c0) / MX_BLOCK] = (unsigned char)byte;
       if (r < R && c < kp) {
@@ -282,7 +287,7 @@ __global__ void __launch_bounds__(threads_of(VEC)) mx4_rows_kernel(const T* __re
         const int c = c0 + MX_BLOCK * j + lane;
         if (ACT != IPC_ACT_RELU && ACT != IPC_ACT_IDENTITY) v[j] = (r < R && c < K) ? mx_f<float, ACT>(v[j]) : 0.f;
         else v[j] = mx_f<float, ACT>(v[j]);
-        const uint32_t byte = mx4_scale_byte(__reduce_max_sync(0xffffffffu, abs_bits(v[j])));
+        const uint32_t byte = mx4_scale_byte(__reduce_max_sync(0xffffffffu, f_bits<ACT>(v[j])));
         if (lane == 0) s_scale[rr][j] = (unsigned char)byte;
         const float lo = byte == MX_NAN_BYTE ? 0.f : v[j] * mx_inv_scale(byte);
         const float hi = __shfl_down_sync(0xffffffffu, lo, 1);
@@ -394,7 +399,7 @@ __global__ void __launch_bounds__(THREADS, turned_ctas(sizeof(T), ACT)) mx4_turn
       for (int i = 0; i < MX_BLOCK; ++i) {
         f[i] = mx_f<float, ACT>(St<T>::ld(v[i].v[h]));
         if (ACT == IPC_ACT_SIGMOID && !(in[h] && kb + i < K)) f[i] = 0.f;  // (the other f are 0 at 0)
-        top[h] = max(top[h], abs_bits(f[i]));
+        top[h] = max(top[h], f_bits<ACT>(f[i]));
       }
     }
     const uint32_t byte = mx4_scale_byte(top[h]);

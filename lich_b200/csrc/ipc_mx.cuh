@@ -118,7 +118,9 @@ __device__ __forceinline__ float mx_recip(float x) {  // 1 <= x <= 2 in fp32
 template <typename T, int ACT>
 __device__ __forceinline__ float mx_f(float x) {
   if constexpr (ACT == IPC_ACT_RELU) {
-    return x <= 0.f ? 0.f : x;
+    float y;  // (one instruction, where a comparison that lets NaN through takes two)
+    asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(y) : "f"(x));
+    return y;
   } else if constexpr (ACT == IPC_ACT_GELU) {
     if constexpr (sizeof(T) == 2) {
       return x * mx_recip<T>(1.f + mx_ex2(x * fmaf(-kGelu3 * kLog2e, x * x, -kGelu1 * kLog2e)));  // (z of either sign)
