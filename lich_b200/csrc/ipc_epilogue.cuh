@@ -30,8 +30,9 @@ __device__ __forceinline__ void epilogue(const GemmArgs& p, int g, int m, int n,
   } else if constexpr (MODE == MODE_G) {
     (reinterpret_cast<T*>(p.out) + g * p.gsOut)[idx] = St<T>::st(p.scale * acc);
   } else if constexpr (MODE == MODE_BK) {
-    const float x = (float)p.ck[(long long)m * p.ld_ck + n] * mx_scale(p.cks[(long long)(n / MX_BLOCK) * p.Mg + m]);
-    (reinterpret_cast<T*>(p.out) + g * p.gsOut)[idx] = St<T>::st(mx_df<T, ACT>(x) * acc);
+    const float step = mx_scale(p.cks[(long long)(n / MX_BLOCK) * p.Mg + m]);
+    (reinterpret_cast<T*>(p.out) + g * p.gsOut)[idx] =
+        St<T>::st(mx_df_code<T, ACT>((float)p.ck[(long long)m * p.ld_ck + n], step) * acc);
   } else if constexpr (MODE == MODE_F) {
     T* o = reinterpret_cast<T*>(p.out) + g * p.gsOut;
     o[idx] = St<T>::st(acc);

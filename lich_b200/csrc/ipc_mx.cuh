@@ -95,6 +95,11 @@ __device__ __forceinline__ void mx4_unpack8(uint32_t codes, uint32_t (&h)[4]) {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kGelu1 = 2.f * kGeluK, kGelu3 = 2.f * kGeluK * kGeluC;  // 2 u = x (kGelu1 + kGelu3 x^2)
 
+__device__ __forceinline__ float mx_max_nan(float x, float y) {  // NaN if either is
+  float m;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(x), "f"(y));
+  return m;
+}
 __device__ __forceinline__ float mx_ex2(float x) {
   float z;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(z) : "f"(x));
@@ -118,9 +123,7 @@ __device__ __forceinline__ float mx_recip(float x) {  // 1 <= x <= 2 in fp32
 template <typename T, int ACT>
 __device__ __forceinline__ float mx_f(float x) {
   if constexpr (ACT == IPC_ACT_RELU) {
-    float y;  // (one instruction, where a comparison that lets NaN through takes two)
-    asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(y) : "f"(x));
-    return y;
+    return mx_max_nan(x, 0.f);  // (one instruction, where a comparison that lets NaN through takes two)
   } else if constexpr (ACT == IPC_ACT_GELU) {
     if constexpr (sizeof(T) == 2) {
       return x * mx_recip<T>(1.f + mx_ex2(x * fmaf(-kGelu3 * kLog2e, x * x, -kGelu1 * kLog2e)));  // (z of either sign)
@@ -142,9 +145,7 @@ __device__ __forceinline__ float mx_f(float x) {
 }
 template <typename T, int ACT>
 __device__ __forceinline__ float mx_df(float x) {
-  if constexpr (ACT == IPC_ACT_RELU) {
-    return x > 0.f ? 1.f : x <= 0.f ? 0.f : x;
-  } else if constexpr (ACT == IPC_ACT_TANH) {
+  if constexpr (ACT == IPC_ACT_TANH) {
     const float z = mx_exp<T>(-2.f, fabsf(x)), r = mx_recip<T>(1.f + z);
     return 4.f * z * r * r;
   } else if constexpr (ACT == IPC_ACT_SIGMOID || ACT == IPC_ACT_SILU || ACT == IPC_ACT_GELU) {
@@ -157,6 +158,25 @@ __device__ __forceinline__ float mx_df(float x) {
     return fmaf(ACT == IPC_ACT_SILU ? x : x * fmaf(3.f * kGelu3, x2, kGelu1), d, s);
   } else {
     return act_df<ACT>(x);
+  }
+}
+
+// f'(c * 2^s) for the codes of a block: what depends on its step 2^s alone is the same for all of them (relu's NaN; the exponents of
+// tanh' and sigmoid', which take |c|, and tanh's 4 as the exponent's 2).
+template <typename T, int ACT>
+__device__ __forceinline__ float mx_df_code(float c, float step) {
+  if constexpr (ACT == IPC_ACT_RELU) {
+    return (c > 0.f ? 1.f : 0.f) + step * 0.f;
+  } else if constexpr (sizeof(T) == 2 && (ACT == IPC_ACT_TANH || ACT == IPC_ACT_SIGMOID)) {
+    const float a = mx_max_nan((ACT == IPC_ACT_TANH ? -2.f : -1.f) * kLog2e * step, -3e38f);  // (0 times infinity is no number)
+    if constexpr (ACT == IPC_ACT_TANH) {
+      const float z4 = mx_ex2(fmaf(fabsf(c), a, 2.f)), r = mx_recip<T>(fmaf(0.25f, z4, 1.f));
+      return z4 * r * r;
+    }
+    const float z = mx_ex2(fabsf(c) * a), r = mx_recip<T>(1.f + z);
+    return z * r * r;
+  } else {
+    return mx_df<T, ACT>(c * step);
   }
 }
 

@@ -219,8 +219,8 @@ __global__ void __launch_bounds__(BTHREADS) mx8_columns_kernel(const __grid_cons
     for (int c = 0; c + 1 < C; ++c) sum += other[c * BC * NB + i];
     const int k = c0 + i / NB, b = i % NB;
     if (k < p.Mg && b < B) {
-      const float x = (float)p.ck[(long long)k * p.ld_ck + b] * mx_scale(p.cks[k]);
-      reinterpret_cast<T*>(p.out)[(long long)k * B + b] = St<T>::st(mx_df<T, ACT>(x) * sum);
+      const float f = mx_df_code<T, ACT>((float)p.ck[(long long)k * p.ld_ck + b], mx_scale(p.cks[k]));
+      reinterpret_cast<T*>(p.out)[(long long)k * B + b] = St<T>::st(f * sum);
     }
   }
 }

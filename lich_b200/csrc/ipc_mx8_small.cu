@@ -287,8 +287,9 @@ __global__ void __launch_bounds__(STHREADS) mx8_small_kernel(const __grid_consta
       const int m = m0 + wm * 16 + gq + (r >= 2 ? 8 : 0), n = n0 + wn * 32 + 8 * j + 2 * tq + (r & 1);
       if (m < p.Mg && n < p.Ng) {
         if constexpr (BKM) {
-          const float x = (float)(signed char)(code2[j][r >> 1] >> (8 * (r & 1))) * mx_scale(sbyte[r >> 1]);
-          reinterpret_cast<T*>(p.out)[(long long)m * p.Ng + n] = St<T>::st(mx_df<T, ACT>(x) * acc[j][r]);
+          const float c = (float)(signed char)(code2[j][r >> 1] >> (8 * (r & 1)));
+          reinterpret_cast<T*>(p.out)[(long long)m * p.Ng + n] =
+              St<T>::st(mx_df_code<T, ACT>(c, mx_scale(sbyte[r >> 1])) * acc[j][r]);
         } else {
           epilogue<T, IPC_ACT_IDENTITY, MODE>(p, 0, m, n, acc[j][r]);
         }

@@ -311,7 +311,7 @@ __device__ __forceinline__ uint4 epi_vec_bk(const uint4& codes, int half, float 
   uint4 o;
   T* oh = reinterpret_cast<T*>(&o);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) oh[j] = St<T>::st(mx_df<T, ACT>(c[j] * step) * __uint_as_float(acc8[j]));
+  for (int j = 0; j < 8; ++j) oh[j] = St<T>::st(mx_df_code<T, ACT>(c[j], step) * __uint_as_float(acc8[j]));
   return o;
 }
 // ... and the coalesced pass stores it and cast(f(x)) of the stored x (the A_out of the forward sweep)
