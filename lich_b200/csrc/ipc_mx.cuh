@@ -100,6 +100,11 @@ __device__ __forceinline__ float mx_max_nan(float x, float y) {  // NaN if eithe
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(x), "f"(y));
   return m;
 }
+__device__ __forceinline__ float mx_min_nan(float x, float y) {
+  float m;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(x), "f"(y));
+  return m;
+}
 __device__ __forceinline__ float mx_ex2(float x) {
   float z;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(z) : "f"(x));

@@ -99,7 +99,7 @@ __device__ __forceinline__ uint4 shifted(const Row8<VEC>& r, int left) {
 }
 
 // Whether f(x^) is kept in two parts: relu and identity give c * 2^s, which 16 bits hold (below fp16's smallest normal
-// number to within half its smallest step).
+// number to within half its smallest step; 2^16, which fp16 states above 65024 read back as, is its infinity).
 __host__ __device__ constexpr bool s_low(int act, int mode) {
   return mode != MODE_BK && act != IPC_ACT_RELU && act != IPC_ACT_IDENTITY;
 }
@@ -189,7 +189,9 @@ __global__ void __launch_bounds__(STHREADS) mx8_small_kernel(const __grid_consta
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           const float f = in && k0 + c + e < k_hi ? mx_f<T, ACT>(q[e] * sc) : 0.f;
-          h[e] = St<T>::st(f);
+          // (states up to 2^16 read back from fp16, whose largest number is 65504: the rest goes to the second part)
+          constexpr bool OVER = std::is_same<T, __half>::value && (ACT == IPC_ACT_SILU || ACT == IPC_ACT_GELU);
+          h[e] = St<T>::st(OVER ? mx_min_nan(f, 65504.f) : f);
           if constexpr (LOW) lo[e] = St<T>::st(f - St<T>::ld(h[e]));
         }
         uint4* dst = reinterpret_cast<uint4*>(b + r * LDB + c);

@@ -793,3 +793,27 @@ def test_forward_leaves_the_sms_it_is_told_to():
         N.set_max_ctas(0)
     assert torch.equal(*outs)
     assert times[1] > 3 * times[0]
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("M,K,B", [(40, 72, 200), (33, 65, 97), (20, 30, 3)])
+def test_largest_half_precision_states(M, K, B, act):
+    """65504 reads back as 64 * 2^10, which fp16 does not hold: where f(x^) is kept in two parts or in fp32 the products stay
+    finite, and the bounds are the usual ones."""
+    from lich_b200.tilelang_kernels import KernelConfig
+    mx = _mx()
+    dt = torch.float16
+    x = _rand((K, B), 110, 1.0, dt)
+    x[3] = 65504
+    x[4, ::2] = -65504
+    c, s = _ckpt(x)
+    xhat = X.load8(c.cpu(), s.cpu(), B)
+    assert xhat.max() == 65536
+    e = _rand((M, B), 111, 0.01, dt)
+    a = O.act_forward(act, xhat)
+    ref, S = e.double() @ a.t(), e.double().abs() @ a.abs().t()
+    err = (e.double().abs() @ (_act_err(act, xhat, dt) + U[dt] * a.abs() + TINY[dt]).t()) * (1 + 2.0 ** -8) + S * B * 2.0 ** -23
+    dw = torch.zeros(M, K, device=DEV)
+    backend = "auto" if B <= 4 else "simt"
+    mx.build_weight_delta_checkpoint(M, K, B, act, "float16", 1.0, "float32", KernelConfig(backend=backend))(dw, e.to(DEV), c, s)
+    _within(dw, ref, err + 2.0 ** -23 * ref.abs())
