@@ -424,10 +424,16 @@ int ipc_fused_gemm_ws(int mode, const void* a, const void* b, void* out, const v
 }
 
 // ------------------------------------------------------------- microscaled operands (ipc_mx.cuh)
+// ... whose sizes, rounded up to whole blocks and tiles, have to stay in 32 bits
+static int mx_checks(int M, int K, int B, int act, int dtype, int algo) {
+  constexpr int most = 0x7fffffff - 511;
+  IPC_REQUIRE(M <= most && K <= most && B <= most, "size above %d (%d, %d, %d)", most, M, K, B);
+  return common_checks(M, K, B, 1, act, dtype, algo);
+}
 static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 int ipc_mx8_store(const void* x, signed char* codes, unsigned char* scales, int D, int B, int dtype, void* stream) {
-  int rc = common_checks(D, 1, B, 1, IPC_ACT_IDENTITY, dtype, IPC_ALGO_AUTO);
+  int rc = mx_checks(D, 1, B, IPC_ACT_IDENTITY, dtype, IPC_ALGO_AUTO);
   if (rc) return rc;
   if (D == 0 || B == 0) return IPC_OK;
   IPC_REQUIRE(x && codes && scales, "null operand pointer");
@@ -437,7 +443,7 @@ int ipc_mx8_store(const void* x, signed char* codes, unsigned char* scales, int 
 
 int ipc_mx8_restore(const signed char* codes, const unsigned char* scales, void* out, int D, int B, int act, int dtype,
                     void* stream) {
-  int rc = common_checks(D, 1, B, 1, act, dtype, IPC_ALGO_AUTO);
+  int rc = mx_checks(D, 1, B, act, dtype, IPC_ALGO_AUTO);
   if (rc) return rc;
   if (D == 0 || B == 0) return IPC_OK;
   IPC_REQUIRE(codes && scales && out, "null operand pointer");
@@ -494,7 +500,7 @@ static Mx8WeightWs mx8_weight_ws(int mode, int M, int K, int B, int dtype, int a
 }
 
 int ipc_mx8_weight_ws_bytes(int mode, int M, int K, int B, int dtype, int algo, size_t* bytes) {
-  int rc = common_checks(M, K, B, 1, IPC_ACT_IDENTITY, dtype, algo);
+  int rc = mx_checks(M, K, B, IPC_ACT_IDENTITY, dtype, algo);
   if (rc) return rc;
   IPC_REQUIRE(mode == IPC_MODE_WEIGHT || mode == IPC_MODE_WDELTA || mode == IPC_MODE_WGRAD, "not a weight mode: %d", mode);
   IPC_REQUIRE(bytes != nullptr, "null result pointer");
@@ -505,7 +511,7 @@ int ipc_mx8_weight_ws_bytes(int mode, int M, int K, int B, int dtype, int algo, 
 int ipc_mx8_weight(int mode, void* out, const void* e, const signed char* codes, const unsigned char* scales, int M,
                    int K, int B, float scale, int flags, int act, int dtype, int algo, void* workspace,
                    size_t workspace_bytes, void* stream) {
-  int rc = common_checks(M, K, B, 1, act, dtype, algo);
+  int rc = mx_checks(M, K, B, act, dtype, algo);
   if (rc) return rc;
   IPC_REQUIRE(mode == IPC_MODE_WEIGHT || mode == IPC_MODE_WDELTA || mode == IPC_MODE_WGRAD, "not a weight mode: %d", mode);
   IPC_REQUIRE((flags & ~IPC_FLAG_ACCUMULATE) == 0, "only IPC_FLAG_ACCUMULATE applies (flags = %d)", flags);
@@ -577,7 +583,7 @@ static size_t mx8_backward_ws(int M, int K, int B, int dtype, int algo, size_t* 
 }
 
 int ipc_mx8_backward_ws_bytes(int M, int K, int B, int dtype, int algo, size_t* bytes) {
-  int rc = common_checks(M, K, B, 1, IPC_ACT_IDENTITY, dtype, algo);
+  int rc = mx_checks(M, K, B, IPC_ACT_IDENTITY, dtype, algo);
   if (rc) return rc;
   IPC_REQUIRE(bytes != nullptr, "null result pointer");
   size_t w;
@@ -588,7 +594,7 @@ int ipc_mx8_backward_ws_bytes(int M, int K, int B, int dtype, int algo, size_t* 
 int ipc_mx8_backward(void* e_up, const void* w, const void* e, const signed char* codes, const unsigned char* scales,
                      int M, int K, int B, int act, int dtype, int algo, void* workspace, size_t workspace_bytes,
                      void* stream) {
-  int rc = common_checks(M, K, B, 1, act, dtype, algo);
+  int rc = mx_checks(M, K, B, act, dtype, algo);
   if (rc) return rc;
   IPC_REQUIRE(algo != IPC_ALGO_OUTER, "IPC_ALGO_OUTER applies to the weight update only");
   if (K == 0 || B == 0) return IPC_OK;
@@ -625,7 +631,7 @@ int ipc_mx8_backward(void* e_up, const void* w, const void* e, const signed char
 
 int ipc_mxfp4_quantize(const void* x, unsigned char* codes, unsigned char* scales, int R, int K, int turned, int act,
                        int dtype, void* stream) {
-  int rc = common_checks(R, K, 1, 1, act, dtype, IPC_ALGO_AUTO);
+  int rc = mx_checks(R, K, 1, act, dtype, IPC_ALGO_AUTO);
   if (rc) return rc;
   if (R == 0 || K == 0) return IPC_OK;
   IPC_REQUIRE(x && codes && scales, "null operand pointer");
@@ -635,7 +641,7 @@ int ipc_mxfp4_quantize(const void* x, unsigned char* codes, unsigned char* scale
 
 int ipc_mxfp4_restore(const unsigned char* codes, const unsigned char* scales, void* out, int R, int K, int dtype,
                       void* stream) {
-  int rc = common_checks(R, K, 1, 1, IPC_ACT_IDENTITY, dtype, IPC_ALGO_AUTO);
+  int rc = mx_checks(R, K, 1, IPC_ACT_IDENTITY, dtype, IPC_ALGO_AUTO);
   if (rc) return rc;
   if (R == 0 || K == 0) return IPC_OK;
   IPC_REQUIRE(codes && scales && out, "null operand pointer");
@@ -645,7 +651,7 @@ int ipc_mxfp4_restore(const unsigned char* codes, const unsigned char* scales, v
 
 int ipc_mxfp4_forward(const unsigned char* w, const unsigned char* w_scales, const unsigned char* a,
                       const unsigned char* a_scales, void* out, int M, int K, int B, int dtype, void* stream) {
-  int rc = common_checks(M, K, B, 1, IPC_ACT_IDENTITY, dtype, IPC_ALGO_AUTO);
+  int rc = mx_checks(M, K, B, IPC_ACT_IDENTITY, dtype, IPC_ALGO_AUTO);
   if (rc) return rc;
   if (M == 0 || B == 0) return IPC_OK;
   IPC_REQUIRE(out && (K == 0 || (w && w_scales && a && a_scales)), "null operand pointer");

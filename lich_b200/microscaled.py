@@ -67,6 +67,7 @@ _scratch: weakref.WeakValueDictionary = weakref.WeakValueDictionary()
 _ws_lock = threading.Lock()
 
 BLOCK = 32
+MAX_SIZE = 2 ** 31 - 512  # of a row or a column: the C entries' sizes, padded to whole tiles, are 32-bit integers
 # what torch.cuda.current_device() and current_stream().cuda_stream come down to, at a tenth of their cost
 _current_device, _current_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
@@ -362,6 +363,8 @@ def _builder(build):
 def _validate(*sizes, activation="identity", dtype):
     if min(int(n) for n in sizes) < 0:
         raise ValueError(f"negative size in {sizes}")
+    if max(int(n) for n in sizes) > MAX_SIZE:
+        raise ValueError(f"a size in {sizes} is above {MAX_SIZE}")
     N.act_code(activation)
     N.dtype_code(N.torch_dtype(dtype))
 

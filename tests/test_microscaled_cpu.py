@@ -114,3 +114,30 @@ def test_the_call_layer_hands_everything_unusual_to_the_operator():
     with pytest.raises(ValueError):
         mx._Call(object(), 0, 0, [], (), 0.0)
     assert mx.build_mxfp4_forward(4, 5, 6, dtype="float16") is mx.build_mxfp4_forward(4, 5, 6, dtype="float16")
+
+
+def test_sizes_beyond_31_bits_are_refused():
+    """The C entries take 32-bit sizes: a larger one would be cut to its low bits and a part of the tensor worked on."""
+    from lich_b200 import _native as N
+    from lich_b200 import microscaled as mx
+    for n in (2 ** 32 + 32, 2 ** 31, 2 ** 31 - 1):
+        for build in (lambda: mx.build_checkpoint(1, n, "float16"), lambda: mx.build_checkpoint(n, 1, "float16"),
+                      lambda: mx.build_checkpoint_restore(1, n, "tanh", "float16"),
+                      lambda: mx.build_weight_update_checkpoint(1, 1, n, "tanh", "float16", 0.1),
+                      lambda: mx.build_weight_delta_checkpoint(n, 1, 1, "tanh", "float16", 0.1),
+                      lambda: mx.build_error_backward_checkpoint(1, n, 1, "tanh", "float16"),
+                      lambda: mx.build_mxfp4_quantize(1, n, "tanh", "float16"),
+                      lambda: mx.build_mxfp4_restore(n, 1, "float16"), lambda: mx.build_mxfp4_forward(1, 1, n, "float16")):
+            with pytest.raises(ValueError, match="size"):
+                build()
+    lib, big, A = N.load(), 2 ** 31 - 1, N.IPC_ERR_ARG
+    assert lib.ipc_mx8_store(None, None, None, 4, big, 1, None) == A
+    assert lib.ipc_mx8_restore(None, None, None, big, 4, 0, 1, None) == A
+    assert lib.ipc_mx8_weight(3, None, None, None, None, 4, big, 4, 1.0, 0, 0, 1, 0, None, 0, None) == A
+    assert lib.ipc_mx8_backward(None, None, None, None, None, 4, 4, big, 0, 1, 0, None, 0, None) == A
+    assert lib.ipc_mxfp4_quantize(None, None, None, 4, big, 0, 0, 1, None) == A
+    assert lib.ipc_mxfp4_restore(None, None, None, big, 4, 1, None) == A
+    assert lib.ipc_mxfp4_forward(None, None, None, None, None, 4, big, 4, 1, None) == A
+    n = ctypes.c_size_t(0)
+    assert lib.ipc_mx8_weight_ws_bytes(3, 4, 4, big, 1, 0, ctypes.byref(n)) == A
+    assert lib.ipc_mx8_backward_ws_bytes(big, 4, 4, 1, 0, ctypes.byref(n)) == A
