@@ -6,7 +6,8 @@ Blocks of 32 numbers share one power of two (formats and layouts: ``include/ipc_
 dtype that writes its output tensors in place on the current CUDA stream, raises ``ValueError`` for tensors of another
 shape, dtype, device or layout before anything is launched, and holds (per device and stream) whatever workspace it
 needs.  Large products with a checkpoint need one of the size of the states in 16 bits; a program that runs many of them in
-order passes one buffer of its own instead: ``kernel(..., workspace=buffer)``, ``kernel.workspace_bytes()`` long.
+order passes one buffer of its own instead: ``kernel(..., workspace=buffer)``, ``kernel.workspace_bytes()`` long.  Of a
+``KernelConfig`` these products follow ``backend`` (auto, simt, tcgen05) and refuse the rest.
 
     codes, scales = empty_checkpoint(D, B, device=dev)                       # states x [D, B] kept in 8 bits
     build_checkpoint(D, B, "bfloat16")(x, codes, scales)
@@ -369,6 +370,17 @@ def _validate(*sizes, activation="identity", dtype):
     N.dtype_code(N.torch_dtype(dtype))
 
 
+def _backend(cfg: KernelConfig, dtype) -> None:
+    """Refuse what a checkpoint product could only ignore."""
+    algo = _algo(cfg)
+    if algo == N.ALGO_CODES["outer"]:
+        raise ValueError("no outer-product kernel reads checkpoints: backend must be auto, simt or tcgen05")
+    if algo == N.ALGO_CODES["tcgen05"] and N.torch_dtype(dtype) is torch.float32:
+        raise ValueError("the tensor cores take 16-bit storage: backend tcgen05 is not for float32")
+    if cfg.tune() is not None:
+        raise ValueError("checkpoint products choose their own tiles, splits and CTAs: of cfg only backend applies (tc_* = 0)")
+
+
 @_builder
 def build_checkpoint(D: int, B: int, dtype: str):
     """``kernel(x [D, B], codes, scales)``: the states in 8 bits."""
@@ -388,6 +400,7 @@ def build_weight_update_checkpoint(M: int, K: int, B: int, activation: str, dtyp
                                    cfg: KernelConfig = KernelConfig()):
     """``kernel(w [M, K], e [M, B], codes, scales)``: ``W += alpha * E @ f(x^)^T`` in place."""
     _validate(M, K, B, activation=activation, dtype=dtype)
+    _backend(cfg, dtype)
     return CheckpointWeightKernel(N.MODE_WEIGHT, M, K, B, activation, dtype, alpha, N.torch_dtype(dtype), cfg)
 
 
@@ -397,6 +410,7 @@ def build_weight_delta_checkpoint(M: int, K: int, B: int, activation: str, dtype
     """``kernel(dw [M, K], e [M, B], codes, scales, accumulate=False)``: ``dw = alpha * E @ f(x^)^T``, in float32 (which
     alone can accumulate) or in ``dtype``."""
     _validate(M, K, B, activation=activation, dtype=dtype)
+    _backend(cfg, dtype)
     out = N.torch_dtype(delta_dtype)
     if out is not torch.float32 and out is not N.torch_dtype(dtype):
         raise ValueError(f"a weight delta is kept in float32 or in {dtype}, not in {delta_dtype}")
@@ -409,6 +423,7 @@ def build_error_backward_checkpoint(M: int, K: int, B: int, activation: str, dty
                                     cfg: KernelConfig = KernelConfig()):
     """``kernel(w [M, K], e [M, B], codes, scales, e_up [K, B])``: ``e_up = f'(x^) * (W^T @ E)``."""
     _validate(M, K, B, activation=activation, dtype=dtype)
+    _backend(cfg, dtype)
     return CheckpointBackwardKernel(M, K, B, activation, dtype, cfg)
 
 

@@ -141,3 +141,22 @@ def test_sizes_beyond_31_bits_are_refused():
     n = ctypes.c_size_t(0)
     assert lib.ipc_mx8_weight_ws_bytes(3, 4, 4, big, 1, 0, ctypes.byref(n)) == A
     assert lib.ipc_mx8_backward_ws_bytes(big, 4, 4, 1, 0, ctypes.byref(n)) == A
+
+
+def test_configs_that_a_checkpoint_product_cannot_follow_are_refused():
+    """"outer" has no kernel that reads checkpoints, and fp32 storage none on the tensor cores; tile, split and CTA overrides
+    would be dropped."""
+    from lich_b200 import microscaled as mx
+    from lich_b200.tilelang_kernels import KernelConfig
+    for build in (lambda dt, cfg: mx.build_weight_update_checkpoint(8, 8, 8, "tanh", dt, 0.1, cfg),
+                  lambda dt, cfg: mx.build_weight_delta_checkpoint(8, 8, 8, "tanh", dt, 0.1, "float32", cfg),
+                  lambda dt, cfg: mx.build_error_backward_checkpoint(8, 8, 8, "tanh", dt, cfg)):
+        for backend in ("auto", "simt", "generic", "tcgen05"):
+            build("bfloat16", KernelConfig(backend=backend))
+        build("float32", KernelConfig(64, 128, 16, 128, 2, True, 8, False))  # the reference's tile fields mean nothing here
+        for dt, cfg in (("bfloat16", KernelConfig(backend="outer")), ("float32", KernelConfig(backend="tcgen05")),
+                        ("bfloat16", KernelConfig(tc_bn=128)), ("bfloat16", KernelConfig(tc_splits=2)),
+                        ("bfloat16", KernelConfig(tc_raster=4)), ("bfloat16", KernelConfig(tc_max_ctas=64)),
+                        ("bfloat16", KernelConfig(tc_pair=1)), ("bfloat16", KernelConfig(backend="nothing"))):
+            with pytest.raises(ValueError):
+                build(dt, cfg)
