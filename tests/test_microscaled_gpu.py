@@ -817,3 +817,58 @@ def test_largest_half_precision_states(M, K, B, act):
     backend = "auto" if B <= 4 else "simt"
     mx.build_weight_delta_checkpoint(M, K, B, act, "float16", 1.0, "float32", KernelConfig(backend=backend))(dw, e.to(DEV), c, s)
     _within(dw, ref, err + 2.0 ** -23 * ref.abs())
+
+
+@pytest.mark.parametrize("threads", [False, True])
+@pytest.mark.parametrize("M,K,B", [(256, 512, 4096), (130, 259, 1029)])
+def test_streams_with_workspaces_do_not_meet(M, K, B, threads):
+    """One operator whose calls need a workspace, on three streams at once with inputs of their own, from one thread or one
+    each: what each stream computes is what it computes alone."""
+    import threading
+
+    from lich_b200.tilelang_kernels import KernelConfig
+    mx = _mx()
+    cfg = KernelConfig(backend="tcgen05")
+    k = mx.build_weight_delta_checkpoint(M, K, B, "silu", "bfloat16", 1.0, "float32", cfg)
+    kb = mx.build_error_backward_checkpoint(M, K, B, "silu", "bfloat16", cfg)
+    assert k.workspace_bytes() > 0 and (kb.workspace_bytes() > 0) == (B % 8 != 0)
+    w = _rand((M, K), 120, 0.1, torch.bfloat16).to(DEV)
+    given = [(_rand((M, B), 121 + i, 0.3, torch.bfloat16).to(DEV), *_ckpt(_rand((K, B), 131 + i, 1.5, torch.bfloat16)))
+             for i in range(3)]
+
+    def run(e, c, s, dw, up):
+        k(dw, e, c, s)
+        kb(w, e, c, s, up)
+
+    def empty():
+        return torch.empty(M, K, device=DEV), torch.empty(K, B, device=DEV, dtype=torch.bfloat16)
+
+    alone = [empty() for _ in given]
+    for g, o in zip(given, alone):
+        run(*g, *o)
+        torch.cuda.synchronize()
+    e, c, s = given[0]
+    a = O.act_forward("silu", X.load8(c.cpu(), s.cpu(), B))
+    S = e.cpu().double().abs() @ a.abs().t()
+    _within(alone[0][0], e.cpu().double() @ a.t(), S * (2.0 ** -8 + B * 2.0 ** -23))
+    streams = [torch.cuda.Stream(DEV) for _ in given]
+    outs = [[empty() for _ in range(20)] for _ in given]
+    torch.cuda.synchronize()
+
+    def work(i, n):
+        with torch.cuda.stream(streams[i]):
+            for o in outs[i][n:n + 1] if n is not None else outs[i]:
+                run(*given[i], *o)
+
+    if threads:
+        ts = [threading.Thread(target=work, args=(i, None)) for i in range(3)]
+        [t.start() for t in ts]
+        [t.join() for t in ts]
+    else:
+        for n in range(20):
+            for i in range(3):
+                work(i, n)
+    torch.cuda.synchronize()
+    for want, got in zip(alone, outs):
+        for dw, up in got:
+            assert torch.equal(dw, want[0]) and torch.equal(up, want[1])
