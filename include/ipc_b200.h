@@ -320,7 +320,10 @@ int ipc_weight_update_opt(void* w, const void* e, const void* x_up, int M, int K
  *           nearest of +-{0, 0.5, 1, 1.5, 2, 3, 4, 6} (ties to the even code; bit 3
  *           of a code is the sign, bits 0-2 the place in this list).
  * A block that holds an infinity or a NaN is kept as codes 0 with the scale
- * byte 255 and reads back as NaN.
+ * byte 255 and reads back as NaN; f of it is NaN, relu's too, and so is f'
+ * (identity's is 1).  A checkpoint of fp16 states above 65024 may stand for 2^16,
+ * which fp16 holds as infinity.  Sizes go up to 2^31 - 512; the kernels that
+ * store and restore take up to 2097120 rows (IPC_ERR_ARG above).
  *
  * 8-bit checkpoint of states x [D, B], blocks along the batch:
  *   codes  [D, 32 ceil(B/32)] int8 (16-byte aligned; padding is 0)
@@ -345,10 +348,15 @@ int ipc_mx8_restore(const signed char* codes, const unsigned char* scales, void*
  *   IPC_MODE_WGRAD   out = cast(scale * E @ A^T) in `dtype`
  * The workspace (16-byte aligned; *_ws_bytes gives its size, which may be 0) need
  * not be initialised; calls that share one must be ordered on one stream.
- * IPC_ALGO_AUTO runs large products on the tcgen05 GEMMs (f(x^) rounded to
- * `dtype`), a few samples in fp32 FMAs, and the rest, of any size and alignment,
- * in one launch of an mma.sync kernel that keeps f(x^) in two parts
- * (IPC_ALGO_SIMT asks for it); fp32 storage otherwise runs on the generic kernel.
+ * IPC_ALGO_AUTO runs large products (from about 1e8 multiply-adds) on the tcgen05
+ * GEMMs, a few samples in fp32 FMAs, and the rest, of any size and alignment, in
+ * one launch of an mma.sync kernel that keeps f(x^) in two parts (IPC_ALGO_SIMT
+ * asks for it); fp32 storage otherwise runs on the generic kernel.
+ * The tcgen05 GEMMs round f(x^) to `dtype`, whatever the result's type: a sum there
+ * is off by about that rounding, while the other kernels' are near fp32's.  They
+ * take tensors on 16-byte boundaries: an e, w or in-place out that starts between
+ * them (rows of another length do not matter) goes to the mma.sync kernel, many
+ * times slower for large products.
  * IPC_ALGO_OUTER is IPC_ERR_ARG.
  */
 #define IPC_MODE_WGRAD 6

@@ -1,4 +1,5 @@
-// Products with an 8-bit checkpoint of a few samples, in fp32 FMAs (nothing but the result is rounded):
+// Products with an 8-bit checkpoint of a few samples, in fp32 FMAs (f and f' of ipc_mx.cuh in fp32, off by 2^-20 of themselves,
+// tanh in 16-bit storage by 2^-11; the result is rounded once):
 //   W, WD, G   (up to 16) out[m][k] from sum_b E[m][b] f(x^[k][b]): bound by writing (W: reading and writing) M x K numbers.
 //              A CTA takes 64 x 256 of them, with its 256 states' f and its 64 errors' rows in shared memory.
 //   BK         (up to 4) out[k][b] = f'(x^[k][b]) sum_m W[m][k] E[m][b]: bound by one read of W.  A CTA takes 64 columns of

@@ -7,7 +7,8 @@
 // walks the reduction in steps of 64, the next step's operands in registers while mma.sync works on this one's in shared
 // memory.  The states are read as codes and f is applied on the way to shared memory: no restored copy, no second launch,
 // and where f(x^) does not fit 16 bits, a second operand holds what the first rounds off: the MMAs are idle anyway, and
-// the sum then has fp32's accuracy (the rounding of f would be as large as the result's own).
+// the sum then is as accurate as f itself, 2^-20 for sigmoid, silu and gelu, 2^-11 for tanh (tanh.approx: as much as
+// fp16's rounding, an eighth of bf16's), instead of a rounding of f as large as the result's own.
 // A long reduction with few tiles is split over the CTAs of a cluster, whose partial sums meet in the first CTA's
 // shared memory and are added in rank order (deterministic).
 #include "ipc_epilogue.cuh"
